@@ -293,6 +293,72 @@ int i8l_dequant_i32(const int32_t *acc, int64_t lda, const float *sa, int32_t sa
                     int32_t bias_dtype, void *out, int32_t out_dtype, int64_t ldo,
                     int32_t M, int32_t N, void *stream);
 
+/* ---- 4-bit operands (MXFP4) ------------------------------------------------------
+ * Blocks of 32 consecutive values along K: each value an e2m1 code (0, 0.5, 1, 1.5, 2, 3,
+ * 4, 6, bit 3 the sign), each block one e8m0 scale byte b for 2^(b-127), 0xFF for NaN.
+ *
+ *   codes   row r at q + r*ldq bytes, value 2j in the low, 2j+1 in the high nibble of
+ *           byte j; ldq >= K/2
+ *   scales  tiles of 128 rows x 4 blocks, 512 bytes each: the byte of (row r, block b) is
+ *           at ((r/128)*ceil(K/128) + b/4)*512 + (r%32)*16 + ((r/32)%4)*4 + b%4.
+ *           i8l_mxfp4_scale_bytes(rows, K) bytes in all; the quantisers write every one,
+ *           0 past the last row or block.
+ *
+ * A block's scale is 2^(floor(log2 max|y|) - 2), at least 2^-127; its values are
+ * y / scale rounded to nearest (ties to even) and saturated at +-6.  A block of zeros has
+ * byte 0; a block that holds an infinity or a NaN has byte 0xFF and zero codes, so
+ * everything made of it is NaN.  K must be a multiple of 32, at most 2^26.
+ * No reference counterpart: the reference's linears are int8.
+ */
+size_t i8l_mxfp4_scale_bytes(int32_t rows, int32_t K);
+
+/* Block-quantises x[M,K] (dtype I8L_BF16/F16/F32, rows ldx elements apart; a column slice
+ * or any alignment is fine).  For activations and for weights ([N,K]). */
+int i8l_quant_mxfp4(const void *x, int64_t ldx, int32_t dtype, uint8_t *q, int64_t ldq,
+                    uint8_t *scale, int32_t M, int32_t K, void *stream);
+
+/* y = silu(gate) * up of [gate | up] rows of 2I values, block-quantised: the product is
+ * rounded to float32 and then to act_dtype (I8L_BF16/F16), both as if computed exactly. */
+int i8l_silu_mul_quant_mxfp4(const void *gate_up, int64_t ld, int32_t act_dtype, uint8_t *q,
+                             int64_t ldq, uint8_t *scale, int32_t M, int32_t I, void *stream);
+
+/* add + RMSNorm, block-quantised: i8l_add_rmsnorm_quant's y with 1/sqrt(mean + eps)
+ * rounded once from float64.  residual and rout may be NULL together. */
+int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                                const void *weight, int32_t act_dtype, int32_t w_dtype,
+                                uint8_t *q, int64_t ldq, uint8_t *scale, void *rout,
+                                int64_t ldro, int32_t M, int32_t K, double eps, void *stream);
+
+/* out[M,K] = the values that codes and scales stand for (I8L_BF16/F16/F32). */
+int i8l_dequant_mxfp4(const uint8_t *q, int64_t ldq, const uint8_t *scale, void *out, int64_t ldo,
+                      int32_t out_dtype, int32_t M, int32_t K, void *stream);
+
+/*
+ * RMSNorm of every query and key head of a qkv product and its rotation by the token's
+ * position, in one pass:
+ *     n = x / sqrt(mean(x^2) + eps) * weight          (per head, in float32)
+ *     pairs (a, b) of n's first rot_dim values -> (a cos - b sin, b cos + a sin)
+ * then one rounding to act_dtype (I8L_BF16/F16).
+ *   qkv       token t's row at qkv + t*ld elements: `heads` query heads, then `kv_heads`
+ *             key heads, head_dim values each; what follows (the values) is not read
+ *   weights   head_dim values of w_dtype, one vector for queries and one for keys
+ *   positions one int32 (positions_i64 = 0) or int64 per token
+ *   cos_sin   [max_pos, rot_dim] of cs_dtype: rot_dim/2 cosines, then rot_dim/2 sines; a
+ *             token whose position is outside [0, max_pos) comes out as NaN
+ *   pairs     (i, i + rot_dim/2), or (2i, 2i+1) with interleaved
+ *   q_out     token t's query heads at q_out + t*ldq, k_out likewise.  They may be the
+ *             heads' own places in qkv; no other overlap is allowed.
+ * head_dim: a multiple of 8 up to 256.  rot_dim: a multiple of 16 (8 with interleaved) up
+ * to head_dim.  Rows must be 16-byte aligned.
+ * No reference counterpart (its stand-in leaves attention out).
+ */
+int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, const void *q_weight,
+                     const void *k_weight, int32_t w_dtype, float eps, const void *positions,
+                     int32_t positions_i64, const void *cos_sin, int32_t cs_dtype, int64_t max_pos,
+                     void *q_out, int64_t ldq, void *k_out, int64_t ldk, int32_t tokens,
+                     int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t rot_dim,
+                     int32_t interleaved, void *stream);
+
 /* One-line message for the last non-OK return on this host thread. */
 const char *i8l_last_error(void);
 

@@ -48,6 +48,7 @@ _lock = threading.Lock()
 
 _vp, _i8p, _fp = ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p
 _i32, _i64, _f32, _sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); the same list the CPU tests check against the header.
 SIGNATURES = {
@@ -73,6 +74,14 @@ SIGNATURES = {
     "i8l_quant_rows_ex": (_i32, [_vp, _i64, _i32, _i8p, _i64, _fp, _i32, _i32, _i32, _fp, _fp, _vp]),
     "i8l_dequant_i32": (_i32, [_vp, _i64, _fp, _i32, _fp, _i32, _vp, _i32, _vp, _i32, _i64, _i32, _i32,
                                _vp]),
+    "i8l_mxfp4_scale_bytes": (_sz, [_i32, _i32]),
+    "i8l_quant_mxfp4": (_i32, [_vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _vp]),
+    "i8l_silu_mul_quant_mxfp4": (_i32, [_vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _vp]),
+    "i8l_add_rmsnorm_quant_mxfp4": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _i64,
+                                           _i32, _i32, _f64, _vp]),
+    "i8l_dequant_mxfp4": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
+    "i8l_qk_norm_rope": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _f32, _vp, _i32, _vp, _i32, _i64, _vp, _i64,
+                                _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "i8l_last_error": (ctypes.c_char_p, []),
     "i8l_read_status": (_i32, [ctypes.POINTER(_i32)]),
     "i8l_clear_status": (_i32, []),
@@ -132,6 +141,18 @@ def check(code: int) -> None:
     if code == EINVAL:
         raise ValueError(msg)
     raise RuntimeError(f"int8_linear native call failed ({code}): {msg}")
+
+
+def on_device(index: int, fn, args: tuple) -> None:
+    """check(fn(*args)) with CUDA device `index` current: launches go to the current device,
+    which need not be the one the tensors are on."""
+    import torch
+
+    if index == torch.cuda.current_device():
+        check(fn(*args))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args))
 
 
 # Called when the status word shows a kernel gave up a wait, and by clear_status():

@@ -1,0 +1,509 @@
+// MXFP4 quantisers for sm_100a and the way back:
+//   quant_mxfp4              block-quantise a bf16/fp16/fp32 matrix
+//   silu_mul_quant_mxfp4     SiLU-and-mul, then the same
+//   add_rmsnorm_quant_mxfp4  residual add + RMSNorm, then the same
+//   dequant_mxfp4            the values that codes and scales stand for
+// They stand beside the per-token int8 quantisers (quant.cu) and compute the same y; only
+// what y is stored in differs.  A block's scale depends on its own 32 values, so there is
+// no row reduction in the plain and SiLU quantisers: a lane takes eight values, four
+// neighbouring lanes share a block (two shuffles), and the matrix is walked as one flat
+// list of eight-value vectors.  All four kernels move each byte once and are bound by HBM.
+//
+// A 4-bit value next to the border between two steps flips on the last bit of y, so y is
+// computed to the bit: the norm's mean in float64, and SiLU in float32 with a second, exact
+// pass for the few values where the float32 error could change the rounding.
+#include <algorithm>
+
+#include "common.cuh"
+#include "internal.h"
+#include "mxfp4.cuh"
+#include "rows.cuh"
+
+namespace i8l {
+
+constexpr int kFlatThreads = 256;
+
+// Unsigned division by a constant of the launch: floor(n / d) for n < 2^31 as a multiply
+// and a shift (the round-up method: m = ceil(2^(32+s) / d), s = ceil(log2 d)).
+struct FastDiv {
+  uint32_t d, m, s;
+  explicit FastDiv(uint32_t div = 1) : d(div), m(0), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = static_cast<uint32_t>(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    const uint32_t t = __umulhi(n, m);
+    return (t + n) >> s;  // t + n < 2^32 for n < 2^31
+  }
+};
+
+struct MxOut {
+  uint8_t *q;
+  long long ldq;  // bytes
+  uint8_t *sf;
+  int ktiles;  // 128-value tiles along K
+};
+
+// Writes one block's scale byte and, after the row's last block, the zero bytes up to the
+// end of its word.
+__device__ __forceinline__ void store_sf(const MxOut &o, long long row, int block, int blocks, uint32_t byte) {
+  uint8_t *p = o.sf + sf_word_offset(row, block >> 2, o.ktiles);
+  p[block & 3] = static_cast<uint8_t>(byte);
+  if (block == blocks - 1)
+    for (int i = (block & 3) + 1; i < 4; ++i) p[i] = 0;
+}
+
+// Zero words of the scale tiles below the last row: word i of (rows_pad - rows) * ktiles.
+__device__ __forceinline__ void zero_pad_word(const MxOut &o, long long rows, long long i) {
+  *reinterpret_cast<uint32_t *>(o.sf + sf_word_offset(rows + i / o.ktiles, static_cast<int>(i % o.ktiles), o.ktiles)) = 0u;
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void *base, long long idx, bool vec, float (&v)[8]) {
+  using T = typename ActType<DT>::T;
+  const T *p = static_cast<const T *>(base) + idx;
+  if (vec) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / kPer; ++h) {
+      const uint4 raw = reinterpret_cast<const uint4 *>(p)[h];
+      const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[h * kPer + i] = ActType<DT>::to_f32(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ActType<DT>::to_f32(p[i]);
+  }
+}
+
+// ------------------------------------------------------------------ SiLU
+
+// float32(g / (1 + exp(-g)) * u) in float64: within 2^-50 of the exact value before its
+// one rounding.  Kept out of line: few values come here.
+__device__ __noinline__ float silu_mul_exact(float g, float u) {
+  const double gd = g;
+  return static_cast<float>(gd / (1.0 + exp(-gd)) * static_cast<double>(u));
+}
+
+// Two values of y = round_DT(float32(silu(g) * u)), the float32 rounding being that of the
+// exact product.  In float32, expf and the full-range division are within 2 ulp each (their
+// documented bounds), the sum and the product within 0.5: 5 ulp of at most 2^-23 relative
+// each.  With a margin of one more, y is right wherever both ends of
+// [v (1 - 6*2^-23), v (1 + 6*2^-23)] round alike; elsewhere (about one value in 2000 for
+// bf16) the value is computed again in float64.  Results near or below the smallest normal
+// float32 have no such relative bound and take that way too, but for products with zero.
+template <int DT>
+__device__ __forceinline__ void silu_mul2(float g0, float g1, float u0, float u1, float &y0, float &y1) {
+  float d0, d1, v0, v1, l0, l1, h0, h1;
+  add2_rn(d0, d1, 1.0f, 1.0f, expf(-g0), expf(-g1));
+  mul2_rn(v0, v1, div_full(g0, d0), div_full(g1, d1), u0, u1);
+  constexpr float kLow = 1.0f - 6.0f / 8388608.0f, kHigh = 1.0f + 6.0f / 8388608.0f;
+  mul2_rn(l0, l1, v0, v1, kLow, kLow);
+  mul2_rn(h0, h1, v0, v1, kHigh, kHigh);
+  round2_through<DT>(l0, l1);
+  round2_through<DT>(h0, h1);
+  y0 = l0;
+  y1 = l1;
+  constexpr float kTiny = 1e-36f;
+  if (l0 != h0 || (fabsf(v0) < kTiny && g0 != 0.f && u0 != 0.f)) y0 = round_through<DT>(silu_mul_exact(g0, u0));
+  if (l1 != h1 || (fabsf(v1) < kTiny && g1 != 0.f && u1 != 0.f)) y1 = round_through<DT>(silu_mul_exact(g1, u1));
+}
+
+// ------------------------------------------------------------------ flat quantisers
+
+struct FlatArgs {
+  const void *x;
+  long long ldx;
+  MxOut o;
+  int rows, blocks;        // rows of this launch, 32-value blocks per row
+  uint32_t vectors;        // rows * blocks * 4
+  uint32_t pad_words;      // zero words below the last row
+  FastDiv per_row;         // vectors per row
+  int vec;                 // 16-byte loads allowed
+};
+
+// kSilu: x holds [gate | up] rows of 2K values.
+template <int DT, bool kSilu, int U>
+__global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t base = blockIdx.x * (kFlatThreads * U) + threadIdx.x;
+  const long long K = static_cast<long long>(a.blocks) * kMxBlock;
+  float y[U][8];
+  uint32_t row[U], vec[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t id = base + u * kFlatThreads;
+    row[u] = a.per_row.div(id);
+    vec[u] = id - row[u] * a.per_row.d;
+    if (id < a.vectors) {
+      const long long at = row[u] * a.ldx + vec[u] * 8u;
+      load8<DT>(a.x, at, a.vec, y[u]);
+      if constexpr (kSilu) {
+        float up[8];
+        load8<DT>(a.x, at + K, a.vec, up);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) silu_mul2<DT>(y[u][i], y[u][i + 1], up[i], up[i + 1], y[u][i], y[u][i + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[u][i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t id = base + u * kFlatThreads;
+    uint32_t byte;
+    const uint32_t w = mx_quantise8(y[u], byte);
+    if (id < a.vectors) {
+      *reinterpret_cast<uint32_t *>(a.o.q + row[u] * a.o.ldq + vec[u] * 4u) = w;
+      if ((threadIdx.x & 3) == 0) store_sf(a.o, row[u], static_cast<int>(vec[u] >> 2), a.blocks, byte);
+    } else if (id - a.vectors < a.pad_words) {
+      zero_pad_word(a.o, a.rows, id - a.vectors);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ add + RMSNorm
+
+struct MxNormArgs {
+  const void *x;
+  long long ldx;
+  const void *res;
+  long long ldr;
+  const void *w;
+  int w_dtype, w_vec;
+  void *rout;
+  long long ldro;
+  MxOut o;
+  int rows, K;
+  double eps;
+  uint32_t pad_words;
+  int vec;  // 16-byte loads and stores allowed
+};
+
+__device__ __forceinline__ double block_sum_f64(double v, double *red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
+  if (l == 0) red[w] = v;
+  __syncthreads();
+  v = l < nw ? red[l] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One row per CTA, the row in registers.  The squares are summed in float64 (a float32
+// squares exactly into one) and 1/sqrt(mean + eps) is rounded once to float32, so the
+// factor does not depend on the order of the sum.
+template <int DT, int NV>
+__global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  using T = typename ActType<DT>::T;
+  const long long row = blockIdx.x;
+  if (row >= a.rows) {  // zero words of the scale tiles below the last row
+    const long long i = (row - a.rows) * blockDim.x + threadIdx.x;
+    if (i < a.pad_words) zero_pad_word(a.o, a.rows, i);
+    return;
+  }
+  __shared__ double red[32];
+  float h[NV][8];
+  double ss = 0.0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int col = col_of<8>(v);
+    if (col < a.K) {
+      load8<DT>(a.x, row * a.ldx + col, a.vec, h[v]);
+      if (a.res) {
+        float r[8];
+        load8<DT>(a.res, row * a.ldr + col, a.vec, r);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) add2_rn(h[v][i], h[v][i + 1], h[v][i], h[v][i + 1], r[i], r[i + 1]);
+        T *p = static_cast<T *>(a.rout) + row * a.ldro;
+        if (a.vec) {
+          store_vec<DT, 8>(p, col, h[v]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[col + i] = ActType<DT>::from_f32(h[v][i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fma(static_cast<double>(h[v][i]), static_cast<double>(h[v][i]), ss);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[v][i] = 0.f;
+    }
+  }
+  ss = block_sum_f64(ss, red);
+  const float rs = static_cast<float>(1.0 / sqrt(ss / a.K + a.eps));
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int col = col_of<8>(v);
+    if (col < a.K) {
+      float w[8];
+      load_weight_vec<8>(a.w, a.w_dtype, col, a.w_vec != 0, w);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        float n0, n1;
+        mul2_rn(n0, n1, h[v][i], h[v][i + 1], rs, rs);
+        n0 = round_to_weight(n0, a.w_dtype);
+        n1 = round_to_weight(n1, a.w_dtype);
+        mul2_rn(h[v][i], h[v][i + 1], n0, n1, w[i], w[i + 1]);
+        round2_through<DT>(h[v][i], h[v][i + 1]);
+      }
+    }
+    uint32_t byte;
+    const uint32_t packed = mx_quantise8(h[v], byte);
+    if (col < a.K) {
+      *reinterpret_cast<uint32_t *>(a.o.q + row * a.o.ldq + col / 2) = packed;
+      if ((threadIdx.x & 3) == 0) store_sf(a.o, row, col / kMxBlock, a.K / kMxBlock, byte);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ dequantisation
+
+struct DeqArgs {
+  const uint8_t *q;
+  long long ldq;
+  const uint8_t *sf;
+  int ktiles;
+  void *out;
+  long long ldo;
+  uint32_t vectors;
+  FastDiv per_row;
+  int vec;
+};
+
+template <int DT, int U>
+__global__ void __launch_bounds__(kFlatThreads) mx_dequant_kernel(const DeqArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  using T = typename ActType<DT>::T;
+  const uint32_t base = blockIdx.x * (kFlatThreads * U) + threadIdx.x;
+  uint32_t row[U], vec[U], w[U], byte[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t id = base + u * kFlatThreads;
+    row[u] = a.per_row.div(id);
+    vec[u] = id - row[u] * a.per_row.d;
+    w[u] = byte[u] = 0u;
+    if (id < a.vectors) {
+      w[u] = *reinterpret_cast<const uint32_t *>(a.q + row[u] * a.ldq + vec[u] * 4u);
+      const int block = static_cast<int>(vec[u] >> 2);
+      byte[u] = a.sf[sf_word_offset(row[u], block >> 2, a.ktiles) + (block & 3)];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (base + u * kFlatThreads >= a.vectors) continue;
+    float v[8];
+    mx_unpack8(w[u], v);
+    const float s = mx_scale_value(byte[u]);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) mul2_rn(v[i], v[i + 1], v[i], v[i + 1], s, s);
+    T *p = static_cast<T *>(a.out) + row[u] * a.ldo + vec[u] * 8u;
+    if (a.vec) {
+      if constexpr (DT == I8L_F32) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        store_vec<DT, 8>(p, 0, v);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = ActType<DT>::from_f32(v[i]);
+    }
+  }
+}
+
+}  // namespace i8l
+
+using namespace i8l;
+
+namespace {
+
+int finish_launch(cudaError_t err, const char *what) {
+  if (err != cudaSuccess) return cuda_error(err, what);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? I8L_OK : cuda_error(e, what);
+}
+
+constexpr int kMxMaxK = 1 << 26;  // 128 rows of vectors fit a flat kernel's 31-bit index
+
+// Shape and output checks that the quantisers share.
+int check_mx(int32_t M, int32_t K, const void *q, int64_t ldq, const void *sf) {
+  if (M < 0 || K < 0) return set_error(I8L_EINVAL, "negative size M=%d K=%d", M, K);
+  if (K % kMxBlock) return set_error(I8L_ENOTSUP, "K=%d must be a multiple of 32 (whole blocks)", K);
+  if (K > kMxMaxK) return set_error(I8L_ENOTSUP, "K=%d is above %d", K, kMxMaxK);
+  if (M == 0 || K == 0) return I8L_OK;
+  if (!q || !sf) return set_error(I8L_EINVAL, "NULL pointer argument");
+  if (ldq < K / 2) return set_error(I8L_EINVAL, "packed row stride %lld < K/2", static_cast<long long>(ldq));
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(sf)) % 4 || ldq % 4)
+    return set_error(I8L_ENOTSUP, "packed rows and scales must be 4-byte aligned");
+  return I8L_OK;
+}
+
+int act_size(int dtype) { return dtype == I8L_F32 ? 4 : 2; }
+
+bool vec_rows(const void *p, int64_t ld, int dtype) { return aligned16(p) && (ld * act_size(dtype)) % 16 == 0; }
+
+// Rows of one launch of a flat kernel: the vector count stays below 2^31 with the padding
+// words on top, in whole scale tiles.
+int64_t flat_rows(int32_t K) {
+  const int64_t rows = ((1LL << 30) / (K / 8)) & ~127LL;
+  return std::max<int64_t>(rows, 128);
+}
+
+template <bool kSilu>
+int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uint8_t *sf, int32_t M, int32_t K,
+             void *stream, const char *what) {
+  const int blocks = K / kMxBlock, ktiles = (K + 127) / 128;
+  const int64_t step = flat_rows(K);
+  for (int64_t r0 = 0; r0 < M; r0 += step) {
+    const int rows = static_cast<int>(std::min<int64_t>(step, M - r0));
+    const int pad = (128 - rows % 128) % 128;
+    FlatArgs a;
+    a.x = static_cast<const uint8_t *>(x) + r0 * ldx * act_size(dtype);
+    a.ldx = ldx;
+    a.o = MxOut{q + r0 * ldq, ldq, sf + (r0 / 128) * ktiles * kSfTileBytes, ktiles};
+    a.rows = rows;
+    a.blocks = blocks;
+    a.vectors = static_cast<uint32_t>(rows) * (blocks * 4u);
+    a.pad_words = static_cast<uint32_t>(pad) * ktiles;
+    a.per_row = FastDiv(blocks * 4u);
+    a.vec = vec_rows(x, ldx, dtype) && (!kSilu || (static_cast<int64_t>(K) * act_size(dtype)) % 16 == 0);
+    constexpr int U = kSilu ? 1 : 2;
+    const int64_t work = static_cast<int64_t>(a.vectors) + a.pad_words;
+    const dim3 grid(static_cast<unsigned>((work + kFlatThreads * U - 1) / (kFlatThreads * U)));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t err;
+    if (dtype == I8L_BF16)
+      err = launch(mx_quant_kernel<I8L_BF16, kSilu, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+    else if (dtype == I8L_F16)
+      err = launch(mx_quant_kernel<I8L_F16, kSilu, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+    else if constexpr (!kSilu)
+      err = launch(mx_quant_kernel<I8L_F32, false, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+    else
+      err = cudaErrorInvalidValue;
+    if (int e = finish_launch(err, what)) return e;
+  }
+  return I8L_OK;
+}
+
+}  // namespace
+
+extern "C" size_t i8l_mxfp4_scale_bytes(int32_t rows, int32_t K) {
+  if (rows <= 0 || K <= 0) return 0;
+  return static_cast<size_t>((static_cast<int64_t>(rows) + 127) / 128) * ((static_cast<int64_t>(K) + 127) / 128) *
+         kSfTileBytes;
+}
+
+extern "C" int i8l_quant_mxfp4(const void *x, int64_t ldx, int32_t dtype, uint8_t *q, int64_t ldq, uint8_t *scale,
+                               int32_t M, int32_t K, void *stream) {
+  if (dtype < I8L_BF16 || dtype > I8L_F32)
+    return set_error(I8L_ENOTSUP, "dtype code %d not supported (bf16, fp16 or fp32)", dtype);
+  if (int e = check_mx(M, K, q, ldq, scale)) return e;
+  if (M == 0 || K == 0) return I8L_OK;
+  if (!x) return set_error(I8L_EINVAL, "NULL pointer argument");
+  if (ldx < K) return set_error(I8L_EINVAL, "row stride smaller than K");
+  return run_flat<false>(x, ldx, dtype, q, ldq, scale, M, K, stream, "quant_mxfp4 launch");
+}
+
+extern "C" int i8l_silu_mul_quant_mxfp4(const void *gate_up, int64_t ld, int32_t act_dtype, uint8_t *q, int64_t ldq,
+                                        uint8_t *scale, int32_t M, int32_t I, void *stream) {
+  if (act_dtype != I8L_BF16 && act_dtype != I8L_F16)
+    return set_error(I8L_ENOTSUP, "activation dtype code %d not supported (bf16 or fp16)", act_dtype);
+  if (int e = check_mx(M, I, q, ldq, scale)) return e;
+  if (M == 0 || I == 0) return I8L_OK;
+  if (!gate_up) return set_error(I8L_EINVAL, "NULL pointer argument");
+  if (ld < 2LL * I) return set_error(I8L_EINVAL, "row stride too small");
+  return run_flat<true>(gate_up, ld, act_dtype, q, ldq, scale, M, I, stream, "silu_mul_quant_mxfp4 launch");
+}
+
+extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const void *residual, int64_t ldr,
+                                           const void *weight, int32_t act_dtype, int32_t w_dtype, uint8_t *q,
+                                           int64_t ldq, uint8_t *scale, void *rout, int64_t ldro, int32_t M,
+                                           int32_t K, double eps, void *stream) {
+  if (act_dtype != I8L_BF16 && act_dtype != I8L_F16)
+    return set_error(I8L_ENOTSUP, "activation dtype code %d not supported (bf16 or fp16)", act_dtype);
+  if (w_dtype < I8L_BF16 || w_dtype > I8L_F32)
+    return set_error(I8L_ENOTSUP, "weight dtype code %d not supported", w_dtype);
+  if (int e = check_mx(M, K, q, ldq, scale)) return e;
+  if (M == 0 || K == 0) return I8L_OK;
+  if (!x || !weight) return set_error(I8L_EINVAL, "NULL pointer argument");
+  if ((residual == nullptr) != (rout == nullptr))
+    return set_error(I8L_EINVAL, "residual and residual_out must be given together");
+  if (ldx < K || (residual && (ldr < K || ldro < K))) return set_error(I8L_EINVAL, "row stride smaller than K");
+  const bool vec = vec_rows(x, ldx, act_dtype) &&
+                   (!residual || (vec_rows(residual, ldr, act_dtype) && vec_rows(rout, ldro, act_dtype)));
+  RowShape rs;
+  if (!row_shape(K, 8, &rs)) return set_error(I8L_ENOTSUP, "row of %d values is too long", K);
+  const int ktiles = (K + 127) / 128;
+  MxNormArgs a;
+  a.x = x;
+  a.ldx = ldx;
+  a.res = residual;
+  a.ldr = ldr;
+  a.w = weight;
+  a.w_dtype = w_dtype;
+  a.w_vec = aligned16(weight) ? 1 : 0;
+  a.rout = rout;
+  a.ldro = ldro;
+  a.o = MxOut{q, ldq, scale, ktiles};
+  a.rows = M;
+  a.K = K;
+  a.eps = eps;
+  a.pad_words = static_cast<uint32_t>((128 - M % 128) % 128) * ktiles;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int nv = rs.nv, th = rs.threads;
+  const dim3 grid(static_cast<unsigned>(M) + (a.pad_words + th - 1) / th);
+  cudaError_t err = cudaSuccess;
+  a.vec = vec ? 1 : 0;
+  if (act_dtype == I8L_BF16) {
+    I8L_DISPATCH_NV(nv, (err = launch(mx_norm_quant_kernel<I8L_BF16, NV>, grid, dim3(th), 0, s, 1, a)))
+  } else {
+    I8L_DISPATCH_NV(nv, (err = launch(mx_norm_quant_kernel<I8L_F16, NV>, grid, dim3(th), 0, s, 1, a)))
+  }
+  return finish_launch(err, "add_rmsnorm_quant_mxfp4 launch");
+}
+
+extern "C" int i8l_dequant_mxfp4(const uint8_t *q, int64_t ldq, const uint8_t *scale, void *out, int64_t ldo,
+                                 int32_t out_dtype, int32_t M, int32_t K, void *stream) {
+  if (out_dtype < I8L_BF16 || out_dtype > I8L_F32)
+    return set_error(I8L_ENOTSUP, "dtype code %d not supported (bf16, fp16 or fp32)", out_dtype);
+  if (int e = check_mx(M, K, q, ldq, scale)) return e;
+  if (M == 0 || K == 0) return I8L_OK;
+  if (!out) return set_error(I8L_EINVAL, "NULL pointer argument");
+  if (ldo < K) return set_error(I8L_EINVAL, "row stride smaller than K");
+  const int ktiles = (K + 127) / 128;
+  const int64_t step = flat_rows(K);
+  for (int64_t r0 = 0; r0 < M; r0 += step) {
+    const int rows = static_cast<int>(std::min<int64_t>(step, M - r0));
+    DeqArgs a;
+    a.q = q + r0 * ldq;
+    a.ldq = ldq;
+    a.sf = scale + (r0 / 128) * ktiles * kSfTileBytes;
+    a.ktiles = ktiles;
+    a.out = static_cast<uint8_t *>(out) + r0 * ldo * act_size(out_dtype);
+    a.ldo = ldo;
+    a.vectors = static_cast<uint32_t>(rows) * (K / 8u);
+    a.per_row = FastDiv(K / 8u);
+    a.vec = vec_rows(out, ldo, out_dtype);
+    constexpr int U = 4;
+    const dim3 grid((a.vectors + kFlatThreads * U - 1) / (kFlatThreads * U));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t err;
+    if (out_dtype == I8L_BF16)
+      err = launch(mx_dequant_kernel<I8L_BF16, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+    else if (out_dtype == I8L_F16)
+      err = launch(mx_dequant_kernel<I8L_F16, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+    else
+      err = launch(mx_dequant_kernel<I8L_F32, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+    if (int e = finish_launch(err, "dequant_mxfp4 launch")) return e;
+  }
+  return I8L_OK;
+}

@@ -1,0 +1,103 @@
+// Microscaled 4-bit floating point (MXFP4) on the device: blocks of 32 consecutive
+// values along K, each value in e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives),
+// each block with one power-of-two scale in e8m0 (byte b stands for 2^(b - 127), 0xFF for
+// NaN).
+//
+// Packed codes: row r at q + r*ldq bytes, value 2j in the low and 2j+1 in the high nibble
+// of byte j.  Scales: tiles of 128 rows x 4 blocks (128 values), 512 bytes each, the tiles
+// of one 128-row group in order of K:
+//     byte of (row r, block b) = ((r/128) * ceil(K/128) + b/4) * 512
+//                                + (r%32)*16 + ((r/32)%4)*4 + b%4
+// which is the order that a tensor core takes block scales in, so the GEMM copies a tile
+// as it lies.  Bytes of a tile past the last row or the last block are 0.
+#pragma once
+
+#include "common.cuh"
+
+namespace i8l {
+
+constexpr int kMxBlock = 32;       // values per scale
+constexpr int kSfTileBytes = 512;  // 128 rows x 4 blocks
+
+// Byte offset of the word that holds the scales of blocks 4*kt .. 4*kt+3 of a row.
+__host__ __device__ __forceinline__ long long sf_word_offset(long long row, int kt, int ktiles) {
+  return ((row >> 7) * ktiles + kt) * kSfTileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+// Scale byte of a block whose largest magnitude has the float32 bits `amax` (sign clear):
+// 2^(floor(log2 amax) - 2), so the largest value lands in [4, 8) and saturates at 6; at
+// least 2^-127.  The float's biased exponent minus 2 is that byte, subnormals included
+// (their exponent field 0 clamps to 0).  Infinity or NaN anywhere makes the block NaN.
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax) {
+  const uint32_t e = amax >> 23;
+  return e == 255u ? 255u : (e < 2u ? 0u : e - 2u);
+}
+
+// 2^(127 - byte): the factor that takes a block's values into e2m1 range, exact for the
+// bytes mx_scale_byte gives (0..252).  A product with it is exact too, or too small to
+// round to anything but zero.
+__device__ __forceinline__ float mx_inv_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+// 2^(byte - 127), NaN for 0xFF; 2^-127 is a float32 subnormal.
+__device__ __forceinline__ float mx_scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7fc00000u : (byte == 0u ? 0x00400000u : byte << 23));
+}
+
+// Eight values times `inv`, rounded to e2m1 (nearest, ties to even, saturating), packed
+// with the first value in the lowest nibble.
+__device__ __forceinline__ uint32_t mx_pack8(const float (&y)[8], float inv) {
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) mul2_rn(p[i], p[i + 1], y[i], y[i + 1], inv, inv);
+  uint32_t w;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(w)
+      : "f"(p[0]), "f"(p[1]), "f"(p[2]), "f"(p[3]), "f"(p[4]), "f"(p[5]), "f"(p[6]), "f"(p[7]));
+  return w;
+}
+
+// Eight packed e2m1 codes as floats (exact).
+__device__ __forceinline__ void mx_unpack8(uint32_t w, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// Largest float32 magnitude, as bits, of eight values: NaN and infinity compare above
+// every finite value, which a float maximum would not do for NaN.
+__device__ __forceinline__ uint32_t mx_amax8(const float (&y)[8]) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(y[i]) & 0x7fffffffu);
+  return m;
+}
+
+// One lane's eight values of a block shared by four neighbouring lanes: the scale from the
+// four lanes' maximum, then this lane's four packed bytes (zero codes in a NaN block).
+// Every lane of the warp takes part; lanes without values pass zeros.
+__device__ __forceinline__ uint32_t mx_quantise8(const float (&y)[8], uint32_t &byte) {
+  uint32_t m = mx_amax8(y);
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  byte = mx_scale_byte(m);
+  return byte == 255u ? 0u : mx_pack8(y, mx_inv_scale(byte));
+}
+
+}  // namespace i8l

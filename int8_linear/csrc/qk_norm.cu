@@ -1,0 +1,233 @@
+// RMSNorm of every query and key head of a qkv product and the rotation by the token's
+// position, in one pass, for sm_100a.  For a head x of `dim` values with norm weight w
+// (one weight for queries, one for keys):
+//     n = x / sqrt(mean(x^2) + eps) * w
+//     y = n with its first `rot` values rotated in pairs (a, b) by the position's angles:
+//         a' = a cos - b sin,  b' = b cos + a sin
+// where pair i is (n[i], n[i + rot/2]), or (n[2i], n[2i + 1]) when interleaved.  Everything
+// is float32 between the load and one rounding at the store.
+//
+// A group of lanes, eight values each, holds one head in registers: the sum of squares is
+// a butterfly over the group, and the other half of a pair comes from another lane of the
+// group by a shuffle.  A group keeps its token's cosines and sines in registers and walks
+// over the heads of that token, so the angles are read once per group and not per head.
+// The kernel reads and writes each value once and is bound by HBM.
+#include <algorithm>
+
+#include "common.cuh"
+#include "internal.h"
+#include "rows.cuh"
+
+namespace i8l {
+
+constexpr int kQkThreads = 256;
+
+struct QkArgs {
+  const void *qkv;
+  long long ld;
+  const void *wq, *wk;
+  int w_dtype;
+  const void *positions;
+  int pos64;
+  const void *cos_sin;
+  int cs_dtype;
+  long long max_pos;
+  void *q;
+  long long ldq;  // elements between tokens; heads are `dim` apart
+  void *k;
+  long long ldk;
+  int tokens, heads, kv_heads, dim, rot;
+  int parts;       // groups per token
+  long long groups;  // tokens * parts
+  float eps;
+  int interleaved;
+  int w_vec, cs_vec;
+};
+
+// G lanes per head (a power of two, G * 8 >= dim).  In place is fine: a lane stores the
+// elements that it alone loaded, after every exchange within its head.
+template <int DT, int G>
+__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  using T = typename ActType<DT>::T;
+  const long long group = (static_cast<long long>(blockIdx.x) * kQkThreads + threadIdx.x) / G;
+  const int lane = threadIdx.x % G;
+  const bool live = group < a.groups;
+  const long long token = live ? group / a.parts : 0;
+  const int part = live ? static_cast<int>(group - token * a.parts) : 0;
+  const int c0 = lane * 8;
+  const bool mine = live && c0 < a.dim;
+  const int half = a.rot / 2;
+
+  long long pos = 0;
+  if (live)
+    pos = a.pos64 ? static_cast<const long long *>(a.positions)[token] : static_cast<const int *>(a.positions)[token];
+  // A position outside the table has no angles: the token's heads come out as NaN.
+  const bool known = a.rot == 0 || (pos >= 0 && pos < a.max_pos);
+  const bool turns = mine && c0 < a.rot;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    cs[i] = 1.f;
+    sn[i] = 0.f;
+  }
+  if (turns && known) {
+    const uint8_t *table = static_cast<const uint8_t *>(a.cos_sin) +
+                           pos * a.rot * (a.cs_dtype == I8L_F32 ? 4 : 2);
+    if (a.interleaved) {
+      // pairs (2i, 2i + 1): both take angle i
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        cs[i] = load_weight(table, a.cs_dtype, (c0 + i) / 2);
+        sn[i] = load_weight(table, a.cs_dtype, half + (c0 + i) / 2);
+      }
+    } else {
+      const int j = c0 < half ? c0 : c0 - half;
+      load_weight_vec<8>(table, a.cs_dtype, j, a.cs_vec != 0, cs);
+      load_weight_vec<8>(table, a.cs_dtype, half + j, a.cs_vec != 0, sn);
+    }
+    // the first value of a pair subtracts its partner's share
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (a.interleaved ? i % 2 == 0 : c0 < half) sn[i] = -sn[i];
+  }
+  // The lane of this group that holds the other values of this lane's pairs.
+  const int partner = !a.interleaved && turns ? (c0 < half ? lane + half / 8 : lane - half / 8) : lane;
+
+  float w[8];
+  int loaded = -1;  // which weight `w` holds: 0 queries, 1 keys
+  const int all = a.heads + a.kv_heads;
+  // Every group of a warp takes the same number of turns: the shuffles are warp-wide.
+  for (int turn = 0; turn * a.parts < all; ++turn) {
+    const int head = part + turn * a.parts;
+    const bool here = mine && head < all;
+    const int key = head >= a.heads ? 1 : 0;
+    if (here && key != loaded) load_weight_vec<8>(key ? a.wk : a.wq, a.w_dtype, c0, a.w_vec != 0, w);
+    loaded = key;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (here) load_vec<DT, 8>(static_cast<const T *>(a.qkv) + token * a.ld + static_cast<long long>(head) * a.dim, c0, x);
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
+    float rs = 1.0f / sqrtf(ss / static_cast<float>(a.dim) + a.eps);
+    if (!known) rs = __int_as_float(0x7fc00000);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = here ? x[i] * rs * w[i] : 0.f;
+    if (a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = turns ? x[i] * cs[i] + x[i ^ 1] * sn[i] : x[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float other = __shfl_sync(0xffffffffu, x[i], partner, G);
+        y[i] = turns ? x[i] * cs[i] + other * sn[i] : x[i];
+      }
+    }
+    if (here) {
+      T *dst = key ? static_cast<T *>(a.k) + token * a.ldk + static_cast<long long>(head - a.heads) * a.dim
+                   : static_cast<T *>(a.q) + token * a.ldq + static_cast<long long>(head) * a.dim;
+      store_vec<DT, 8>(dst, c0, y);
+    }
+  }
+}
+
+}  // namespace i8l
+
+using namespace i8l;
+
+namespace {
+
+template <int DT>
+cudaError_t launch_qk(const QkArgs &a, int lanes, cudaStream_t s) {
+  const long long per_block = kQkThreads / lanes;
+  const dim3 grid(static_cast<unsigned>((a.groups + per_block - 1) / per_block));
+  switch (lanes) {
+    case 1: return launch(qk_norm_rope_kernel<DT, 1>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 2: return launch(qk_norm_rope_kernel<DT, 2>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 4: return launch(qk_norm_rope_kernel<DT, 4>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 8: return launch(qk_norm_rope_kernel<DT, 8>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 16: return launch(qk_norm_rope_kernel<DT, 16>, grid, dim3(kQkThreads), 0, s, 1, a);
+    default: return launch(qk_norm_rope_kernel<DT, 32>, grid, dim3(kQkThreads), 0, s, 1, a);
+  }
+}
+
+}  // namespace
+
+extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, const void *q_weight,
+                                const void *k_weight, int32_t w_dtype, float eps, const void *positions,
+                                int32_t positions_i64, const void *cos_sin, int32_t cs_dtype, int64_t max_pos,
+                                void *q_out, int64_t ldq, void *k_out, int64_t ldk, int32_t tokens, int32_t heads,
+                                int32_t kv_heads, int32_t head_dim, int32_t rot_dim, int32_t interleaved,
+                                void *stream) {
+  if (act_dtype != I8L_BF16 && act_dtype != I8L_F16)
+    return set_error(I8L_ENOTSUP, "activation dtype code %d not supported (bf16 or fp16)", act_dtype);
+  if (w_dtype < I8L_BF16 || w_dtype > I8L_F32 || cs_dtype < I8L_BF16 || cs_dtype > I8L_F32)
+    return set_error(I8L_ENOTSUP, "weight dtype code %d or angle dtype code %d not supported", w_dtype, cs_dtype);
+  if (tokens < 0 || heads < 0 || kv_heads < 0 || head_dim <= 0 || rot_dim < 0 || rot_dim > head_dim || max_pos < 0)
+    return set_error(I8L_EINVAL, "bad size tokens=%d heads=%d kv_heads=%d head_dim=%d rot_dim=%d", tokens, heads,
+                     kv_heads, head_dim, rot_dim);
+  if (head_dim % 8 || head_dim > 256)
+    return set_error(I8L_ENOTSUP, "head_dim %d must be a multiple of 8, at most 256", head_dim);
+  if (rot_dim % (interleaved ? 8 : 16))
+    return set_error(I8L_ENOTSUP, "rot_dim %d must be a multiple of %d", rot_dim, interleaved ? 8 : 16);
+  const int64_t all = static_cast<int64_t>(heads) + kv_heads;
+  if (all > INT32_MAX / 256) return set_error(I8L_ENOTSUP, "too many heads: %lld", static_cast<long long>(all));
+  if (tokens == 0 || all == 0) return I8L_OK;
+  if (!qkv || !positions || (rot_dim && !cos_sin) || (heads && (!q_weight || !q_out)) ||
+      (kv_heads && (!k_weight || !k_out)))
+    return set_error(I8L_EINVAL, "NULL pointer argument");
+  if (ld < all * head_dim || (heads && ldq < static_cast<int64_t>(heads) * head_dim) ||
+      (kv_heads && ldk < static_cast<int64_t>(kv_heads) * head_dim))
+    return set_error(I8L_EINVAL, "row stride smaller than the heads of a token");
+  if (!aligned16(qkv) || ld % 8 || (heads && (!aligned16(q_out) || ldq % 8)) ||
+      (kv_heads && (!aligned16(k_out) || ldk % 8)))
+    return set_error(I8L_ENOTSUP, "qkv, q_out and k_out rows must be 16-byte aligned");
+  QkArgs a{};
+  a.qkv = qkv;
+  a.ld = ld;
+  a.wq = q_weight;
+  a.wk = k_weight;
+  a.w_dtype = w_dtype;
+  a.positions = positions;
+  a.pos64 = positions_i64 ? 1 : 0;
+  a.cos_sin = cos_sin;
+  a.cs_dtype = cs_dtype;
+  a.max_pos = max_pos;
+  a.q = q_out;
+  a.ldq = ldq;
+  a.k = k_out;
+  a.ldk = ldk;
+  a.tokens = tokens;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.rot = rot_dim;
+  a.eps = eps;
+  a.interleaved = interleaved ? 1 : 0;
+  a.w_vec = (!heads || aligned16(q_weight)) && (!kv_heads || aligned16(k_weight)) ? 1 : 0;
+  // every row of angles, and its second half, starts on 16 bytes
+  a.cs_vec = aligned16(cos_sin) && (rot_dim / 2 * (cs_dtype == I8L_F32 ? 4 : 2)) % 16 == 0 ? 1 : 0;
+  int lanes = 1;
+  while (lanes * 8 < head_dim) lanes *= 2;
+  // One head per group until the groups fill the SMs twice over, then up to four heads per
+  // group, which share one read of the angles.
+  DeviceInfo di;
+  if (int e = device_info(&di)) return e;
+  const int64_t fill = 2LL * di.sms * (2048 / lanes);
+  int64_t per = std::min<int64_t>(4, std::max<int64_t>(1, static_cast<int64_t>(tokens) * all / fill));
+  a.parts = static_cast<int>((all + per - 1) / per);
+  a.groups = static_cast<long long>(tokens) * a.parts;
+  if (a.groups / (kQkThreads / lanes) >= INT32_MAX)
+    return set_error(I8L_ENOTSUP, "%d tokens x %lld heads is too large", tokens, static_cast<long long>(all));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t err = act_dtype == I8L_BF16 ? launch_qk<I8L_BF16>(a, lanes, s) : launch_qk<I8L_F16>(a, lanes, s);
+  if (err != cudaSuccess) return cuda_error(err, "qk_norm_rope launch");
+  err = cudaGetLastError();
+  return err == cudaSuccess ? I8L_OK : cuda_error(err, "qk_norm_rope launch");
+}

@@ -1,0 +1,196 @@
+"""4-bit linears (MXFP4) for B200 (sm_100a): quantisers and the product.
+
+The operands are microscaled 4-bit floating point: blocks of 32 consecutive values along K,
+each value an e2m1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign), each block one e8m0
+power-of-two scale.  They take a quarter of bf16's bytes and half of int8's, and the tensor
+cores multiply them at twice the int8 rate.
+
+    quant_mxfp4(x)                                   -> (q, s)
+    add_rmsnorm_quant_mxfp4(x, residual, w, eps)     -> (q, s, residual_out)
+    silu_mul_quant_mxfp4(gate_up)                    -> (q, s)
+    dequant_mxfp4(q, s, out_dtype)                   -> the values they stand for
+    w4a4_mm(a_q, b_q, scale_a, scale_b, out_dtype, bias)
+
+stand beside per_token_quant, add_rmsnorm_quant, silu_mul_quant and w8a8_mm and are called
+as those are.  q is uint8 [rows, K/2], the value with the even index in the low nibble.  s
+is uint8 [ceil(rows/128), ceil(K/128), 512], the tensor core's own order: the scale of row
+r, block b is s[r // 128, b // 4, (r % 32) * 16 + (r // 32) % 4 * 4 + b % 4], the byte 127
+standing for 1; bytes of no row or block are 0.  So a weight is quantised once, with
+quant_mxfp4, and a slice of 128-row groups of q and s is the operand of those rows.
+
+A block's scale is 2^(floor(log2 max|y|) - 2), the rule of the OCP microscaling format: the
+block's largest value lands between 4 and 8 steps and saturates at 6.  Values are rounded to
+the nearest, ties to even.  A block that holds an infinity or a NaN becomes NaN.  The
+kernels are csrc/mxfp4.cu and csrc/gemm_mxfp4_sm100.cu behind the C ABI; the quantisers are
+torch custom ops too, under torch.ops.int8_linear.  The reference package
+(AshrithaG/int8-linear) has no 4-bit form.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from int8_linear import _native
+from int8_linear._native import NotSupported
+from int8_linear.fused_quant import _ACT, _WEIGHT
+from int8_linear.kernel import current_stream
+
+BLOCK = 32
+_FLOAT = _WEIGHT  # bf16, fp16 and fp32
+
+__all__ = ["quant_mxfp4", "add_rmsnorm_quant_mxfp4", "silu_mul_quant_mxfp4", "dequant_mxfp4"]
+
+
+def _rows(x: torch.Tensor, name: str, kinds: dict) -> tuple[int, int]:
+    if x.dtype not in kinds:
+        raise NotSupported(f"{name} must be one of {[str(k) for k in kinds]}, got {x.dtype}")
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise NotSupported(f"{name} must be a 2-D tensor with contiguous rows")
+    if not x.is_cuda:
+        raise ValueError(f"the 4-bit quantisers run on a CUDA device, got {x.device}")
+    return x.shape
+
+
+def _empty(m: int, k: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+    if k % BLOCK:
+        raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks)")
+    return (torch.empty((m, k // 2), dtype=torch.uint8, device=device),
+            torch.empty((-(-m // 128), -(-k // 128), 512), dtype=torch.uint8, device=device))
+
+
+def quant_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q uint8 [M, K/2], s uint8 [ceil(M/128), ceil(K/128), 512]) of a bf16, fp16 or fp32
+    matrix with contiguous rows: an activation (a column slice of a wider matrix is fine,
+    no copy is made) or a weight [N, K].  K must be a multiple of 32."""
+    m, k = _rows(x, "x", _FLOAT)
+    q, s = _empty(m, k, x.device)
+    if m and k:
+        dev = x.get_device()
+        _native.on_device(dev, _native.load().i8l_quant_mxfp4, (
+            x.data_ptr(), x.stride(0), _FLOAT[x.dtype], q.data_ptr(), k // 2, s.data_ptr(), m, k,
+            current_stream(dev)))
+    return q, s
+
+
+def add_rmsnorm_quant_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float):
+    """(q, s, residual_out [M, K] or None): fused_quant.add_rmsnorm_quant with its result in
+    4 bits.  h = x + residual in float32 (residual_out is h rounded to x's type);
+    r = 1 / sqrt(mean(h^2) + eps), computed in float64 and rounded once to float32;
+    y = round(round(h * r) * weight), first to the weight's type, then to x's; y is
+    block-quantised.  x and residual bf16/fp16 with contiguous rows."""
+    m, k = _rows(x, "x", _ACT)
+    if weight.dtype not in _WEIGHT or weight.numel() != k or weight.device != x.device:
+        raise ValueError(f"weight must hold {k} bf16/fp16/fp32 values on {x.device}, got {weight.dtype} "
+                         f"{tuple(weight.shape)} on {weight.device}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
+                                 or residual.device != x.device or (k > 1 and residual.stride(1) != 1)):
+        raise ValueError("residual must match x in shape, dtype and device and have contiguous rows")
+    q, s = _empty(m, k, x.device)
+    rout = torch.empty((m, k), dtype=x.dtype, device=x.device) if residual is not None else None
+    if m and k:
+        w = weight if weight.is_contiguous() else weight.contiguous()
+        dev = x.get_device()
+        _native.on_device(dev, _native.load().i8l_add_rmsnorm_quant_mxfp4, (
+            x.data_ptr(), x.stride(0), residual.data_ptr() if residual is not None else None,
+            residual.stride(0) if residual is not None else 0, w.data_ptr(), _ACT[x.dtype], _WEIGHT[w.dtype],
+            q.data_ptr(), k // 2, s.data_ptr(), rout.data_ptr() if rout is not None else None, k, m, k, eps,
+            current_stream(dev)))
+    return q, s, rout
+
+
+def silu_mul_quant_mxfp4(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q, s) of silu(gate) * up for bf16/fp16 rows [gate | up] of 2K values:
+    fused_quant.silu_mul_quant with its result in 4 bits.  The product is rounded to
+    float32 and then to gate_up's type, as if computed exactly, before the blocks."""
+    m, k2 = _rows(gate_up, "gate_up", _ACT)
+    if k2 % 2:
+        raise ValueError(f"gate_up rows of {k2} values are not [gate | up]")
+    k = k2 // 2
+    q, s = _empty(m, k, gate_up.device)
+    if m and k:
+        dev = gate_up.get_device()
+        _native.on_device(dev, _native.load().i8l_silu_mul_quant_mxfp4, (
+            gate_up.data_ptr(), gate_up.stride(0), _ACT[gate_up.dtype], q.data_ptr(), k // 2, s.data_ptr(), m, k,
+            current_stream(dev)))
+    return q, s
+
+
+def _operand(q: torch.Tensor, s: torch.Tensor, rows: int, k: int, name: str) -> None:
+    """Checks that s holds the scales of a [rows, k] operand on q's device."""
+    want = (-(-rows // 128), -(-k // 128), 512)
+    if s.dtype != torch.uint8:
+        raise NotSupported(f"{name} must be uint8 scale bytes, got {s.dtype}")
+    if tuple(s.shape) != want or s.device != q.device:
+        raise ValueError(f"{name} must be the {list(want)} scale tiles of [{rows}, {k}] on {q.device}, got "
+                         f"{tuple(s.shape)} on {s.device}")
+
+
+def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """[M, K] values that codes q [M, K/2] and scales s stand for, in bf16, fp16 or fp32."""
+    if q.dtype != torch.uint8 or out_dtype not in _FLOAT:
+        raise NotSupported(f"uint8 codes to bf16, fp16 or fp32 only, got {q.dtype} to {out_dtype}")
+    if q.dim() != 2 or (q.shape[1] > 1 and q.stride(1) != 1):
+        raise NotSupported("q must be a 2-D tensor with contiguous rows")
+    m, k = q.shape[0], 2 * q.shape[1]
+    if k % BLOCK:
+        raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks)")
+    _operand(q, s, m, k, "s")
+    if not q.is_cuda:
+        raise ValueError(f"dequant_mxfp4 runs on a CUDA device, got {q.device}")
+    out = torch.empty((m, k), dtype=out_dtype, device=q.device)
+    if m and k:
+        if q.data_ptr() % 4 or q.stride(0) % 4:
+            q = q.clone(memory_format=torch.contiguous_format)
+        sc = s if s.is_contiguous() and s.data_ptr() % 4 == 0 else s.clone(memory_format=torch.contiguous_format)
+        dev = q.get_device()
+        _native.on_device(dev, _native.load().i8l_dequant_mxfp4, (
+            q.data_ptr(), q.stride(0), sc.data_ptr(), out.data_ptr(), k, _FLOAT[out_dtype], m, k,
+            current_stream(dev)))
+    return out
+
+
+@torch.library.custom_op("int8_linear::quant_mxfp4", mutates_args=())
+def quant_mxfp4_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return quant_mxfp4(x.contiguous())
+
+
+def _fake(x, m, k):
+    return (x.new_empty((m, k // 2), dtype=torch.uint8),
+            x.new_empty(((m + 127) // 128, (k + 127) // 128, 512), dtype=torch.uint8))
+
+
+@quant_mxfp4_op.register_fake
+def _(x):
+    return _fake(x, x.shape[0], x.shape[1])
+
+
+@torch.library.custom_op("int8_linear::rmsnorm_quant_mxfp4", mutates_args=())
+def rmsnorm_quant_mxfp4_op(x: torch.Tensor, weight: torch.Tensor, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    q, s, _ = add_rmsnorm_quant_mxfp4(x.contiguous(), None, weight, eps)
+    return q, s
+
+
+@rmsnorm_quant_mxfp4_op.register_fake
+def _(x, weight, eps):
+    return _fake(x, x.shape[0], x.shape[1])
+
+
+@torch.library.custom_op("int8_linear::add_rmsnorm_quant_mxfp4", mutates_args=())
+def add_rmsnorm_quant_mxfp4_op(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                               eps: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return add_rmsnorm_quant_mxfp4(x.contiguous(), residual.contiguous(), weight, eps)
+
+
+@add_rmsnorm_quant_mxfp4_op.register_fake
+def _(x, residual, weight, eps):
+    return (*_fake(x, x.shape[0], x.shape[1]), torch.empty_like(x))
+
+
+@torch.library.custom_op("int8_linear::silu_mul_quant_mxfp4", mutates_args=())
+def silu_mul_quant_mxfp4_op(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return silu_mul_quant_mxfp4(gate_up.contiguous())
+
+
+@silu_mul_quant_mxfp4_op.register_fake
+def _(gate_up):
+    return _fake(gate_up, gate_up.shape[0], gate_up.shape[1] // 2)

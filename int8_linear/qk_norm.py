@@ -1,0 +1,90 @@
+"""RMSNorm of every query and key head with the position rotation in the same pass, on
+B200 (sm_100a).
+
+    qk_norm_rope(qkv, q_weight, k_weight, eps, positions, cos_sin, heads, kv_heads) -> (q, k)
+
+is the step between the qkv linear of a Qwen3-shaped layer and its attention: each head is
+normalised over its own values, scaled by its weight and rotated by its token's position.
+The kernel is csrc/qk_norm.cu behind the C ABI; float32 inside, one rounding at the end.
+The reference package (AshrithaG/int8-linear) leaves this step to vLLM.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from int8_linear import _native
+from int8_linear._native import NotSupported
+from int8_linear.fused_quant import _ACT, _WEIGHT
+from int8_linear.kernel import current_stream
+
+__all__ = ["qk_norm_rope"]
+
+
+def _out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor, name: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if tuple(out.shape) != shape or out.dtype != like.dtype or out.device != like.device \
+            or out.stride(2) != 1 or out.stride(1) != shape[2]:
+        raise ValueError(f"{name} must be a {like.dtype} {list(shape)} tensor on {like.device} whose heads "
+                         f"follow one another, got {out.dtype} {tuple(out.shape)} strides {out.stride()}")
+    return out
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
+                 positions: torch.Tensor, cos_sin: torch.Tensor, heads: int, kv_heads: int, *,
+                 interleaved: bool = False, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q [M, heads, D], k [M, kv_heads, D]) of a bf16/fp16 qkv [M, >= (heads + kv_heads) D].
+
+    A row of qkv holds the query heads, then the key heads; what follows is left alone.
+    For each head, n = x / sqrt(mean(x^2) + eps) * weight, then the first R values of n
+    are rotated in pairs (a, b) -> (a cos - b sin, b cos + a sin).  D is the weights'
+    length; `positions` [M] (int32 or int64) picks the rows of `cos_sin` [positions, R],
+    R/2 cosines followed by R/2 sines (bf16, fp16 or fp32).  Pair i is (n[i], n[i + R/2]),
+    or (n[2i], n[2i + 1]) with `interleaved`.  A token whose position is not a row of
+    cos_sin comes out as NaN.
+
+    `q_out` and `k_out` are [M, heads, D] tensors to write into, any distance between
+    tokens; they may be the heads' own places in qkv
+    (`qkv[:, :heads * D].view(M, heads, D)`), but overlap it in no other way.
+
+    Takes D a multiple of 8 up to 256, R a multiple of 16 (8 with interleaved) up to D and
+    16-byte aligned rows; raises NotSupported for others, ValueError for inconsistent
+    arguments.  R = 0 only normalises."""
+    if qkv.dtype not in _ACT:
+        raise NotSupported(f"activations must be bfloat16 or float16, got {qkv.dtype}")
+    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        raise NotSupported("qkv must be a 2-D activation with contiguous rows")
+    m, width = qkv.shape
+    d = q_weight.numel()
+    if q_weight.dtype not in _WEIGHT or k_weight.dtype != q_weight.dtype or k_weight.numel() != d or d == 0:
+        raise ValueError(f"q_weight and k_weight must hold one head's values in one bf16/fp16/fp32 type, got "
+                         f"{q_weight.dtype} {tuple(q_weight.shape)} and {k_weight.dtype} {tuple(k_weight.shape)}")
+    if heads < 0 or kv_heads < 0 or width < (heads + kv_heads) * d:
+        raise ValueError(f"qkv rows of {width} values do not hold {heads} + {kv_heads} heads of {d}")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (m,):
+        raise ValueError(f"positions must be {m} int32 or int64 values, got {positions.dtype} "
+                         f"{tuple(positions.shape)}")
+    if cos_sin.dim() != 2 or cos_sin.dtype not in _WEIGHT or cos_sin.shape[1] > d or cos_sin.shape[1] % 2:
+        raise ValueError(f"cos_sin must be a bf16/fp16/fp32 [positions, even rot <= {d}] table, got "
+                         f"{cos_sin.dtype} {tuple(cos_sin.shape)}")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("positions", positions),
+                    ("cos_sin", cos_sin)):
+        if t.device != qkv.device:
+            raise ValueError(f"{name} is on {t.device}, qkv on {qkv.device}")
+    if not qkv.is_cuda:
+        raise ValueError(f"qk_norm_rope runs on a CUDA device, got {qkv.device}")
+    q = _out(q_out, (m, heads, d), qkv, "q_out")
+    k = _out(k_out, (m, kv_heads, d), qkv, "k_out")
+    if m == 0 or heads + kv_heads == 0:
+        return q, k
+    wq, wk, pos, table = (t if t.is_contiguous() else t.contiguous()
+                          for t in (q_weight, k_weight, positions, cos_sin))
+    dev = qkv.get_device()
+    args = (qkv.data_ptr(), qkv.stride(0), _ACT[qkv.dtype], wq.data_ptr(), wk.data_ptr(), _WEIGHT[wq.dtype],
+            eps, pos.data_ptr(), pos.dtype == torch.int64, table.data_ptr(), _WEIGHT[table.dtype],
+            table.shape[0], q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), m, heads, kv_heads, d,
+            table.shape[1], interleaved, current_stream(dev))
+    _native.on_device(dev, _native.load().i8l_qk_norm_rope, args)
+    return q, k
