@@ -334,6 +334,19 @@ int i8l_dequant_mxfp4(const uint8_t *q, int64_t ldq, const uint8_t *scale, void 
                       int32_t out_dtype, int32_t M, int32_t K, void *stream);
 
 /*
+ * out[M,N] = cast(A[M,K] @ W[N,K]^T + bias) for 4-bit A and W, float32 accumulation on
+ * the tcgen05 tensor cores.  A and W: codes at lda/ldw bytes a row and scales as above,
+ * all 16-byte aligned.  bias NULL or N values of bias_dtype (I8L_BF16/F16/F32); out rows
+ * at ldc elements of out_dtype (I8L_BF16/F16/F32).  The result of a shape and tile does
+ * not vary from run to run.  tile: NULL or zeroed for the library's choice; of a given
+ * one, tok_tile, cluster and stages count.
+ */
+int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, const uint8_t *W, int64_t ldw,
+                const uint8_t *sw, const void *bias, int32_t bias_dtype, void *out,
+                int32_t out_dtype, int64_t ldc, int32_t M, int32_t N, int32_t K,
+                const i8l_tile *tile, void *stream);
+
+/*
  * RMSNorm of every query and key head of a qkv product and its rotation by the token's
  * position, in one pass:
  *     n = x / sqrt(mean(x^2) + eps) * weight          (per head, in float32)

@@ -80,6 +80,8 @@ SIGNATURES = {
     "i8l_add_rmsnorm_quant_mxfp4": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i32, _vp, _i64, _vp, _vp, _i64,
                                            _i32, _i32, _f64, _vp]),
     "i8l_dequant_mxfp4": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
+    "i8l_w4a4_mm": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i64, _i32, _i32, _i32,
+                           ctypes.POINTER(I8LTile), _vp]),
     "i8l_qk_norm_rope": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _f32, _vp, _i32, _vp, _i32, _i64, _vp, _i64,
                                 _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "i8l_last_error": (ctypes.c_char_p, []),

@@ -38,6 +38,7 @@
 #include "common.cuh"
 #include "epilogue.cuh"
 #include "internal.h"
+#include "tmap.h"
 
 namespace i8l {
 
@@ -1386,25 +1387,6 @@ __global__ void __launch_bounds__(kThreads, (TN <= 64 || kVar == kVarNarrow) ? 2
 
 // ------------------------------------------------------------------ host side
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                  const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
 // Tensor map over an int8 [rows, K] matrix with row stride `ld` bytes, boxes of
 // 128 bytes along K by `box_rows` rows, 128-byte swizzle, zero fill outside.
 static int make_operand_map(CUtensorMap *map, const int8_t *ptr, int64_t rows, int64_t k,
@@ -1422,27 +1404,6 @@ static int make_operand_map(CUtensorMap *map, const int8_t *ptr, int64_t rows, i
     return set_error(I8L_ECUDA, "cuTensorMapEncodeTiled failed (CUresult %d) for [%lld x %lld], ld %lld",
                      static_cast<int>(r), static_cast<long long>(rows), static_cast<long long>(k),
                      static_cast<long long>(ld));
-  return I8L_OK;
-}
-
-// Tensor map over a row-major 2-D matrix of `rows` x `cols` elements (row stride
-// `ld_bytes`), boxes of box_cols x box_rows.
-static int make_map(CUtensorMap *map, CUtensorMapDataType type, const void *ptr, int64_t rows,
-                    int64_t cols, int64_t ld_bytes, int box_cols, int box_rows,
-                    CUtensorMapSwizzle swizzle, const char *what) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return set_error(I8L_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld_bytes)};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, type, 2, const_cast<void *>(ptr), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return set_error(I8L_ECUDA, "cuTensorMapEncodeTiled failed (CUresult %d) for the %s map [%lld x %lld]",
-                     static_cast<int>(r), what, static_cast<long long>(rows),
-                     static_cast<long long>(cols));
   return I8L_OK;
 }
 

@@ -332,8 +332,6 @@ int finish_launch(cudaError_t err, const char *what) {
   return e == cudaSuccess ? I8L_OK : cuda_error(e, what);
 }
 
-constexpr int kMxMaxK = 1 << 26;  // 128 rows of vectors fit a flat kernel's 31-bit index
-
 // Shape and output checks that the quantisers share.
 int check_mx(int32_t M, int32_t K, const void *q, int64_t ldq, const void *sf) {
   if (M < 0 || K < 0) return set_error(I8L_EINVAL, "negative size M=%d K=%d", M, K);

@@ -18,6 +18,7 @@ namespace i8l {
 
 constexpr int kMxBlock = 32;       // values per scale
 constexpr int kSfTileBytes = 512;  // 128 rows x 4 blocks
+constexpr int kMxMaxK = 1 << 26;   // 128 rows of eight-value vectors fit a 31-bit index
 
 // Byte offset of the word that holds the scales of blocks 4*kt .. 4*kt+3 of a row.
 __host__ __device__ __forceinline__ long long sf_word_offset(long long row, int kt, int ktiles) {
@@ -41,6 +42,56 @@ __device__ __forceinline__ float mx_inv_scale(uint32_t byte) { return __uint_as_
 // 2^(byte - 127), NaN for 0xFF; 2^-127 is a float32 subnormal.
 __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : (byte == 0u ? 0x00400000u : byte << 23));
+}
+
+// ---------------------------------------------------------------- tensor cores
+// tcgen05.mma.kind::mxf4 multiplies packed e2m1 tiles, 64 values (32 bytes) of K per
+// instruction, with the scales of both operands in TMEM: a scale tile (128 rows x 4 blocks)
+// is four columns there, row r in lane r % 32 of column r / 32, its four blocks in the four
+// bytes; an instruction takes two of the bytes, chosen by the scale ids of its descriptor.
+
+// One 512-byte scale tile from shared memory into four TMEM columns, replicated to the
+// lanes of all four warps; in order with this thread's later tcgen05.mma.
+__device__ __forceinline__ void sf_to_tmem(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// The same in both CTAs of a pair, each from its own shared memory.
+__device__ __forceinline__ void sf_to_tmem_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Shared-memory descriptor of a scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups
+// 128 bytes apart.
+__device__ __forceinline__ uint64_t sf_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(1) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+
+// Instruction descriptor: e2m1 x e2m1 with e8m0 scales, both K-major; `sf_id` (0 or 2) is
+// the first of the two scale bytes, the same in both operands.
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int sf_id) {
+  return (static_cast<uint32_t>(sf_id) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) | (static_cast<uint32_t>(sf_id) << 29);
+}
+
+// D[tmem] (+)= A * B, 64 values of K.
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                         uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+      : "memory");
+}
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+      : "memory");
 }
 
 // Eight values times `inv`, rounded to e2m1 (nearest, ties to even, saturating), packed

@@ -28,17 +28,19 @@ torch custom ops too, under torch.ops.int8_linear.  The reference package
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from int8_linear import _native
 from int8_linear._native import NotSupported
 from int8_linear.fused_quant import _ACT, _WEIGHT
-from int8_linear.kernel import current_stream
+from int8_linear.kernel import Config, current_stream
 
 BLOCK = 32
 _FLOAT = _WEIGHT  # bf16, fp16 and fp32
 
-__all__ = ["quant_mxfp4", "add_rmsnorm_quant_mxfp4", "silu_mul_quant_mxfp4", "dequant_mxfp4"]
+__all__ = ["w4a4_mm", "quant_mxfp4", "add_rmsnorm_quant_mxfp4", "silu_mul_quant_mxfp4", "dequant_mxfp4"]
 
 
 def _rows(x: torch.Tensor, name: str, kinds: dict) -> tuple[int, int]:
@@ -146,6 +148,82 @@ def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = tor
         _native.on_device(dev, _native.load().i8l_dequant_mxfp4, (
             q.data_ptr(), q.stride(0), sc.data_ptr(), out.data_ptr(), k, _FLOAT[out_dtype], m, k,
             current_stream(dev)))
+    return out
+
+
+SPLIT_TILES = (16, 32, 64, 128)
+
+
+def _tile(config: Config) -> _native.I8LTile:
+    """The C tile of a Config for the 4-bit product: swap_ab token tiles with split 0, 1 or 3."""
+    if config.split not in (0, 1, 3) or not config.swapped or config.bm not in SPLIT_TILES or config.bn != 128:
+        raise NotSupported(f"{config.name}: 4-bit tiles are bm in {SPLIT_TILES} x bn 128 with swap_ab")
+    return _native.I8LTile(swap_ab=1, tok_tile=config.bm, w_tile=128, stages=config.stages, split=config.split,
+                           cluster=1 if config.split == 1 else config.cluster)
+
+
+def _aligned16(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it if its rows do not start on 16-byte boundaries (what TMA needs)."""
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+            out_dtype: torch.dtype = torch.bfloat16, bias: torch.Tensor | None = None, *,
+            config: Config | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A @ W^T + bias [M, N] for 4-bit A [M, K] and W [N, K].
+
+    As w8a8_mm, with 4-bit operands: a_q is [M, K/2] codes, b_q the transposed view
+    [K/2, N] of a weight's [N, K/2] codes (`w_q.t()`), scale_a and scale_b their scale tiles
+    as quant_mxfp4 gives them.  The sum is float32 on the tensor cores, bias (bf16, fp16 or
+    fp32, [N]) is added in float32, and one rounding makes the bf16, fp16 or fp32 output.
+    `out` is an [M, N] tensor with contiguous rows to write into.  `config` picks a tiling
+    (swap_ab token tiles of 16 to 128, split 1 or 3, cluster, stages) in place of the
+    library's choice.  Raises NotSupported for what the kernel does not take and ValueError
+    for inconsistent arguments."""
+    if a_q.dtype != torch.uint8 or b_q.dtype != torch.uint8:
+        raise NotSupported(f"uint8 4-bit codes only, got {a_q.dtype} and {b_q.dtype}")
+    if a_q.dim() != 2 or b_q.dim() != 2 or a_q.shape[1] != b_q.shape[0]:
+        raise ValueError(f"cannot multiply {tuple(a_q.shape)} by {tuple(b_q.shape)}")
+    m, half = a_q.shape
+    n, k = b_q.shape[1], 2 * half
+    if k == 0 or k % BLOCK:
+        raise NotSupported(f"K={k} must be a positive multiple of {BLOCK} (whole blocks)")
+    if n > 1 and b_q.stride(0) != 1:
+        raise NotSupported("b_q must be the K-contiguous [K/2, N] view of an [N, K/2] weight")
+    _operand(a_q, scale_a, m, k, "scale_a")
+    _operand(b_q, scale_b, n, k, "scale_b")
+    if bias is not None:
+        if tuple(bias.shape) != (n,) or bias.device != a_q.device:
+            raise ValueError(f"bias must have shape ({n},) on {a_q.device}, got {tuple(bias.shape)} on {bias.device}")
+        if bias.dtype not in _FLOAT:
+            raise NotSupported(f"bias dtype {bias.dtype} not supported")
+        bias = bias if bias.is_contiguous() else bias.contiguous()
+    if out_dtype not in _FLOAT:
+        raise NotSupported(f"output dtype {out_dtype} not supported")
+    if not a_q.is_cuda or b_q.device != a_q.device:
+        raise ValueError(f"w4a4_mm runs on one CUDA device; got tensors on {a_q.device} and {b_q.device}")
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype, device=a_q.device)
+    elif tuple(out.shape) != (m, n) or out.dtype != out_dtype or out.device != a_q.device \
+            or (n > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be a {out_dtype} [{m}, {n}] tensor with contiguous rows on "
+                         f"{a_q.device}, got {out.dtype} {tuple(out.shape)} strides {out.stride()}")
+    tile = _tile(config) if config is not None else None
+    if m == 0 or n == 0:
+        return out
+    a, w = _aligned16(a_q), b_q.t()
+    if b_q.data_ptr() % 16 or b_q.stride(1) % 16:
+        w = _aligned16(w)
+    sa, sb = (s if s.is_contiguous() and s.data_ptr() % 16 == 0 else s.clone(memory_format=torch.contiguous_format)
+              for s in (scale_a, scale_b))
+    dev = a_q.get_device()
+    _native.on_device(dev, _native.load().i8l_w4a4_mm, (
+        a.data_ptr(), a.stride(0), sa.data_ptr(), w.data_ptr(), w.stride(0), sb.data_ptr(),
+        bias.data_ptr() if bias is not None else None, _FLOAT[bias.dtype] if bias is not None else 0,
+        out.data_ptr(), _FLOAT[out_dtype], out.stride(0), m, n, k,
+        ctypes.byref(tile) if tile is not None else None, current_stream(dev)))
     return out
 
 
