@@ -1816,7 +1816,9 @@ static int gemm_run(const int8_t *A, int64_t lda, const int8_t *W, int64_t ldw, 
                         ? 2
                         : (tile && tile->store ? tile->store : ((swap && M <= 32) ? 2 : 1));
   CUtensorMap mo{}, mw{};
-  if (aligned_out && store == 1) {
+  // A TMA store ends a row at a 16-byte boundary, with zeros past the last column: rows that
+  // end elsewhere (an `out` inside wider rows) are stored plainly.
+  if (aligned_out && store == 1 && (static_cast<int64_t>(N) * esize) % 16 == 0) {
     static const CUtensorMapDataType kTypes[4] = {
         CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
         CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_INT32};
