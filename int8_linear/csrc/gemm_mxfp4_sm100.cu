@@ -38,6 +38,8 @@ struct MxGemmArgs {
   int out_dtype;
   long long ldc;
   int vec_store;        // four consecutive outputs of a row may be stored at once
+  int tma_out;          // pair tiles: outputs leave through shared memory by TMA stores
+  int group;            // pair tiles: token tiles that walk over the weight together
   int *status;
 };
 
@@ -285,11 +287,330 @@ __global__ void __launch_bounds__(kSplitThreads)
   }
 }
 
+// ------------------------------------------------------------------ pair tiles
+
+constexpr int kPairThreads = 192;  // producer, MMA issuer, four epilogue warps
+constexpr int kPairEpi = 4;
+constexpr int kPairN = 256;        // weight rows of a tile; each CTA holds half of them
+constexpr int kPairXBytes = kMxRows * kMxRowBytes;
+constexpr int kPairYBytes = kPairN / 2 * kMxRowBytes;
+constexpr int kPairStageBytes = kPairXBytes + kPairYBytes + 3 * kSfStageBytes;
+constexpr int kPairBufBytes = 2048;                              // 32 rows x 64 bytes of output
+constexpr int kPairStaging = kPairEpi * 2 * kPairBufBytes;
+// TMEM columns: two accumulators of 256 columns that share 32 of them, then the scales of
+// one stage (8 for the tokens' 128 rows, 16 for the weight's 256).
+constexpr int kPairAcc1 = 224;
+constexpr int kPairSf = 480;
+
+static size_t pair_smem(int stages) {
+  return 1024 /* alignment slack */ + static_cast<size_t>(stages) * kPairStageBytes + kPairStaging +
+         2 * kPairN * 4 /* bias, per accumulator */ + static_cast<size_t>(2 * stages + 6) * 8 + 16;
+}
+
+// Tile index -> (token tile, weight tile): `group` token tiles walk over the weight tiles
+// together, so that the pairs running at one time share operands in L2.
+__device__ __forceinline__ void pair_coords(const MxGemmArgs &a, int t, int &tm, int &tn) {
+  const int per_group = a.group * a.tiles_n;
+  const int g = t / per_group, first = g * a.group;
+  const int gsz = min(a.tiles_m - first, a.group);
+  const int r = t - g * per_group;
+  tm = first + r % gsz;
+  tn = r / gsz;
+}
+
+// One 32-column chunk of this thread's token row: bias, rounding, and the store through the
+// warp's staging buffer (64-byte rows in the 64-byte swizzle, one TMA store) or straight to
+// memory.
+__device__ __forceinline__ void pair_emit(const MxGemmArgs &a, const CUtensorMap *map_out, int m0, int n0, int lane,
+                                          const float *bias, const uint32_t (&r0)[16], const uint32_t (&r1)[16],
+                                          uint8_t *staging, uint32_t &count) {
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    v[j] = __uint_as_float(r0[j]);
+    v[16 + j] = __uint_as_float(r1[j]);
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 b = *reinterpret_cast<const float4 *>(bias + j);
+      v[j] += b.x;
+      v[j + 1] += b.y;
+      v[j + 2] += b.z;
+      v[j + 3] += b.w;
+    }
+  }
+  if (a.tma_out) {
+    const int halves = a.out_dtype == I8L_F32 ? 2 : 1;  // boxes of 16 float32 or 32 16-bit columns
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h >= halves) break;
+      if (count >= 2 && lane == 0) bulk_wait_read<1>();
+      __syncwarp();
+      uint8_t *buf = staging + (count & 1u) * kPairBufBytes;
+      ++count;
+      uint32_t w[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        w[j] = halves == 2 ? __float_as_uint(v[16 * h + j]) : pack16x2(a.out_dtype, v[2 * j], v[2 * j + 1]);
+      uint8_t *rowp = buf + lane * 64;
+      const int sw = (lane >> 1) & 3;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4 *>(rowp + ((c ^ sw) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        const int n = n0 + 16 * h;
+        if (n < a.N && m0 < a.M) tma_store_2d(map_out, buf, n, m0);  // skip boxes wholly outside
+        bulk_commit();
+      }
+    }
+  } else if (m0 + lane < a.M) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float q[4] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
+      if (n0 + j < a.N) store_out4(a, m0 + lane, n0 + j, q);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+    mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                   const __grid_constant__ CUtensorMap map_sfx, const __grid_constant__ CUtensorMap map_sfy,
+                   const __grid_constant__ CUtensorMap map_out, const MxGemmArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int S = a.stages;
+  uint8_t *sx = smem, *sy = sx + S * kPairXBytes, *ssx = sy + S * kPairYBytes, *ssy = ssx + S * kSfStageBytes;
+  uint8_t *staging = ssy + S * 2 * kSfStageBytes;
+  float *bias_cols = reinterpret_cast<float *>(staging + kPairStaging);
+  uint64_t *full = reinterpret_cast<uint64_t *>(bias_cols + 2 * kPairN);
+  uint64_t *empty = full + S, *acc_full = empty + S, *acc_empty = acc_full + 2, *shared_free = acc_empty + 2,
+           *drain = shared_free + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = static_cast<int>(blockIdx.x & 1u);
+  const bool leader = rank == 0;
+  const int first_tile = static_cast<int>(blockIdx.x >> 1), step = static_cast<int>(gridDim.x >> 1);
+  const int total = a.tiles_m * a.tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 2 * kPairEpi);  // both CTAs' epilogue warps
+    }
+    mbar_init(shared_free, 2 * kPairEpi);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_y);
+    tma_prefetch_desc(&map_sfx);
+    tma_prefetch_desc(&map_sfy);
+    if (a.tma_out) tma_prefetch_desc(&map_out);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  cluster_sync();  // both CTAs' barriers and TMEM are set up before either signals the other
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol = policy_evict_last();
+      const uint32_t tx = 2u * kPairStageBytes;  // both CTAs' loads, counted on the even CTA's barrier
+      auto load_w = [&](int st, int kb, int tn) {
+        const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
+        tma_load_2d_pair(sy + st * kPairYBytes, &map_y, bar, kb * kMxRowBytes, tn * kPairN + rank * (kPairN / 2), pol);
+        tma_load_2d_pair(ssy + st * 2 * kSfStageBytes, &map_sfy, bar, kb * 2 * kSfWords, tn * 2, pol);
+      };
+      auto load_a = [&](int st, int kb, int tm) {
+        const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
+        tma_load_2d_pair(sx + st * kPairXBytes, &map_x, bar, kb * kMxRowBytes, (2 * tm + rank) * kMxRows, pol);
+        tma_load_2d_pair(ssx + st * kSfStageBytes, &map_sfx, bar, kb * 2 * kSfWords, 2 * tm + rank, pol);
+      };
+      // The first tile's weight stages do not wait for the previous kernel.
+      int tm, tn, pre = 0;
+      if (first_tile < total) {
+        pair_coords(a, first_tile, tm, tn);
+        for (; pre < min(S, a.kblocks); ++pre) {
+          if (leader) mbar_arrive_expect_tx(&full[pre], tx);
+          load_w(pre, pre, tn);
+        }
+      }
+      pdl_wait();
+      bool ok = true;
+      int st = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      for (int t = first_tile; ok && t < total; t += step) {
+        pair_coords(a, t, tm, tn);
+        for (int kb = 0; kb < a.kblocks; ++kb) {
+          if (issued >= pre) {
+            if (!mbar_wait_bounded(&empty[st], phase ^ 1u, abort_flag, a.status, kStatusProducerWait)) {
+              ok = false;
+              break;
+            }
+            if (leader) mbar_arrive_expect_tx(&full[st], tx);
+            load_w(st, kb, tn);
+          }
+          load_a(st, kb, tm);
+          ++issued;
+          if (++st == S) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok && leader) {
+        // Let the loads already issued land; the odd CTA stays until the even one leaves.
+        for (long long i = 0; i < (issued < S ? issued : S); ++i) {
+          if (--st < 0) {
+            st = S - 1;
+            phase ^= 1u;
+          }
+          volatile int no_abort = 0;
+          mbar_wait_bounded(&full[st], phase, &no_abort, a.status, kStatusDrainWait);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      bool ok = true, any = false;
+      int st = 0, n = 0;
+      uint32_t phase = 0;
+      for (int t = first_tile; ok && t < total; t += step, ++n) {
+        const int acc = n & 1;
+        // This accumulator's last tile has been read, and so have the columns that it
+        // shares with the other accumulator's tile.
+        if (!mbar_wait_bounded(&acc_empty[acc], ((n >> 1) & 1) ^ 1, abort_flag, a.status, kStatusMmaWait) ||
+            (n > 0 && !mbar_wait_bounded(shared_free, (n - 1) & 1, abort_flag, a.status, kStatusMmaWait))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + (acc ? kPairAcc1 : 0), sf = tmem + kPairSf;
+        for (int kb = 0; kb < a.kblocks; ++kb) {
+          if (!mbar_wait_bounded(&full[st], phase, abort_flag, a.status, kStatusMmaWait)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int steps = min(4, (a.K - kb * kMxStageK + 63) / 64);
+          const uint64_t ad = sw128_kmajor_desc(smem_u32(sx + st * kPairXBytes));
+          const uint64_t bd = sw128_kmajor_desc(smem_u32(sy + st * kPairYBytes));
+          const uint64_t xd = sf_desc(smem_u32(ssx + st * kSfStageBytes));
+          const uint64_t yd = sf_desc(smem_u32(ssy + st * 2 * kSfStageBytes));
+          constexpr uint64_t kTileStep = kSfTileBytes >> 4;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (2 * h < steps) {
+              sf_to_tmem_pair(sf + 4 * h, xd + h * kTileStep);
+              sf_to_tmem_pair(sf + 8 + 8 * h, yd + h * kTileStep);
+              sf_to_tmem_pair(sf + 12 + 8 * h, yd + (2 + h) * kTileStep);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k < steps)
+              mma_mxf4_pair(d, ad + 2 * k, bd + 2 * k,
+                            k & 1 ? idesc_mxf4(2 * kMxRows, kPairN, 2) : idesc_mxf4(2 * kMxRows, kPairN, 0),
+                            sf + 4 * (k >> 1), sf + 8 + 8 * (k >> 1), kb == 0 && k == 0 ? 0u : 1u);
+          }
+          any = true;
+          mma_commit_pair_mc(&empty[st], 0x3);
+          if (++st == S) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        mma_commit_pair_mc(&acc_full[acc], 0x3);
+      }
+      if (!ok && any) {
+        mma_commit_pair(drain);
+        volatile int no_abort = 0;
+        mbar_wait_bounded(drain, 0, &no_abort, a.status, kStatusDrainWait);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;  // TMEM lanes this warp may access
+    const int tid = threadIdx.x - 64;
+    auto release = [&](uint64_t *bar) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader)
+          mbar_arrive(bar);
+        else
+          mbar_arrive_remote(map_to_rank(smem_u32(bar), 0));
+      }
+    };
+    pdl_wait();
+    uint8_t *buf = staging + quarter * 2 * kPairBufBytes;
+    uint32_t count = 0;
+    int n = 0;
+    for (int t = first_tile; t < total; t += step, ++n) {
+      int tm, tn;
+      pair_coords(a, t, tm, tn);
+      const int acc = n & 1;
+      const int m0 = (2 * tm + rank) * kMxRows + quarter * 32, n0 = tn * kPairN;
+      const int ncols = min(kPairN, a.N - n0);
+      float *bias = bias_cols + acc * kPairN;
+      if (a.bias)
+        for (int c = tid; c < kPairN; c += kPairEpi * 32)
+          bias[c] = c < ncols ? load_scalar_f(a.bias, a.bias_dtype, n0 + c) : 0.f;
+      const bool ok = mbar_wait_bounded(&acc_full[acc], (n >> 1) & 1, abort_flag, a.status, kStatusEpilogueWait);
+      // All four warps go on or all stop; the barrier also publishes the bias columns.
+      if (!named_bar_and(2, kPairEpi * 32, ok)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? kPairAcc1 : 0);
+      // The shared columns first: the last chunk of accumulator 0, the first of 1.
+      for (int i = 0; i < kPairN / 32; ++i) {
+        const int c0 = acc ? 32 * i : (i == 0 ? kPairN - 32 : 32 * (i - 1));
+        uint32_t r0[16], r1[16];
+        const bool live = c0 < ncols;
+        if (live) {
+          tmem_ld16(taddr + c0, r0);
+          tmem_ld16(taddr + c0 + 16, r1);
+          tmem_ld_wait();
+        }
+        if (i == 0) release(shared_free);
+        if (i == kPairN / 32 - 1) release(&acc_empty[acc]);
+        if (live) pair_emit(a, &map_out, m0, n0 + c0, lane, bias + c0, r0, r1, buf, count);
+      }
+    }
+    if (lane == 0) bulk_wait<0>();
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  // Neither CTA leaves while the other may still signal it or read its shared memory.
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
 // ------------------------------------------------------------------ host side
 
 struct MxPlan {
-  int tn;       // tokens per split tile
-  int cluster;  // CTAs sharing a tile's K
+  int pair;     // CTA pairs on 256 x 256 tiles
+  int tn;       // tokens per tile
+  int cluster;  // split tiles: CTAs sharing a tile's K
   int stages;
 };
 
@@ -325,6 +646,19 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   DeviceInfo di;
   if (int e = device_info(&di)) return e;
   const int kblocks = (K + kMxStageK - 1) / kMxStageK;
+  *p = MxPlan{};
+  if (tile && tile->split == 4 ? true : !(tile && (tile->tok_tile || tile->split)) && M > 256) {
+    if (tile && tile->split == 4 && (tile->swap_ab || tile->tok_tile != 128 || tile->w_tile != 256))
+      return set_error(I8L_ENOTSUP, "CTA pairs (split 4) take tok_tile 128 x w_tile 256 tiles without swap_ab");
+    p->pair = 1;
+    p->tn = 2 * kMxRows;
+    p->cluster = 2;
+    const int most = std::min(16, (di.max_smem_optin - static_cast<int>(pair_smem(0))) / (kPairStageBytes + 16));
+    p->stages = tile && tile->stages ? tile->stages : most;
+    if (p->stages < 2 || p->stages > most)
+      return set_error(I8L_ENOTSUP, "stages %d outside [2, %d] for this tile", p->stages, most);
+    return I8L_OK;
+  }
   p->tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   if (tile && tile->tok_tile) p->tn = tile->tok_tile;
   if (p->tn != 16 && p->tn != 32 && p->tn != 64 && p->tn != 128)
@@ -382,12 +716,15 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
     return set_error(I8L_ENOTSUP, "bias dtype code %d not supported", bias_dtype);
   MxPlan p;
   if (int e = make_mx_plan(M, N, K, tile, &p)) return e;
+  DeviceInfo di;
+  if (int e = device_info(&di)) return e;
   MxGemmArgs a{};
   a.M = M;
   a.N = N;
   a.K = K;
   a.kblocks = (K + kMxStageK - 1) / kMxStageK;
-  a.tiles_n = (N + kMxRows - 1) / kMxRows;
+  const int w_rows = p.pair ? kPairN : kMxRows;
+  a.tiles_n = (N + w_rows - 1) / w_rows;
   a.tiles_m = (M + p.tn - 1) / p.tn;
   a.cluster = p.cluster;
   a.stages = p.stages;
@@ -400,9 +737,37 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
   a.vec_store = reinterpret_cast<uintptr_t>(out) % (4 * esize) == 0 && ldc % 4 == 0 ? 1 : 0;
   a.status = status_ptr();
   CUtensorMap mx, my, msx, msy;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (static_cast<int64_t>(a.tiles_m) * a.tiles_n * p.cluster > INT32_MAX)
+    return set_error(I8L_ENOTSUP, "%d x %d outputs are too many tiles", M, N);
+  if (p.pair) {
+    if (int e = operand_maps(&mx, &msx, A, lda, sa, M, K, kMxRows, 1)) return e;
+    if (int e = operand_maps(&my, &msy, W, ldw, sw, N, K, kPairN / 2, 2)) return e;
+    CUtensorMap mo{};
+    // A TMA store ends a row at a 16-byte boundary, with zeros past the last column, so rows
+    // that end elsewhere are stored plainly.
+    if (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldc * esize) % 16 == 0 &&
+        (static_cast<int64_t>(N) * esize) % 16 == 0) {
+      static const CUtensorMapDataType kTypes[3] = {CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                                    CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
+      if (int e = make_map(&mo, kTypes[out_dtype], out, M, N, ldc * esize, 64 / esize, 32, CU_TENSOR_MAP_SWIZZLE_64B,
+                           "output"))
+        return e;
+      a.tma_out = 1;
+    }
+    a.group = std::min(8, a.tiles_m);
+    static size_t configured[64] = {};
+    const size_t smem = pair_smem(a.stages);
+    if (int e = allow_smem(mx_pair_kernel, smem, configured)) return e;
+    const int pairs = std::min(a.tiles_m * a.tiles_n, (tile && tile->ctas ? tile->ctas : di.sms) / 2);
+    cudaError_t e = launch(mx_pair_kernel, dim3(2 * std::max(1, pairs)), dim3(kPairThreads), smem, s, 2, mx, my, msx,
+                           msy, mo, a);
+    if (e != cudaSuccess) return cuda_error(e, "mxfp4 gemm launch");
+    e = cudaGetLastError();
+    return e == cudaSuccess ? I8L_OK : cuda_error(e, "mxfp4 gemm launch");
+  }
   if (int e = operand_maps(&mx, &msx, W, ldw, sw, N, K, kMxRows, 1)) return e;
   if (int e = operand_maps(&my, &msy, A, lda, sa, M, K, p.tn, 1)) return e;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (p.tn) {
     case 16: return launch_split<16>(mx, my, msx, msy, a, s);
     case 32: return launch_split<32>(mx, my, msx, msy, a, s);

@@ -64,6 +64,14 @@ def test_every_split_tile(tn, cluster, stages):
         exact(200, 200, 2336, cfg, seed=cluster)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (128, 256, 256), (256, 256, 64), (257, 513, 1056), (300, 40, 2336),
+                                   (1000, 1000, 992), (2600, 3000, 288)])
+@pytest.mark.parametrize("stages,ctas", [(0, 0), (2, 0), (3, 6)])
+def test_pair_tiles(m, n, k, stages, ctas):
+    """Few pairs make each one walk over many tiles, through both accumulators."""
+    exact(m, n, k, Config(128, 256, split=4, stages=stages, ctas=ctas))
+
+
 def test_scale_bytes_of_no_row_do_not_matter():
     exact(5, 130, 160, nan_pad=True)
     exact(140, 130, 160, nan_pad=True)
@@ -97,7 +105,7 @@ def test_quantised_operands(m, n, k, dtype):
     near(a, sa, va, b, sb, vb, dtype, rand((n,), 3, 0.1, dtype))
 
 
-@pytest.mark.parametrize("m,n,k", [(9, 130, 320), (130, 70, 320)])
+@pytest.mark.parametrize("m,n,k", [(9, 130, 320), (130, 70, 320), (300, 270, 320)])
 def test_strides_pointers_and_out(m, n, k):
     """Rows of wider matrices, pointers that TMA cannot take (copied), an unaligned or
     strided out, whose other bytes stay as they were."""
@@ -129,6 +137,8 @@ def test_nan_blocks_reach_their_rows_and_columns_only():
     a, sa = mxfp4.quant_mxfp4(x)
     b, sb = mxfp4.quant_mxfp4(w)
     got = mxfp4.w4a4_mm(a, b.t(), sa, sb)
+    pair = mxfp4.w4a4_mm(a, b.t(), sa, sb, config=Config(128, 256, split=4))
+    assert torch.equal(got.isnan(), pair.isnan())
     want = torch.zeros((40, 200), dtype=torch.bool, device="cuda")
     want[7], want[:, 150] = True, True
     assert torch.equal(got.isnan(), want) and torch.isfinite(got[~want]).all()
