@@ -10,6 +10,15 @@
 // partial tile in its own shared memory; after a cluster barrier each CTA adds, for its
 // share of the outputs, every CTA's partial in rank order through distributed shared
 // memory.  So a shape's result does not vary from run to run.
+//
+// Pair tiles (mx_pair_kernel), for larger batches, bound by the tensor cores: two CTAs on
+// two SMs compute tiles of 256 tokens x 256 weight rows with cta_group::2 MMAs, each loading
+// half of both operands' rows, so an SM fills 32 KB per 256 values of K where one CTA alone
+// would need 48.  Scales: each CTA holds its own tokens' and, since it computes every column
+// of its 128 rows, the whole weight tile's.  TMEM's 512 columns do not hold two accumulators
+// of 256 and the scales, so every other tile has 192 weight rows: 256 + 192 columns of
+// accumulators leave 64 for the scales, and one tile's epilogue runs beside the next tile's
+// MMAs.  XXXPAIR
 #include <algorithm>
 
 #include "common.cuh"
@@ -39,7 +48,7 @@ struct MxGemmArgs {
   long long ldc;
   int vec_store;        // four consecutive outputs of a row may be stored at once
   int tma_out;          // pair tiles: outputs leave through shared memory by TMA stores
-  int group;            // pair tiles: token tiles that walk over the weight together
+  FastDiv per_col;      // pair tiles: token tiles (a division per tile and role took 500 cycles)
   int *status;
 };
 
@@ -99,22 +108,23 @@ __device__ __forceinline__ void store_out4(const MxGemmArgs &a, int m, int n0, c
 // The MMAs of one stage: its scale tiles into TMEM, then up to four steps of 64 values.
 // Steps past K are left out, so a scale tile past the end is never used.
 template <int TN>
-__device__ __forceinline__ void split_stage_mmas(uint32_t d, uint32_t sf, const uint8_t *x, const uint8_t *y,
-                                                 const uint8_t *sfx, const uint8_t *sfy, int k_left, bool first) {
+__device__ __forceinline__ void split_stage_mmas(uint32_t elected, uint32_t d, uint32_t sf, uint32_t x, uint32_t y,
+                                                 uint32_t sfx, uint32_t sfy, int k_left, bool first) {
   const int steps = min(4, (k_left + 63) / 64);
-  const uint64_t ad = sw128_kmajor_desc(smem_u32(x)), bd = sw128_kmajor_desc(smem_u32(y));
+  const uint64_t ad = sw128_kmajor_desc(x), bd = sw128_kmajor_desc(y);
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     if (2 * t < steps) {
-      sf_to_tmem(sf + 4 * t, sf_desc(smem_u32(sfx + t * kSfTileBytes)));
-      sf_to_tmem(sf + 8 + 4 * t, sf_desc(smem_u32(sfy + t * kSfTileBytes)));
+      sf_to_tmem<false>(elected, sf + 4 * t, sf_desc(sfx + t * kSfTileBytes));
+      sf_to_tmem<false>(elected, sf + 8 + 4 * t, sf_desc(sfy + t * kSfTileBytes));
     }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (k < steps)
-      mma_mxf4(d, ad + 2 * k, bd + 2 * k, k & 1 ? idesc_mxf4(kMxRows, TN, 2) : idesc_mxf4(kMxRows, TN, 0),
-               sf + 4 * (k >> 1), sf + 8 + 4 * (k >> 1), first && k == 0 ? 0u : 1u);
+      mma_mxf4<false>(elected, d, ad + 2 * k, bd + 2 * k,
+                      k & 1 ? idesc_mxf4(kMxRows, TN, 2) : idesc_mxf4(kMxRows, TN, 0), sf + 4 * (k >> 1),
+                      sf + 8 + 4 * (k >> 1), first && k == 0 ? 0u : 1u);
   }
 }
 
@@ -135,7 +145,7 @@ __global__ void __launch_bounds__(kSplitThreads)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0), lane = threadIdx.x % 32;
   const int rank = a.cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int tile = static_cast<int>(blockIdx.x) / a.cluster;
   const int tx = tile % a.tiles_n, ty = tile / a.tiles_n;
@@ -162,7 +172,7 @@ __global__ void __launch_bounds__(kSplitThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_launch_dependents();
 
   if (warp == 0 && lane == 0) {
@@ -206,29 +216,29 @@ __global__ void __launch_bounds__(kSplitThreads)
         mbar_wait_bounded(&full[st], phase, &no_abort, a.status, kStatusDrainWait);
       }
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
+    const uint32_t elected = elect_one();
     bool ok = true, any = false;
     int st = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!mbar_wait_bounded(&full[st], phase, abort_flag, a.status, kStatusMmaWait)) {
-        ok = false;
-        break;
-      }
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[st], phase, abort_flag, a.status, kStatusMmaWait));
+      if (!ok) break;
       tc_fence_after();
-      split_stage_mmas<TN>(tmem, tmem + TN, sx + st * L::kXBytes, sy + st * L::kYBytes, ssx + st * kSfStageBytes,
-                           ssy + st * kSfStageBytes, a.K - kb * kMxStageK, !any);
+      split_stage_mmas<TN>(elected, tmem, tmem + TN, smem_u32(sx + st * L::kXBytes), smem_u32(sy + st * L::kYBytes),
+                           smem_u32(ssx + st * kSfStageBytes), smem_u32(ssy + st * kSfStageBytes),
+                           a.K - kb * kMxStageK, !any);
       any = true;
-      mma_commit(&empty[st]);
+      mma_commit_elected<false>(elected, smem_u32(&empty[st]));
       if (++st == S) {
         st = 0;
         phase ^= 1u;
       }
     }
     if (ok) {
-      mma_commit(done);
+      mma_commit_elected<false>(elected, smem_u32(done));
     } else if (any) {
-      mma_commit(drain);
+      mma_commit_elected<false>(elected, smem_u32(drain));
       volatile int no_abort = 0;
       mbar_wait_bounded(drain, 0, &no_abort, a.status, kStatusDrainWait);
     }
@@ -289,113 +299,143 @@ __global__ void __launch_bounds__(kSplitThreads)
 
 // ------------------------------------------------------------------ pair tiles
 
-constexpr int kPairThreads = 192;  // producer, MMA issuer, four epilogue warps
-constexpr int kPairEpi = 4;
-constexpr int kPairN = 256;        // weight rows of a tile; each CTA holds half of them
+constexpr int kPairEpi = 8;        // epilogue warps: two for each quarter of the TMEM lanes
+constexpr int kPairThreads = 64 + 32 * kPairEpi;  // and the producer and the MMA issuer
+constexpr int kPairBufBytes = 4096;  // an epilogue warp's staging: 32 rows of 128 bytes
+constexpr int kPairStaging = kPairEpi * kPairBufBytes;
+
+// Weight rows of the two kinds of tile; each CTA holds half of a tile's rows.  Along N they
+// take turns: 256 rows, 192, 256, ...
+constexpr int kWide = 256, kNarrow = 192, kBoth = kWide + kNarrow;
+constexpr int kPairSfGroups = 3;  // 128-row scale groups that a tile's rows can lie in
 constexpr int kPairXBytes = kMxRows * kMxRowBytes;
-constexpr int kPairYBytes = kPairN / 2 * kMxRowBytes;
-constexpr int kPairStageBytes = kPairXBytes + kPairYBytes + 3 * kSfStageBytes;
-constexpr int kPairBufBytes = 2048;                              // 32 rows x 64 bytes of output
-constexpr int kPairStaging = kPairEpi * 2 * kPairBufBytes;
-// TMEM columns: two accumulators of 256 columns that share 32 of them, then the scales of
-// one stage (8 for the tokens' 128 rows, 16 for the weight's 256).
-constexpr int kPairAcc1 = 224;
-constexpr int kPairSf = 480;
+constexpr int kPairYBytes = kWide / 2 * kMxRowBytes;
+constexpr int kPairStageBytes = kPairXBytes + kPairYBytes + (1 + kPairSfGroups) * kSfStageBytes;
+// TMEM columns: a wide tile's accumulator, a narrow one's, then the scales of one stage: 8
+// columns for the tokens' 128 rows, 12 and 12 for the weight's three groups.
+constexpr int kPairSf = kBoth;
 
-static size_t pair_smem(int stages) {
+constexpr size_t pair_smem(int stages) {
   return 1024 /* alignment slack */ + static_cast<size_t>(stages) * kPairStageBytes + kPairStaging +
-         2 * kPairN * 4 /* bias, per accumulator */ + static_cast<size_t>(2 * stages + 6) * 8 + 16;
+         static_cast<size_t>(2 * stages + 5) * 8 + 16;
 }
 
-// Tile index -> (token tile, weight tile): `group` token tiles walk over the weight tiles
-// together, so that the pairs running at one time share operands in L2.
-__device__ __forceinline__ void pair_coords(const MxGemmArgs &a, int t, int &tm, int &tn) {
-  const int per_group = a.group * a.tiles_n;
-  const int g = t / per_group, first = g * a.group;
-  const int gsz = min(a.tiles_m - first, a.group);
-  const int r = t - g * per_group;
-  tm = first + r % gsz;
-  tn = r / gsz;
-}
+// The tiles of one pair of CTAs: wide and narrow ones by turns while both last.  Pair p takes
+// every `pairs`-th wide tile from p on and every `pairs`-th narrow one from pairs - 1 - p on,
+// so that a pair with one wide tile more than others has no narrow one more too.
+struct PairWalk {
+  int wide, narrow;  // the next tile of each kind
+  int step, turn;
 
-// One 32-column chunk of this thread's token row: bias, rounding, and the store through the
-// warp's staging buffer (64-byte rows in the 64-byte swizzle, one TMA store) or straight to
-// memory.
-__device__ __forceinline__ void pair_emit(const MxGemmArgs &a, const CUtensorMap *map_out, int m0, int n0, int lane,
-                                          const float *bias, const uint32_t (&r0)[16], const uint32_t (&r1)[16],
-                                          uint8_t *staging, uint32_t &count) {
-  float v[32];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    v[j] = __uint_as_float(r0[j]);
-    v[16 + j] = __uint_as_float(r1[j]);
+  __device__ __forceinline__ PairWalk() {
+    step = static_cast<int>(gridDim.x >> 1);
+    wide = static_cast<int>(blockIdx.x >> 1);
+    narrow = step - 1 - wide;
+    turn = 0;
   }
+
+  // The next tile's kind (0 wide, 1 narrow), token tile and first weight row; false at the end.
+  __device__ __forceinline__ bool next(const MxGemmArgs &a, int &kind, int &tm, int &n0) {
+    const int wide_cols = (a.N + kBoth - 1) / kBoth, narrow_cols = (a.N + kBoth - 1 - kWide) / kBoth;
+    const bool more_wide = wide < a.tiles_m * wide_cols, more_narrow = narrow < a.tiles_m * narrow_cols;
+    if (!more_wide && !more_narrow) return false;
+    kind = (turn && more_narrow) || !more_wide ? 1 : 0;
+    turn = kind ^ 1;
+    const int t = kind ? narrow : wide;
+    if (kind)
+      narrow += step;
+    else
+      wide += step;
+    // All token tiles of one weight tile, then the next: the pairs running at one time share
+    // weight tiles in L2 (walking 4 or 8 token tiles at a time measured the same).
+    const int col = static_cast<int>(a.per_col.div(static_cast<uint32_t>(t)));
+    tm = t - col * a.tiles_m;
+    n0 = col * kBoth + (kind ? kWide : 0);
+    return true;
+  }
+};
+
+// 32 lanes x 32 consecutive columns.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 64 columns from n0 on of a warp's 32 token rows (the first is m0): bias, rounding and the
+// stores, through the warp's staging buffer (rows of 128 bytes in the 128-byte swizzle, then
+// one TMA store; two for float32) or straight to memory.  bias: lane i holds those of columns
+// i and 32 + i.
+template <int DT>
+__device__ __forceinline__ void pair_emit(const MxGemmArgs &a, const CUtensorMap *map_out, int m0, int n0, int lane,
+                                          const float (&bias)[2], const uint32_t (&r)[2][32], uint8_t *staging) {
+  float v[64];
+#pragma unroll
+  for (int j = 0; j < 64; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]);
   if (a.bias) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 b = *reinterpret_cast<const float4 *>(bias + j);
-      v[j] += b.x;
-      v[j + 1] += b.y;
-      v[j + 2] += b.z;
-      v[j + 3] += b.w;
-    }
+    for (int j = 0; j < 64; ++j) v[j] += __shfl_sync(0xffffffffu, bias[j / 32], j % 32);
   }
   if (a.tma_out) {
-    const int halves = a.out_dtype == I8L_F32 ? 2 : 1;  // boxes of 16 float32 or 32 16-bit columns
+    constexpr int kBoxes = DT == I8L_F32 ? 2 : 1, kCols = 64 / kBoxes;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h >= halves) break;
-      if (count >= 2 && lane == 0) bulk_wait_read<1>();
+    for (int h = 0; h < kBoxes; ++h) {
+      if (lane == 0) bulk_wait_read<0>();  // the last store has read the buffer
       __syncwarp();
-      uint8_t *buf = staging + (count & 1u) * kPairBufBytes;
-      ++count;
-      uint32_t w[16];
+      uint8_t *rowp = staging + lane * 128;
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        w[j] = halves == 2 ? __float_as_uint(v[16 * h + j]) : pack16x2(a.out_dtype, v[2 * j], v[2 * j + 1]);
-      uint8_t *rowp = buf + lane * 64;
-      const int sw = (lane >> 1) & 3;
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        *reinterpret_cast<uint4 *>(rowp + ((c ^ sw) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      for (int c = 0; c < 8; ++c) {
+        uint4 w;
+        if constexpr (DT == I8L_F32)
+          w = make_uint4(__float_as_uint(v[32 * h + 4 * c]), __float_as_uint(v[32 * h + 4 * c + 1]),
+                         __float_as_uint(v[32 * h + 4 * c + 2]), __float_as_uint(v[32 * h + 4 * c + 3]));
+        else
+          w = make_uint4(pack16x2(DT, v[8 * c], v[8 * c + 1]), pack16x2(DT, v[8 * c + 2], v[8 * c + 3]),
+                         pack16x2(DT, v[8 * c + 4], v[8 * c + 5]), pack16x2(DT, v[8 * c + 6], v[8 * c + 7]));
+        *reinterpret_cast<uint4 *>(rowp + ((c ^ (lane & 7)) << 4)) = w;
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        const int n = n0 + 16 * h;
-        if (n < a.N && m0 < a.M) tma_store_2d(map_out, buf, n, m0);  // skip boxes wholly outside
+        if (n0 + kCols * h < a.N && m0 < a.M) tma_store_2d(map_out, staging, n0 + kCols * h, m0);
         bulk_commit();
       }
     }
   } else if (m0 + lane < a.M) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
+    for (int j = 0; j < 64; j += 4) {
       const float q[4] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
       if (n0 + j < a.N) store_out4(a, m0 + lane, n0 + j, q);
     }
   }
 }
 
+template <int DT>
 __global__ void __launch_bounds__(kPairThreads, 1)
-    mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
-                   const __grid_constant__ CUtensorMap map_sfx, const __grid_constant__ CUtensorMap map_sfy,
-                   const __grid_constant__ CUtensorMap map_out, const MxGemmArgs a) {
+    mx_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_wide,
+                   const __grid_constant__ CUtensorMap map_narrow, const __grid_constant__ CUtensorMap map_sfx,
+                   const __grid_constant__ CUtensorMap map_sfy, const __grid_constant__ CUtensorMap map_out,
+                   const MxGemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int S = a.stages;
   uint8_t *sx = smem, *sy = sx + S * kPairXBytes, *ssx = sy + S * kPairYBytes, *ssy = ssx + S * kSfStageBytes;
-  uint8_t *staging = ssy + S * 2 * kSfStageBytes;
-  float *bias_cols = reinterpret_cast<float *>(staging + kPairStaging);
-  uint64_t *full = reinterpret_cast<uint64_t *>(bias_cols + 2 * kPairN);
-  uint64_t *empty = full + S, *acc_full = empty + S, *acc_empty = acc_full + 2, *shared_free = acc_empty + 2,
-           *drain = shared_free + 1;
+  uint8_t *staging = ssy + S * kPairSfGroups * kSfStageBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(staging + kPairStaging);
+  uint64_t *empty = full + S, *acc_full = empty + S, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0), lane = threadIdx.x % 32;
   const int rank = static_cast<int>(blockIdx.x & 1u);
   const bool leader = rank == 0;
-  const int first_tile = static_cast<int>(blockIdx.x >> 1), step = static_cast<int>(gridDim.x >> 1);
-  const int total = a.tiles_m * a.tiles_n;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -406,12 +446,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&acc_full[i], 1);
       mbar_init(&acc_empty[i], 2 * kPairEpi);  // both CTAs' epilogue warps
     }
-    mbar_init(shared_free, 2 * kPairEpi);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&map_x);
-    tma_prefetch_desc(&map_y);
+    tma_prefetch_desc(&map_wide);
+    tma_prefetch_desc(&map_narrow);
     tma_prefetch_desc(&map_sfx);
     tma_prefetch_desc(&map_sfy);
     if (a.tma_out) tma_prefetch_desc(&map_out);
@@ -423,50 +463,50 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   cluster_sync();  // both CTAs' barriers and TMEM are set up before either signals the other
   pdl_launch_dependents();
 
+  int kind, tm, n0;
   if (warp == 0) {
     if (lane == 0) {
       const uint64_t pol = policy_evict_last();
-      const uint32_t tx = 2u * kPairStageBytes;  // both CTAs' loads, counted on the even CTA's barrier
-      auto load_w = [&](int st, int kb, int tn) {
+      // Every load of a stage, of both CTAs, is counted on the even CTA's barrier.
+      auto load_w = [&](int st, int kb) {
+        if (leader)
+          mbar_arrive_expect_tx(&full[st], 2u * (kPairStageBytes - (kind ? (kWide - kNarrow) / 2 * kMxRowBytes : 0)));
         const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
-        tma_load_2d_pair(sy + st * kPairYBytes, &map_y, bar, kb * kMxRowBytes, tn * kPairN + rank * (kPairN / 2), pol);
-        tma_load_2d_pair(ssy + st * 2 * kSfStageBytes, &map_sfy, bar, kb * 2 * kSfWords, tn * 2, pol);
+        const int half = (kind ? kNarrow : kWide) / 2;
+        tma_load_2d_pair(sy + st * kPairYBytes, kind ? &map_narrow : &map_wide, bar, kb * kMxRowBytes,
+                         n0 + rank * half, pol);
+        tma_load_2d_pair(ssy + st * kPairSfGroups * kSfStageBytes, &map_sfy, bar, kb * 2 * kSfWords, n0 / 128, pol);
       };
-      auto load_a = [&](int st, int kb, int tm) {
+      auto load_a = [&](int st, int kb) {
         const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
         tma_load_2d_pair(sx + st * kPairXBytes, &map_x, bar, kb * kMxRowBytes, (2 * tm + rank) * kMxRows, pol);
         tma_load_2d_pair(ssx + st * kSfStageBytes, &map_sfx, bar, kb * 2 * kSfWords, 2 * tm + rank, pol);
       };
+      PairWalk walk;
+      bool more = walk.next(a, kind, tm, n0);
       // The first tile's weight stages do not wait for the previous kernel.
-      int tm, tn, pre = 0;
-      if (first_tile < total) {
-        pair_coords(a, first_tile, tm, tn);
-        for (; pre < min(S, a.kblocks); ++pre) {
-          if (leader) mbar_arrive_expect_tx(&full[pre], tx);
-          load_w(pre, pre, tn);
-        }
-      }
+      int pre = 0;
+      if (more)
+        for (; pre < min(S, a.kblocks); ++pre) load_w(pre, pre);
       pdl_wait();
       bool ok = true;
       int st = 0;
       uint32_t phase = 0;
       long long issued = 0;
-      for (int t = first_tile; ok && t < total; t += step) {
-        pair_coords(a, t, tm, tn);
+      for (; ok && more; more = walk.next(a, kind, tm, n0)) {
         for (int kb = 0; kb < a.kblocks; ++kb) {
           if (issued >= pre) {
             if (!mbar_wait_bounded(&empty[st], phase ^ 1u, abort_flag, a.status, kStatusProducerWait)) {
               ok = false;
               break;
             }
-            if (leader) mbar_arrive_expect_tx(&full[st], tx);
-            load_w(st, kb, tn);
+            load_w(st, kb);
           }
-          load_a(st, kb, tm);
+          load_a(st, kb);
           ++issued;
           if (++st == S) {
             st = 0;
@@ -487,109 +527,104 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
+      const uint32_t elected = elect_one();
+      const uint32_t x_lo = desc_lo(smem_u32(sx)), y_lo = desc_lo(smem_u32(sy)), sfx_lo = desc_lo(smem_u32(ssx)),
+                     sfy_lo = desc_lo(smem_u32(ssy)), empty0 = smem_u32(empty);
       bool ok = true, any = false;
-      int st = 0, n = 0;
+      int st = 0;
       uint32_t phase = 0;
-      for (int t = first_tile; ok && t < total; t += step, ++n) {
-        const int acc = n & 1;
-        // This accumulator's last tile has been read, and so have the columns that it
-        // shares with the other accumulator's tile.
-        if (!mbar_wait_bounded(&acc_empty[acc], ((n >> 1) & 1) ^ 1, abort_flag, a.status, kStatusMmaWait) ||
-            (n > 0 && !mbar_wait_bounded(shared_free, (n - 1) & 1, abort_flag, a.status, kStatusMmaWait))) {
-          ok = false;
-          break;
-        }
+      uint32_t phases = 0u;  // bit k: parity of the tiles done in accumulator k
+      PairWalk walk;
+      while (ok && walk.next(a, kind, tm, n0)) {
+        const uint32_t d = tmem + (kind ? kWide : 0), sf = tmem + kPairSf;
+        // The tile starts at a column (one per 32 rows) of its first scale group, and reaches
+        // into a third group only where it has more than 256 - start rows.
+        const int start = n0 % 128;
+        const uint32_t sfy = sf + 8 + static_cast<uint32_t>(start / 32);
+        const uint32_t third = elected && start + (kind ? kNarrow : kWide) > 256 ? 1u : 0u;
+        const uint32_t id0 = kind ? idesc_mxf4(2 * kMxRows, kNarrow, 0) : idesc_mxf4(2 * kMxRows, kWide, 0);
+        const uint32_t id2 = kind ? idesc_mxf4(2 * kMxRows, kNarrow, 2) : idesc_mxf4(2 * kMxRows, kWide, 2);
+        // The last tile in this accumulator has been read.
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&acc_empty[kind], ((phases >> kind) & 1u) ^ 1u, abort_flag,
+                                                       a.status, kStatusMmaWait));
+        if (!ok) break;
+        phases ^= 1u << kind;
         tc_fence_after();
-        const uint32_t d = tmem + (acc ? kPairAcc1 : 0), sf = tmem + kPairSf;
         for (int kb = 0; kb < a.kblocks; ++kb) {
-          if (!mbar_wait_bounded(&full[st], phase, abort_flag, a.status, kStatusMmaWait)) {
-            ok = false;
-            break;
-          }
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[st], phase, abort_flag, a.status, kStatusMmaWait));
+          if (!ok) break;
           tc_fence_after();
-          const int steps = min(4, (a.K - kb * kMxStageK + 63) / 64);
-          const uint64_t ad = sw128_kmajor_desc(smem_u32(sx + st * kPairXBytes));
-          const uint64_t bd = sw128_kmajor_desc(smem_u32(sy + st * kPairYBytes));
-          const uint64_t xd = sf_desc(smem_u32(ssx + st * kSfStageBytes));
-          const uint64_t yd = sf_desc(smem_u32(ssy + st * 2 * kSfStageBytes));
-          constexpr uint64_t kTileStep = kSfTileBytes >> 4;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (2 * h < steps) {
-              sf_to_tmem_pair(sf + 4 * h, xd + h * kTileStep);
-              sf_to_tmem_pair(sf + 8 + 8 * h, yd + h * kTileStep);
-              sf_to_tmem_pair(sf + 12 + 8 * h, yd + (2 + h) * kTileStep);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (k < steps)
-              mma_mxf4_pair(d, ad + 2 * k, bd + 2 * k,
-                            k & 1 ? idesc_mxf4(2 * kMxRows, kPairN, 2) : idesc_mxf4(2 * kMxRows, kPairN, 0),
-                            sf + 4 * (k >> 1), sf + 8 + 8 * (k >> 1), kb == 0 && k == 0 ? 0u : 1u);
-          }
+          const uint32_t al = x_lo + st * (kPairXBytes >> 4), bl = y_lo + st * (kPairYBytes >> 4),
+                         xl = sfx_lo + st * (kSfStageBytes >> 4), yl = sfy_lo + st * (kPairSfGroups * kSfStageBytes >> 4);
+          const int left = a.K - kb * kMxStageK;
           any = true;
-          mma_commit_pair_mc(&empty[st], 0x3);
+          pair_half_stage(elected, third, d, al, bl, xl, yl, sf, sf + 8, sfy, id0, id2, kb != 0, left > 64);
+          if (left > 128)
+            pair_half_stage(elected, third, d, al + 4, bl + 4, xl + (kSfTileBytes >> 4), yl + (kSfTileBytes >> 4),
+                            sf + 4, sf + 20, sfy + 12, id0, id2, 1u, left > 192);
+          mma_commit_elected<true>(elected, empty0 + 8 * st);
           if (++st == S) {
             st = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        mma_commit_pair_mc(&acc_full[acc], 0x3);
+        mma_commit_elected<true>(elected, smem_u32(&acc_full[kind]));
       }
       if (!ok && any) {
-        mma_commit_pair(drain);
+        if (elected) mma_commit_pair(drain);
+        __syncwarp();
         volatile int no_abort = 0;
         mbar_wait_bounded(drain, 0, &no_abort, a.status, kStatusDrainWait);
       }
     }
   } else {
     const int quarter = warp & 3;  // TMEM lanes this warp may access
-    const int tid = threadIdx.x - 64;
-    auto release = [&](uint64_t *bar) {
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (leader)
-          mbar_arrive(bar);
-        else
-          mbar_arrive_remote(map_to_rank(smem_u32(bar), 0));
-      }
-    };
+    const int half = (warp - 2) >> 2;  // takes every other 64-column chunk, from this one on
     pdl_wait();
-    uint8_t *buf = staging + quarter * 2 * kPairBufBytes;
-    uint32_t count = 0;
-    int n = 0;
-    for (int t = first_tile; t < total; t += step, ++n) {
-      int tm, tn;
-      pair_coords(a, t, tm, tn);
-      const int acc = n & 1;
-      const int m0 = (2 * tm + rank) * kMxRows + quarter * 32, n0 = tn * kPairN;
-      const int ncols = min(kPairN, a.N - n0);
-      float *bias = bias_cols + acc * kPairN;
+    uint8_t *buf = staging + (warp - 2) * kPairBufBytes;
+    uint32_t phases = 0u;
+    PairWalk walk;
+    while (walk.next(a, kind, tm, n0)) {
+      const int m0 = (2 * tm + rank) * kMxRows + quarter * 32;
+      const int width = kind ? kNarrow : kWide, ncols = min(width, a.N - n0);
+      float bias[2][2] = {};  // of this warp's chunks, fetched before the accumulator is ready
       if (a.bias)
-        for (int c = tid; c < kPairN; c += kPairEpi * 32)
-          bias[c] = c < ncols ? load_scalar_f(a.bias, a.bias_dtype, n0 + c) : 0.f;
-      const bool ok = mbar_wait_bounded(&acc_full[acc], (n >> 1) & 1, abort_flag, a.status, kStatusEpilogueWait);
-      // All four warps go on or all stop; the barrier also publishes the bias columns.
-      if (!named_bar_and(2, kPairEpi * 32, ok)) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = 64 * half + 128 * (i / 2) + 32 * (i % 2) + lane;
+          if (c < ncols) bias[i / 2][i % 2] = load_scalar_f(a.bias, a.bias_dtype, n0 + c);
+        }
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[kind], (phases >> kind) & 1u, abort_flag, a.status,
+                                                     kStatusEpilogueWait)))
+        break;
+      phases ^= 1u << kind;
       tc_fence_after();
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? kPairAcc1 : 0);
-      // The shared columns first: the last chunk of accumulator 0, the first of 1.
-      for (int i = 0; i < kPairN / 32; ++i) {
-        const int c0 = acc ? 32 * i : (i == 0 ? kPairN - 32 : 32 * (i - 1));
-        uint32_t r0[16], r1[16];
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (kind ? kWide : 0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c0 = 64 * half + 128 * i;
+        const bool last = c0 + 128 >= width;
         const bool live = c0 < ncols;
+        uint32_t r[2][32];
         if (live) {
-          tmem_ld16(taddr + c0, r0);
-          tmem_ld16(taddr + c0 + 16, r1);
+          tmem_ld32(taddr + c0, r[0]);
+          tmem_ld32(taddr + c0 + 32, r[1]);
           tmem_ld_wait();
         }
-        if (i == 0) release(shared_free);
-        if (i == kPairN / 32 - 1) release(&acc_empty[acc]);
-        if (live) pair_emit(a, &map_out, m0, n0 + c0, lane, bias + c0, r0, r1, buf, count);
+        if (last) {  // this warp has read its columns
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (leader)
+              mbar_arrive(&acc_empty[kind]);
+            else
+              mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[kind]), 0));
+          }
+        }
+        if (live) pair_emit<DT>(a, &map_out, m0, n0 + c0, lane, bias[i], r, buf);
+        if (last) break;
       }
     }
     if (lane == 0) bulk_wait<0>();
@@ -608,7 +643,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // ------------------------------------------------------------------ host side
 
 struct MxPlan {
-  int pair;     // CTA pairs on 256 x 256 tiles
+  int pair;     // CTA pairs on 256 tokens x 256 and 192 weight rows
   int tn;       // tokens per tile
   int cluster;  // split tiles: CTAs sharing a tile's K
   int stages;
@@ -640,6 +675,20 @@ static int launch_split(const CUtensorMap &mx, const CUtensorMap &my, const CUte
   return e == cudaSuccess ? I8L_OK : cuda_error(e, "mxfp4 gemm launch");
 }
 
+template <int DT>
+static int launch_pair(const CUtensorMap &mx, const CUtensorMap &my, const CUtensorMap &mn, const CUtensorMap &msx,
+                       const CUtensorMap &msy, const CUtensorMap &mo, const MxGemmArgs &a, int pairs,
+                       cudaStream_t stream) {
+  static size_t configured[64] = {};
+  const size_t smem = pair_smem(a.stages);
+  if (int e = allow_smem(mx_pair_kernel<DT>, smem, configured)) return e;
+  cudaError_t e = launch(mx_pair_kernel<DT>, dim3(2 * pairs), dim3(kPairThreads), smem, stream, 2, mx, my, mn, msx,
+                         msy, mo, a);
+  if (e != cudaSuccess) return cuda_error(e, "mxfp4 gemm launch");
+  e = cudaGetLastError();
+  return e == cudaSuccess ? I8L_OK : cuda_error(e, "mxfp4 gemm launch");
+}
+
 static int split_stage_bytes(int tn) { return kMxRows * kMxRowBytes + tn * kMxRowBytes + 2 * kSfStageBytes; }
 
 static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
@@ -648,12 +697,12 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   const int kblocks = (K + kMxStageK - 1) / kMxStageK;
   *p = MxPlan{};
   if (tile && tile->split == 4 ? true : !(tile && (tile->tok_tile || tile->split)) && M > 256) {
-    if (tile && tile->split == 4 && (tile->swap_ab || tile->tok_tile != 128 || tile->w_tile != 256))
-      return set_error(I8L_ENOTSUP, "CTA pairs (split 4) take tok_tile 128 x w_tile 256 tiles without swap_ab");
+    if (tile && tile->split == 4 && (tile->swap_ab || tile->tok_tile != 128 || tile->w_tile != kWide))
+      return set_error(I8L_ENOTSUP, "CTA pairs (split 4) take tok_tile 128 x w_tile %d tiles without swap_ab", kWide);
     p->pair = 1;
     p->tn = 2 * kMxRows;
     p->cluster = 2;
-    const int most = std::min(16, (di.max_smem_optin - static_cast<int>(pair_smem(0))) / (kPairStageBytes + 16));
+    const int most = (di.max_smem_optin - static_cast<int>(pair_smem(0))) / (kPairStageBytes + 16);
     p->stages = tile && tile->stages ? tile->stages : most;
     if (p->stages < 2 || p->stages > most)
       return set_error(I8L_ENOTSUP, "stages %d outside [2, %d] for this tile", p->stages, most);
@@ -723,7 +772,7 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
   a.N = N;
   a.K = K;
   a.kblocks = (K + kMxStageK - 1) / kMxStageK;
-  const int w_rows = p.pair ? kPairN : kMxRows;
+  const int w_rows = p.pair ? kNarrow : kMxRows;
   a.tiles_n = (N + w_rows - 1) / w_rows;
   a.tiles_m = (M + p.tn - 1) / p.tn;
   a.cluster = p.cluster;
@@ -742,29 +791,29 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
     return set_error(I8L_ENOTSUP, "%d x %d outputs are too many tiles", M, N);
   if (p.pair) {
     if (int e = operand_maps(&mx, &msx, A, lda, sa, M, K, kMxRows, 1)) return e;
-    if (int e = operand_maps(&my, &msy, W, ldw, sw, N, K, kPairN / 2, 2)) return e;
-    CUtensorMap mo{};
+    CUtensorMap mn;
+    if (int e = operand_maps(&my, &msy, W, ldw, sw, N, K, kWide / 2, kPairSfGroups)) return e;
+    if (int e = make_map(&mn, CU_TENSOR_MAP_DATA_TYPE_UINT8, W, N, K / 2, ldw, kMxRowBytes, kNarrow / 2,
+                         CU_TENSOR_MAP_SWIZZLE_128B, "4-bit operand", CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
+      return e;
     // A TMA store ends a row at a 16-byte boundary, with zeros past the last column, so rows
     // that end elsewhere are stored plainly.
+    CUtensorMap mo{};
     if (reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldc * esize) % 16 == 0 &&
         (static_cast<int64_t>(N) * esize) % 16 == 0) {
       static const CUtensorMapDataType kTypes[3] = {CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                                                     CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
-      if (int e = make_map(&mo, kTypes[out_dtype], out, M, N, ldc * esize, 64 / esize, 32, CU_TENSOR_MAP_SWIZZLE_64B,
+      if (int e = make_map(&mo, kTypes[out_dtype], out, M, N, ldc * esize, 128 / esize, 32, CU_TENSOR_MAP_SWIZZLE_128B,
                            "output"))
         return e;
       a.tma_out = 1;
     }
-    a.group = std::min(8, a.tiles_m);
-    static size_t configured[64] = {};
-    const size_t smem = pair_smem(a.stages);
-    if (int e = allow_smem(mx_pair_kernel, smem, configured)) return e;
-    const int pairs = std::min(a.tiles_m * a.tiles_n, (tile && tile->ctas ? tile->ctas : di.sms) / 2);
-    cudaError_t e = launch(mx_pair_kernel, dim3(2 * std::max(1, pairs)), dim3(kPairThreads), smem, s, 2, mx, my, msx,
-                           msy, mo, a);
-    if (e != cudaSuccess) return cuda_error(e, "mxfp4 gemm launch");
-    e = cudaGetLastError();
-    return e == cudaSuccess ? I8L_OK : cuda_error(e, "mxfp4 gemm launch");
+    a.per_col = FastDiv(static_cast<uint32_t>(a.tiles_m));
+    const int64_t tiles = static_cast<int64_t>(a.tiles_m) * ((N + kBoth - 1) / kBoth + (N + kBoth - 1 - kWide) / kBoth);
+    const int pairs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, (tile && tile->ctas ? tile->ctas : di.sms) / 2)));
+    return out_dtype == I8L_BF16  ? launch_pair<I8L_BF16>(mx, my, mn, msx, msy, mo, a, pairs, s)
+           : out_dtype == I8L_F16 ? launch_pair<I8L_F16>(mx, my, mn, msx, msy, mo, a, pairs, s)
+                                  : launch_pair<I8L_F32>(mx, my, mn, msx, msy, mo, a, pairs, s);
   }
   if (int e = operand_maps(&mx, &msx, W, ldw, sw, N, K, kMxRows, 1)) return e;
   if (int e = operand_maps(&my, &msy, A, lda, sa, M, K, p.tn, 1)) return e;

@@ -23,20 +23,6 @@ namespace i8l {
 
 constexpr int kFlatThreads = 256;
 
-// Unsigned division by a constant of the launch: floor(n / d) for n < 2^31 as a multiply
-// and a shift (the round-up method: m = ceil(2^(32+s) / d), s = ceil(log2 d)).
-struct FastDiv {
-  uint32_t d, m, s;
-  explicit FastDiv(uint32_t div = 1) : d(div), m(0), s(0) {
-    while ((1ull << s) < d) ++s;
-    m = static_cast<uint32_t>(((1ull << 32) * ((1ull << s) - d)) / d + 1);
-  }
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
-    const uint32_t t = __umulhi(n, m);
-    return (t + n) >> s;  // t + n < 2^32 for n < 2^31
-  }
-};
-
 struct MxOut {
   uint8_t *q;
   long long ldq;  // bytes

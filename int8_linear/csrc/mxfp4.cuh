@@ -44,20 +44,57 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : (byte == 0u ? 0x00400000u : byte << 23));
 }
 
+// Unsigned division by a constant of the launch: floor(n / d) for n < 2^31 as a multiply
+// and a shift (the round-up method: m = ceil(2^(32+s) / d), s = ceil(log2 d)).
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ explicit FastDiv(uint32_t div = 1) : d(div), m(0), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = static_cast<uint32_t>(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+    const uint32_t t = __umulhi(n, m);
+    return (t + n) >> s;  // t + n < 2^32 for n < 2^31
+  }
+};
+
 // ---------------------------------------------------------------- tensor cores
 // tcgen05.mma.kind::mxf4 multiplies packed e2m1 tiles, 64 values (32 bytes) of K per
 // instruction, with the scales of both operands in TMEM: a scale tile (128 rows x 4 blocks)
 // is four columns there, row r in lane r % 32 of column r / 32, its four blocks in the four
 // bytes; an instruction takes two of the bytes, chosen by the scale ids of its descriptor.
 
-// One 512-byte scale tile from shared memory into four TMEM columns, replicated to the
-// lanes of all four warps; in order with this thread's later tcgen05.mma.
-__device__ __forceinline__ void sf_to_tmem(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// The issuing warp runs these converged, all lanes with the same operands, and `elected` set
+// in one lane: the operands then stay in uniform registers, where one lane in a branch of
+// its own would move each of them there before every instruction (measured on the pair
+// tiles at 4096 x 12288 x 2048: XXX us so, XXX us that way).
+
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
 }
-// The same in both CTAs of a pair, each from its own shared memory.
-__device__ __forceinline__ void sf_to_tmem_pair(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+
+// One 512-byte scale tile from shared memory into four TMEM columns, replicated to the
+// lanes of all four warps; in order with this thread's later tcgen05.mma.  kPair: in both
+// CTAs of a pair, each from its own shared memory.
+template <bool kPair>
+__device__ __forceinline__ void sf_to_tmem(uint32_t elected, uint32_t taddr, uint64_t desc) {
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected)
+        : "memory");
 }
 
 // Shared-memory descriptor of a scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups
@@ -75,23 +112,85 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int sf_id) {
 }
 
 // D[tmem] (+)= A * B, 64 values of K.
-__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
-                                         uint32_t sfb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
-      : "memory");
+template <bool kPair>
+__device__ __forceinline__ void mma_mxf4(uint32_t elected, uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+            d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb), "r"(elected)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+            d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb), "r"(elected)
+        : "memory");
 }
-__device__ __forceinline__ void mma_mxf4_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                              uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+
+// High words of the descriptors: those of sw128_kmajor_desc and sf_desc do not depend on the
+// address.
+constexpr uint32_t kSw128DescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t kSfDescHi = (128u >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
+
+// Half a stage (128 values of K) of a CTA pair in one piece, so that nothing but the tensor
+// instructions and a few additions stands between them: the scale tiles of the first operand
+// (one) and the second (two, and a third where `third` is set in the elected lane), then two
+// MMAs, or one without `second`.  alo .. ylo: low descriptor words; sfx, sfy: TMEM columns
+// that the scales go to; sfy_at: that of the tile's first row.
+__device__ __forceinline__ void pair_half_stage(uint32_t elected, uint32_t third, uint32_t d, uint32_t alo,
+                                                uint32_t blo, uint32_t xlo, uint32_t ylo, uint32_t sfx, uint32_t sfy,
+                                                uint32_t sfy_at, uint32_t idesc0, uint32_t idesc2, uint32_t accumulate,
+                                                bool second) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+      "{\n\t.reg .pred p, q, r;\n\t"
+      ".reg .b64 u, v;\n\t.reg .b32 t, w;\n\t"
+      "setp.ne.b32 p, %9, 0;\n\tsetp.ne.b32 q, %10, 0;\n\tsetp.ne.b32 r, %11, 0;\n\t"
+      "mov.b64 u, {%3, %13};\n\t"
+      "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%5], u;\n\t"
+      "mov.b64 u, {%4, %13};\n\t"
+      "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%6], u;\n\t"
+      "add.u32 t, %6, 4;\n\tadd.u32 w, %4, 64;\n\tmov.b64 u, {w, %13};\n\t"
+      "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [t], u;\n\t"
+      "add.u32 t, %6, 8;\n\tadd.u32 w, %4, 128;\n\tmov.b64 u, {w, %13};\n\t"
+      "@r tcgen05.cp.cta_group::2.32x128b.warpx4 [t], u;\n\t"
+      "mov.b64 u, {%1, %12};\n\tmov.b64 v, {%2, %12};\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], u, v, %8, [%5], [%7], p;\n\t}" ::"r"(d),
+      "r"(alo), "r"(blo), "r"(xlo), "r"(ylo), "r"(sfx), "r"(sfy), "r"(sfy_at), "r"(idesc0), "r"(accumulate),
+      "r"(elected), "r"(third), "r"(kSw128DescHi), "r"(kSfDescHi)
       : "memory");
+  if (second)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        ".reg .b64 u, v;\n\t.reg .b32 t, w;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\tsetp.eq.u32 p, 0, 0;\n\t"
+        "add.u32 t, %1, 2;\n\tadd.u32 w, %2, 2;\n\tmov.b64 u, {t, %7};\n\tmov.b64 v, {w, %7};\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], u, v, %5, [%3], [%4], p;\n\t}" ::"r"(d),
+        "r"(alo), "r"(blo), "r"(sfx), "r"(sfy_at), "r"(idesc2), "r"(elected), "r"(kSw128DescHi)
+        : "memory");
+}
+
+// Arrive once when every tcgen05 operation this thread issued so far has completed: on this
+// CTA's mbarrier (its shared-memory address), or with kPair on those at the same offset in both CTAs of the pair.
+template <bool kPair>
+__device__ __forceinline__ void mma_commit_elected(uint32_t elected, uint32_t bar) {
+  if constexpr (kPair)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::
+            "r"(bar),
+        "h"(static_cast<uint16_t>(0x3)), "r"(elected)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(elected)
+        : "memory");
 }
 
 // Eight values times `inv`, rounded to e2m1 (nearest, ties to even, saturating), packed
