@@ -12,6 +12,8 @@ import os
 import threading
 from pathlib import Path
 
+import torch
+
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libint8linear_b200.so"
 
 OK, ENOTSUP, EINVAL, ECUDA, EWORKSPACE = 0, 1, 2, 3, 4
@@ -145,16 +147,21 @@ def check(code: int) -> None:
     raise RuntimeError(f"int8_linear native call failed ({code}): {msg}")
 
 
-def on_device(index: int, fn, args: tuple) -> None:
+# The current device's index without torch.cuda's lazy-initialisation check (a tensor on the
+# device exists by then).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def on_device(index: int, fn, *args) -> None:
     """check(fn(*args)) with CUDA device `index` current: launches go to the current device,
     which need not be the one the tensors are on."""
-    import torch
-
-    if index == torch.cuda.current_device():
-        check(fn(*args))
+    if index == _current_device():
+        code = fn(*args)
     else:
         with torch.cuda.device(index):
-            check(fn(*args))
+            code = fn(*args)
+    if code:
+        check(code)
 
 
 # Called when the status word shows a kernel gave up a wait, and by clear_status():

@@ -72,28 +72,64 @@ __device__ __noinline__ float silu_mul_exact(float g, float u) {
   return static_cast<float>(gd / (1.0 + exp(-gd)) * static_cast<double>(u));
 }
 
-// Two values of y = round_DT(float32(silu(g) * u)), the float32 rounding being that of the
-// exact product.  In float32, expf and the full-range division are within 2 ulp each (their
-// documented bounds), the sum and the product within 0.5: 5 ulp of at most 2^-23 relative
-// each.  With a margin of one more, y is right wherever both ends of
-// [v (1 - 6*2^-23), v (1 + 6*2^-23)] round alike; elsewhere (about one value in 2000 for
-// bf16) the value is computed again in float64.  Results near or below the smallest normal
-// float32 have no such relative bound and take that way too, but for products with zero.
+// Rounds two floats to the 16-bit type and packs them, v0 low.
 template <int DT>
-__device__ __forceinline__ void silu_mul2(float g0, float g1, float u0, float u1, float &y0, float &y1) {
-  float d0, d1, v0, v1, l0, l1, h0, h1;
-  add2_rn(d0, d1, 1.0f, 1.0f, expf(-g0), expf(-g1));
-  mul2_rn(v0, v1, div_full(g0, d0), div_full(g1, d1), u0, u1);
-  constexpr float kLow = 1.0f - 6.0f / 8388608.0f, kHigh = 1.0f + 6.0f / 8388608.0f;
-  mul2_rn(l0, l1, v0, v1, kLow, kLow);
-  mul2_rn(h0, h1, v0, v1, kHigh, kHigh);
-  round2_through<DT>(l0, l1);
-  round2_through<DT>(h0, h1);
-  y0 = l0;
-  y1 = l1;
-  constexpr float kTiny = 1e-36f;
-  if (l0 != h0 || (fabsf(v0) < kTiny && g0 != 0.f && u0 != 0.f)) y0 = round_through<DT>(silu_mul_exact(g0, u0));
-  if (l1 != h1 || (fabsf(v1) < kTiny && g1 != 0.f && u1 != 0.f)) y1 = round_through<DT>(silu_mul_exact(g1, u1));
+__device__ __forceinline__ uint32_t pack2(float v0, float v1) {
+  uint32_t p;
+  if constexpr (DT == I8L_BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(v1), "f"(v0));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(v1), "f"(v0));
+  return p;
+}
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// One value for which the float32 arithmetic of silu_mul2 does not settle the rounding.
+template <int DT>
+__device__ __noinline__ uint32_t silu_mul_settle(float g, float u) {
+  const float y = g == 0.f || u == 0.f ? g * u : silu_mul_exact(g, u);
+  return pack2<DT>(y, 0.f) & 0xffffu;
+}
+
+// Two values of y = round_DT(float32(silu(g) * u)), packed, the float32 rounding being that
+// of the exact product.
+//
+// v = g * rcp(1 + 2^(-g log2 e)) * u in float32.  In units of 2^-23 relative: the exponent's
+// product and its constant are off by 0.63 |g| at most, ex2.approx by 2, both damped by
+// e/(1 + e) with e = exp(-g), which is below 1 for g < 0 and below 1/2 (times |g|: below 0.3)
+// for g > 0; the sum and the two products add 1/2 each and rcp.approx 1.  So v is within
+// 5 + 0.7 max(-g, 0) of those units, with some margin, and y is right wherever both ends of
+// that interval round alike.  Elsewhere (about one value in 2000 for bf16) it is computed
+// again in float64, and so are values near the end of float32's normal range, which has no
+// such relative bound.
+template <int DT>
+__device__ __forceinline__ uint32_t silu_mul2(uint32_t gw, uint32_t uw) {
+  constexpr float kUnit = 1.0f / 8388608.0f, kTiny = 1e-36f;
+  float g0, g1, u0, u1, p0, p1, d0, d1, v0, v1;
+  unpack2<DT>(gw, g0, g1);
+  unpack2<DT>(uw, u0, u1);
+  mul2_rn(p0, p1, g0, g1, -1.4426950408889634f, -1.4426950408889634f);
+  add2_rn(d0, d1, 1.0f, 1.0f, ex2_approx(p0), ex2_approx(p1));
+  mul2_rn(v0, v1, g0, g1, rcp_approx(d0), rcp_approx(d1));
+  mul2_rn(v0, v1, v0, v1, u0, u1);
+  const float e0 = fmaf(fmaxf(-g0, 0.f), 0.7f * kUnit, 5.0f * kUnit), e1 = fmaf(fmaxf(-g1, 0.f), 0.7f * kUnit, 5.0f * kUnit);
+  uint32_t low = pack2<DT>(fmaf(v0, -e0, v0), fmaf(v1, -e1, v1));
+  const uint32_t high = pack2<DT>(fmaf(v0, e0, v0), fmaf(v1, e1, v1));
+  if (low != high || fminf(fabsf(v0), fabsf(v1)) < kTiny) {
+    if (((low ^ high) & 0xffffu) || fabsf(v0) < kTiny) low = (low & 0xffff0000u) | silu_mul_settle<DT>(g0, u0);
+    if (((low ^ high) >> 16) || fabsf(v1) < kTiny) low = (low & 0xffffu) | (silu_mul_settle<DT>(g1, u1) << 16);
+  }
+  return low;
 }
 
 // ------------------------------------------------------------------ flat quantisers
@@ -109,39 +145,58 @@ struct FlatArgs {
   int vec;                 // 16-byte loads allowed
 };
 
-// kSilu: x holds [gate | up] rows of 2K values.
+// Eight 16-bit values from any alignment, as they lie in memory.
+__device__ __forceinline__ uint4 load8_raw(const void *base, long long idx, bool vec) {
+  const uint16_t *p = static_cast<const uint16_t *>(base) + idx;
+  if (vec) return *reinterpret_cast<const uint4 *>(p);
+  return make_uint4(p[0] | (static_cast<uint32_t>(p[1]) << 16), p[2] | (static_cast<uint32_t>(p[3]) << 16),
+                    p[4] | (static_cast<uint32_t>(p[5]) << 16), p[6] | (static_cast<uint32_t>(p[7]) << 16));
+}
+
+// kSilu: x holds [gate | up] rows of 2K values.  Each thread takes U vectors, a block's
+// width of threads apart, and loads them all before it works on the first.
 template <int DT, bool kSilu, int U>
 __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a) {
+  static_assert(!kSilu || DT != I8L_F32, "SiLU takes 16-bit activations");
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t base = blockIdx.x * (kFlatThreads * U) + threadIdx.x;
   const long long K = static_cast<long long>(a.blocks) * kMxBlock;
-  float y[U][8];
+  constexpr bool kWide = DT == I8L_F32;
+  uint4 x[kWide ? 1 : U], up[kSilu ? U : 1];
+  float y[kWide ? U : 1][8];
   uint32_t row[U], vec[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t id = base + u * kFlatThreads;
     row[u] = a.per_row.div(id);
     vec[u] = id - row[u] * a.per_row.d;
-    if (id < a.vectors) {
-      const long long at = row[u] * a.ldx + vec[u] * 8u;
-      load8<DT>(a.x, at, a.vec, y[u]);
-      if constexpr (kSilu) {
-        float up[8];
-        load8<DT>(a.x, at + K, a.vec, up);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) silu_mul2<DT>(y[u][i], y[u][i + 1], up[i], up[i + 1], y[u][i], y[u][i + 1]);
-      }
-    } else {
+    const bool in = id < a.vectors;
+    const long long at = row[u] * a.ldx + vec[u] * 8u;
+    if constexpr (kWide) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[u][i] = 0.f;
+      if (in) load8<DT>(a.x, at, a.vec, y[u]);
+    } else {
+      x[u] = in ? load8_raw(a.x, at, a.vec) : make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (kSilu) up[u] = in ? load8_raw(a.x, at + K, a.vec) : make_uint4(0u, 0u, 0u, 0u);
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t id = base + u * kFlatThreads;
-    uint32_t byte;
-    const uint32_t w = mx_quantise8(y[u], byte);
+    uint32_t byte, w;
+    if constexpr (kWide) {
+      w = mx_quantise8(y[u], byte);
+    } else {
+      if constexpr (kSilu) {
+        x[u].x = silu_mul2<DT>(x[u].x, up[u].x);
+        x[u].y = silu_mul2<DT>(x[u].y, up[u].y);
+        x[u].z = silu_mul2<DT>(x[u].z, up[u].z);
+        x[u].w = silu_mul2<DT>(x[u].w, up[u].w);
+      }
+      w = mx_quantise8<DT>(x[u], byte);
+    }
     if (id < a.vectors) {
       *reinterpret_cast<uint32_t *>(a.o.q + row[u] * a.o.ldq + vec[u] * 4u) = w;
       if ((threadIdx.x & 3) == 0) store_sf(a.o, row[u], static_cast<int>(vec[u] >> 2), a.blocks, byte);
@@ -238,11 +293,12 @@ __global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) 
         n0 = round_to_weight(n0, a.w_dtype);
         n1 = round_to_weight(n1, a.w_dtype);
         mul2_rn(h[v][i], h[v][i + 1], n0, n1, w[i], w[i + 1]);
-        round2_through<DT>(h[v][i], h[v][i + 1]);
       }
     }
+    const uint4 y = make_uint4(pack2<DT>(h[v][0], h[v][1]), pack2<DT>(h[v][2], h[v][3]), pack2<DT>(h[v][4], h[v][5]),
+                               pack2<DT>(h[v][6], h[v][7]));
     uint32_t byte;
-    const uint32_t packed = mx_quantise8(h[v], byte);
+    const uint32_t packed = mx_quantise8<DT>(y, byte);
     if (col < a.K) {
       *reinterpret_cast<uint32_t *>(a.o.q + row * a.o.ldq + col / 2) = packed;
       if ((threadIdx.x & 3) == 0) store_sf(a.o, row, col / kMxBlock, a.K / kMxBlock, byte);

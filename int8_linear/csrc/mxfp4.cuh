@@ -250,4 +250,40 @@ __device__ __forceinline__ uint32_t mx_quantise8(const float (&y)[8], uint32_t &
   return byte == 255u ? 0u : mx_pack8(y, mx_inv_scale(byte));
 }
 
+// Two 16-bit values as floats.
+template <int DT>
+__device__ __forceinline__ void unpack2(uint32_t w, float &v0, float &v1) {
+  if constexpr (DT == I8L_BF16) {
+    v0 = __uint_as_float(w << 16);
+    v1 = __uint_as_float(w & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    v0 = f.x;
+    v1 = f.y;
+  }
+}
+
+// The same for eight bf16 or fp16 values as they lie in memory.  16-bit floats of one sign
+// are ordered as their bits are, NaN and infinity last, so the maximum is taken two at a
+// time on the bits.
+template <int DT>
+__device__ __forceinline__ uint32_t mx_quantise8(const uint4 &w, uint32_t &byte) {
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+  uint32_t m = __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs), __vmaxu2(w.z & kAbs, w.w & kAbs));
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  m = max(m & 0xffffu, m >> 16);
+  if constexpr (DT == I8L_BF16)
+    m <<= 16;
+  else
+    m = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+  byte = mx_scale_byte(m);
+  float y[8];
+  unpack2<DT>(w.x, y[0], y[1]);
+  unpack2<DT>(w.y, y[2], y[3]);
+  unpack2<DT>(w.z, y[4], y[5]);
+  unpack2<DT>(w.w, y[6], y[7]);
+  return byte == 255u ? 0u : mx_pack8(y, mx_inv_scale(byte));
+}
+
 }  // namespace i8l

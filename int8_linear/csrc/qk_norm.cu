@@ -9,13 +9,14 @@
 //
 // A group of lanes, eight values each, holds one head in registers: the sum of squares is
 // a butterfly over the group, and the other half of a pair comes from another lane of the
-// group by a shuffle.  A group keeps its token's cosines and sines in registers and walks
-// over the heads of that token, so the angles are read once per group and not per head.
-// The kernel reads and writes each value once and is bound by HBM.
+// group by a shuffle.  A group takes up to P neighbouring heads of one token: their loads are
+// all in flight together, and the token's angles are read once for them.  The kernel reads
+// and writes each value once and is bound by HBM.
 #include <algorithm>
 
 #include "common.cuh"
 #include "internal.h"
+#include "mxfp4.cuh"
 #include "rows.cuh"
 
 namespace i8l {
@@ -37,27 +38,34 @@ struct QkArgs {
   void *k;
   long long ldk;
   int tokens, heads, kv_heads, dim, rot;
-  int parts;       // groups per token
-  long long groups;  // tokens * parts
+  int parts;       // groups per token, each with up to P heads
+  uint32_t groups;  // tokens * parts, below 2^31
+  FastDiv per_token;  // parts
   float eps;
   int interleaved;
   int w_vec, cs_vec;
 };
 
-// G lanes per head (a power of two, G * 8 >= dim).  In place is fine: a lane stores the
+// G lanes per head (a power of two, G * 8 >= dim), P heads per group.  In place is fine: a lane stores the
 // elements that it alone loaded, after every exchange within its head.
-template <int DT, int G>
+template <int DT, int G, int P>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   using T = typename ActType<DT>::T;
-  const long long group = (static_cast<long long>(blockIdx.x) * kQkThreads + threadIdx.x) / G;
+  const uint32_t group = blockIdx.x * (kQkThreads / G) + threadIdx.x / G;
   const int lane = threadIdx.x % G;
   const bool live = group < a.groups;
-  const long long token = live ? group / a.parts : 0;
-  const int part = live ? static_cast<int>(group - token * a.parts) : 0;
+  const long long token = live ? a.per_token.div(group) : 0;
+  const int part = live ? static_cast<int>(group - static_cast<uint32_t>(token) * a.parts) : 0;
   const int c0 = lane * 8;
   const bool mine = live && c0 < a.dim;
+  const int all = a.heads + a.kv_heads, head0 = part * P;
+  const T *src = static_cast<const T *>(a.qkv) + token * a.ld + static_cast<long long>(head0) * a.dim + c0;
+  uint4 raw[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    raw[i] = mine && head0 + i < all ? *reinterpret_cast<const uint4 *>(src + i * a.dim) : make_uint4(0u, 0u, 0u, 0u);
   const int half = a.rot / 2;
 
   long long pos = 0;
@@ -97,18 +105,17 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a
 
   float w[8];
   int loaded = -1;  // which weight `w` holds: 0 queries, 1 keys
-  const int all = a.heads + a.kv_heads;
-  // Every group of a warp takes the same number of turns: the shuffles are warp-wide.
-  for (int turn = 0; turn * a.parts < all; ++turn) {
-    const int head = part + turn * a.parts;
+#pragma unroll
+  for (int turn = 0; turn < P; ++turn) {
+    const int head = head0 + turn;
     const bool here = mine && head < all;
     const int key = head >= a.heads ? 1 : 0;
     if (here && key != loaded) load_weight_vec<8>(key ? a.wk : a.wq, a.w_dtype, c0, a.w_vec != 0, w);
     loaded = key;
     float x[8];
+    const T *h = reinterpret_cast<const T *>(&raw[turn]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (here) load_vec<DT, 8>(static_cast<const T *>(a.qkv) + token * a.ld + static_cast<long long>(head) * a.dim, c0, x);
+    for (int i = 0; i < 8; ++i) x[i] = ActType<DT>::to_f32(h[i]);
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
@@ -143,17 +150,17 @@ using namespace i8l;
 
 namespace {
 
-template <int DT>
+template <int DT, int P>
 cudaError_t launch_qk(const QkArgs &a, int lanes, cudaStream_t s) {
-  const long long per_block = kQkThreads / lanes;
-  const dim3 grid(static_cast<unsigned>((a.groups + per_block - 1) / per_block));
+  const unsigned per_block = kQkThreads / lanes;
+  const dim3 grid((a.groups + per_block - 1) / per_block);
   switch (lanes) {
-    case 1: return launch(qk_norm_rope_kernel<DT, 1>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 2: return launch(qk_norm_rope_kernel<DT, 2>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 4: return launch(qk_norm_rope_kernel<DT, 4>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 8: return launch(qk_norm_rope_kernel<DT, 8>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 16: return launch(qk_norm_rope_kernel<DT, 16>, grid, dim3(kQkThreads), 0, s, 1, a);
-    default: return launch(qk_norm_rope_kernel<DT, 32>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 1: return launch(qk_norm_rope_kernel<DT, 1, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 2: return launch(qk_norm_rope_kernel<DT, 2, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 4: return launch(qk_norm_rope_kernel<DT, 4, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 8: return launch(qk_norm_rope_kernel<DT, 8, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 16: return launch(qk_norm_rope_kernel<DT, 16, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    default: return launch(qk_norm_rope_kernel<DT, 32, P>, grid, dim3(kQkThreads), 0, s, 1, a);
   }
 }
 
@@ -215,18 +222,22 @@ extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, 
   a.cs_vec = aligned16(cos_sin) && (rot_dim / 2 * (cs_dtype == I8L_F32 ? 4 : 2)) % 16 == 0 ? 1 : 0;
   int lanes = 1;
   while (lanes * 8 < head_dim) lanes *= 2;
-  // One head per group until the groups fill the SMs twice over, then up to four heads per
-  // group, which share one read of the angles.
+  // One head per group until the groups fill the SMs twice over, then four.
   DeviceInfo di;
   if (int e = device_info(&di)) return e;
-  const int64_t fill = 2LL * di.sms * (2048 / lanes);
-  int64_t per = std::min<int64_t>(4, std::max<int64_t>(1, static_cast<int64_t>(tokens) * all / fill));
-  a.parts = static_cast<int>((all + per - 1) / per);
-  a.groups = static_cast<long long>(tokens) * a.parts;
-  if (a.groups / (kQkThreads / lanes) >= INT32_MAX)
+  const bool four = static_cast<int64_t>(tokens) * all > 2LL * di.sms * (2048 / lanes);
+  a.parts = static_cast<int>(four ? (all + 3) / 4 : all);
+  const int64_t groups = static_cast<int64_t>(tokens) * a.parts;
+  if (groups > INT32_MAX - kQkThreads)
     return set_error(I8L_ENOTSUP, "%d tokens x %lld heads is too large", tokens, static_cast<long long>(all));
+  a.groups = static_cast<uint32_t>(groups);
+  a.per_token = FastDiv(static_cast<uint32_t>(a.parts));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t err = act_dtype == I8L_BF16 ? launch_qk<I8L_BF16>(a, lanes, s) : launch_qk<I8L_F16>(a, lanes, s);
+  cudaError_t err;
+  if (act_dtype == I8L_BF16)
+    err = four ? launch_qk<I8L_BF16, 4>(a, lanes, s) : launch_qk<I8L_BF16, 1>(a, lanes, s);
+  else
+    err = four ? launch_qk<I8L_F16, 4>(a, lanes, s) : launch_qk<I8L_F16, 1>(a, lanes, s);
   if (err != cudaSuccess) return cuda_error(err, "qk_norm_rope launch");
   err = cudaGetLastError();
   return err == cudaSuccess ? I8L_OK : cuda_error(err, "qk_norm_rope launch");

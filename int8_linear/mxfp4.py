@@ -43,34 +43,35 @@ _FLOAT = _WEIGHT  # bf16, fp16 and fp32
 __all__ = ["w4a4_mm", "quant_mxfp4", "add_rmsnorm_quant_mxfp4", "silu_mul_quant_mxfp4", "dequant_mxfp4"]
 
 
-def _rows(x: torch.Tensor, name: str, kinds: dict) -> tuple[int, int]:
+def _rows(x: torch.Tensor, name: str, kinds: dict) -> tuple[int, int, int]:
+    """(rows, columns, device index) of a quantiser's input, or the refusal of it."""
     if x.dtype not in kinds:
         raise NotSupported(f"{name} must be one of {[str(k) for k in kinds]}, got {x.dtype}")
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
         raise NotSupported(f"{name} must be a 2-D tensor with contiguous rows")
-    if not x.is_cuda:
+    dev = x.get_device()
+    if dev < 0:
         raise ValueError(f"the 4-bit quantisers run on a CUDA device, got {x.device}")
-    return x.shape
+    m, k = x.shape
+    return m, k, dev
 
 
-def _empty(m: int, k: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+def _empty(x: torch.Tensor, m: int, k: int) -> tuple[torch.Tensor, torch.Tensor]:
     if k % BLOCK:
         raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks)")
-    return (torch.empty((m, k // 2), dtype=torch.uint8, device=device),
-            torch.empty((-(-m // 128), -(-k // 128), 512), dtype=torch.uint8, device=device))
+    q = x.new_empty((m, k >> 1), dtype=torch.uint8)
+    return q, q.new_empty(((m + 127) >> 7, (k + 127) >> 7, 512))
 
 
 def quant_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q uint8 [M, K/2], s uint8 [ceil(M/128), ceil(K/128), 512]) of a bf16, fp16 or fp32
     matrix with contiguous rows: an activation (a column slice of a wider matrix is fine,
     no copy is made) or a weight [N, K].  K must be a multiple of 32."""
-    m, k = _rows(x, "x", _FLOAT)
-    q, s = _empty(m, k, x.device)
+    m, k, dev = _rows(x, "x", _FLOAT)
+    q, s = _empty(x, m, k)
     if m and k:
-        dev = x.get_device()
-        _native.on_device(dev, _native.load().i8l_quant_mxfp4, (
-            x.data_ptr(), x.stride(0), _FLOAT[x.dtype], q.data_ptr(), k // 2, s.data_ptr(), m, k,
-            current_stream(dev)))
+        _native.on_device(dev, _native.load().i8l_quant_mxfp4, x.data_ptr(), x.stride(0), _FLOAT[x.dtype],
+                          q.data_ptr(), k >> 1, s.data_ptr(), m, k, current_stream(dev))
     return q, s
 
 
@@ -80,23 +81,22 @@ def add_rmsnorm_quant_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weig
     r = 1 / sqrt(mean(h^2) + eps), computed in float64 and rounded once to float32;
     y = round(round(h * r) * weight), first to the weight's type, then to x's; y is
     block-quantised.  x and residual bf16/fp16 with contiguous rows."""
-    m, k = _rows(x, "x", _ACT)
-    if weight.dtype not in _WEIGHT or weight.numel() != k or weight.device != x.device:
+    m, k, dev = _rows(x, "x", _ACT)
+    if weight.dtype not in _WEIGHT or weight.numel() != k or weight.get_device() != dev:
         raise ValueError(f"weight must hold {k} bf16/fp16/fp32 values on {x.device}, got {weight.dtype} "
                          f"{tuple(weight.shape)} on {weight.device}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
-                                 or residual.device != x.device or (k > 1 and residual.stride(1) != 1)):
+                                 or residual.get_device() != dev or (residual.stride(1) != 1 and k > 1)):
         raise ValueError("residual must match x in shape, dtype and device and have contiguous rows")
-    q, s = _empty(m, k, x.device)
-    rout = torch.empty((m, k), dtype=x.dtype, device=x.device) if residual is not None else None
+    q, s = _empty(x, m, k)
+    rout = x.new_empty((m, k)) if residual is not None else None
     if m and k:
         w = weight if weight.is_contiguous() else weight.contiguous()
-        dev = x.get_device()
-        _native.on_device(dev, _native.load().i8l_add_rmsnorm_quant_mxfp4, (
-            x.data_ptr(), x.stride(0), residual.data_ptr() if residual is not None else None,
-            residual.stride(0) if residual is not None else 0, w.data_ptr(), _ACT[x.dtype], _WEIGHT[w.dtype],
-            q.data_ptr(), k // 2, s.data_ptr(), rout.data_ptr() if rout is not None else None, k, m, k, eps,
-            current_stream(dev)))
+        has = residual is not None
+        _native.on_device(dev, _native.load().i8l_add_rmsnorm_quant_mxfp4, x.data_ptr(), x.stride(0),
+                          residual.data_ptr() if has else None, residual.stride(0) if has else 0, w.data_ptr(),
+                          _ACT[x.dtype], _WEIGHT[w.dtype], q.data_ptr(), k >> 1, s.data_ptr(),
+                          rout.data_ptr() if has else None, k, m, k, eps, current_stream(dev))
     return q, s, rout
 
 
@@ -104,50 +104,49 @@ def silu_mul_quant_mxfp4(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.Ten
     """(q, s) of silu(gate) * up for bf16/fp16 rows [gate | up] of 2K values:
     fused_quant.silu_mul_quant with its result in 4 bits.  The product is rounded to
     float32 and then to gate_up's type, as if computed exactly, before the blocks."""
-    m, k2 = _rows(gate_up, "gate_up", _ACT)
+    m, k2, dev = _rows(gate_up, "gate_up", _ACT)
     if k2 % 2:
         raise ValueError(f"gate_up rows of {k2} values are not [gate | up]")
-    k = k2 // 2
-    q, s = _empty(m, k, gate_up.device)
+    k = k2 >> 1
+    q, s = _empty(gate_up, m, k)
     if m and k:
-        dev = gate_up.get_device()
-        _native.on_device(dev, _native.load().i8l_silu_mul_quant_mxfp4, (
-            gate_up.data_ptr(), gate_up.stride(0), _ACT[gate_up.dtype], q.data_ptr(), k // 2, s.data_ptr(), m, k,
-            current_stream(dev)))
+        _native.on_device(dev, _native.load().i8l_silu_mul_quant_mxfp4, gate_up.data_ptr(), gate_up.stride(0),
+                          _ACT[gate_up.dtype], q.data_ptr(), k >> 1, s.data_ptr(), m, k, current_stream(dev))
     return q, s
 
 
-def _operand(q: torch.Tensor, s: torch.Tensor, rows: int, k: int, name: str) -> None:
-    """Checks that s holds the scales of a [rows, k] operand on q's device."""
-    want = (-(-rows // 128), -(-k // 128), 512)
+def _scales(s: torch.Tensor, rows: int, k: int, dev: int, name: str) -> torch.Tensor:
+    """The scale tiles s of a [rows, k] operand on device `dev`, copied if the kernels cannot
+    read them where they lie; raises if they are not that."""
     if s.dtype != torch.uint8:
         raise NotSupported(f"{name} must be uint8 scale bytes, got {s.dtype}")
-    if tuple(s.shape) != want or s.device != q.device:
-        raise ValueError(f"{name} must be the {list(want)} scale tiles of [{rows}, {k}] on {q.device}, got "
-                         f"{tuple(s.shape)} on {s.device}")
+    if s.shape != ((rows + 127) >> 7, (k + 127) >> 7, 512) or s.get_device() != dev:
+        raise ValueError(f"{name} must be the {[-(-rows // 128), -(-k // 128), 512]} scale tiles of [{rows}, {k}] on "
+                         f"device {dev}, got {tuple(s.shape)} on {s.device}")
+    if s.is_contiguous() and s.data_ptr() % 16 == 0:
+        return s
+    return s.clone(memory_format=torch.contiguous_format)
 
 
 def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """[M, K] values that codes q [M, K/2] and scales s stand for, in bf16, fp16 or fp32."""
     if q.dtype != torch.uint8 or out_dtype not in _FLOAT:
         raise NotSupported(f"uint8 codes to bf16, fp16 or fp32 only, got {q.dtype} to {out_dtype}")
-    if q.dim() != 2 or (q.shape[1] > 1 and q.stride(1) != 1):
+    if q.dim() != 2 or (q.stride(1) != 1 and q.shape[1] > 1):
         raise NotSupported("q must be a 2-D tensor with contiguous rows")
-    m, k = q.shape[0], 2 * q.shape[1]
+    m, half = q.shape
+    k, dev = 2 * half, q.get_device()
     if k % BLOCK:
         raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks)")
-    _operand(q, s, m, k, "s")
-    if not q.is_cuda:
+    if dev < 0:
         raise ValueError(f"dequant_mxfp4 runs on a CUDA device, got {q.device}")
-    out = torch.empty((m, k), dtype=out_dtype, device=q.device)
+    s = _scales(s, m, k, dev, "s")
+    out = q.new_empty((m, k), dtype=out_dtype)
     if m and k:
         if q.data_ptr() % 4 or q.stride(0) % 4:
             q = q.clone(memory_format=torch.contiguous_format)
-        sc = s if s.is_contiguous() and s.data_ptr() % 4 == 0 else s.clone(memory_format=torch.contiguous_format)
-        dev = q.get_device()
-        _native.on_device(dev, _native.load().i8l_dequant_mxfp4, (
-            q.data_ptr(), q.stride(0), sc.data_ptr(), out.data_ptr(), k, _FLOAT[out_dtype], m, k,
-            current_stream(dev)))
+        _native.on_device(dev, _native.load().i8l_dequant_mxfp4, q.data_ptr(), q.stride(0), s.data_ptr(),
+                          out.data_ptr(), k, _FLOAT[out_dtype], m, k, current_stream(dev))
     return out
 
 
@@ -164,13 +163,6 @@ def _tile(config: Config) -> _native.I8LTile:
                            "(128 x 256, split 4)")
     return _native.I8LTile(swap_ab=1, tok_tile=config.bm, w_tile=128, stages=config.stages, split=config.split,
                            cluster=1 if config.split == 1 else config.cluster)
-
-
-def _aligned16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy of it if its rows do not start on 16-byte boundaries (what TMA needs)."""
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
 
 
 def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
@@ -191,43 +183,43 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
     if a_q.dim() != 2 or b_q.dim() != 2 or a_q.shape[1] != b_q.shape[0]:
         raise ValueError(f"cannot multiply {tuple(a_q.shape)} by {tuple(b_q.shape)}")
     m, half = a_q.shape
-    n, k = b_q.shape[1], 2 * half
+    n, k, dev = b_q.shape[1], 2 * half, a_q.get_device()
     if k == 0 or k % BLOCK:
         raise NotSupported(f"K={k} must be a positive multiple of {BLOCK} (whole blocks)")
-    if n > 1 and b_q.stride(0) != 1:
+    if b_q.stride(0) != 1 and n > 1:
         raise NotSupported("b_q must be the K-contiguous [K/2, N] view of an [N, K/2] weight")
-    _operand(a_q, scale_a, m, k, "scale_a")
-    _operand(b_q, scale_b, n, k, "scale_b")
+    if dev < 0 or b_q.get_device() != dev:
+        raise ValueError(f"w4a4_mm runs on one CUDA device; got tensors on {a_q.device} and {b_q.device}")
+    sa, sb = _scales(scale_a, m, k, dev, "scale_a"), _scales(scale_b, n, k, dev, "scale_b")
+    bias_ptr, bias_code = None, 0
     if bias is not None:
-        if tuple(bias.shape) != (n,) or bias.device != a_q.device:
+        if bias.shape != (n,) or bias.get_device() != dev:
             raise ValueError(f"bias must have shape ({n},) on {a_q.device}, got {tuple(bias.shape)} on {bias.device}")
         if bias.dtype not in _FLOAT:
             raise NotSupported(f"bias dtype {bias.dtype} not supported")
         bias = bias if bias.is_contiguous() else bias.contiguous()
+        bias_ptr, bias_code = bias.data_ptr(), _FLOAT[bias.dtype]
     if out_dtype not in _FLOAT:
         raise NotSupported(f"output dtype {out_dtype} not supported")
-    if not a_q.is_cuda or b_q.device != a_q.device:
-        raise ValueError(f"w4a4_mm runs on one CUDA device; got tensors on {a_q.device} and {b_q.device}")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=a_q.device)
-    elif tuple(out.shape) != (m, n) or out.dtype != out_dtype or out.device != a_q.device \
-            or (n > 1 and out.stride(1) != 1):
+        out = a_q.new_empty((m, n), dtype=out_dtype)
+    elif out.shape != (m, n) or out.dtype != out_dtype or out.get_device() != dev \
+            or (out.stride(1) != 1 and n > 1):
         raise ValueError(f"out must be a {out_dtype} [{m}, {n}] tensor with contiguous rows on "
                          f"{a_q.device}, got {out.dtype} {tuple(out.shape)} strides {out.stride()}")
-    tile = _tile(config) if config is not None else None
+    tile = ctypes.byref(_tile(config)) if config is not None else None
     if m == 0 or n == 0:
         return out
-    a, w = _aligned16(a_q), b_q.t()
-    if b_q.data_ptr() % 16 or b_q.stride(1) % 16:
-        w = _aligned16(w)
-    sa, sb = (s if s.is_contiguous() and s.data_ptr() % 16 == 0 else s.clone(memory_format=torch.contiguous_format)
-              for s in (scale_a, scale_b))
-    dev = a_q.get_device()
-    _native.on_device(dev, _native.load().i8l_w4a4_mm, (
-        a.data_ptr(), a.stride(0), sa.data_ptr(), w.data_ptr(), w.stride(0), sb.data_ptr(),
-        bias.data_ptr() if bias is not None else None, _FLOAT[bias.dtype] if bias is not None else 0,
-        out.data_ptr(), _FLOAT[out_dtype], out.stride(0), m, n, k,
-        ctypes.byref(tile) if tile is not None else None, current_stream(dev)))
+    # TMA reads rows that start on 16-byte boundaries; others are copied.
+    if a_q.data_ptr() % 16 or a_q.stride(0) % 16 or a_q.stride(1) != 1:
+        a_q = a_q.clone(memory_format=torch.contiguous_format)
+    wp, ldw = b_q.data_ptr(), b_q.stride(1)
+    if wp % 16 or ldw % 16 or b_q.stride(0) != 1:
+        w = b_q.t().clone(memory_format=torch.contiguous_format)
+        wp, ldw = w.data_ptr(), half
+    _native.on_device(dev, _native.load().i8l_w4a4_mm, a_q.data_ptr(), a_q.stride(0), sa.data_ptr(), wp, ldw,
+                      sb.data_ptr(), bias_ptr, bias_code, out.data_ptr(), _FLOAT[out_dtype], out.stride(0), m, n, k,
+                      tile, current_stream(dev))
     return out
 
 

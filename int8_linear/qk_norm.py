@@ -23,8 +23,8 @@ __all__ = ["qk_norm_rope"]
 
 def _out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if tuple(out.shape) != shape or out.dtype != like.dtype or out.device != like.device \
+        return like.new_empty(shape)
+    if out.shape != shape or out.dtype != like.dtype or out.get_device() != like.get_device() \
             or out.stride(2) != 1 or out.stride(1) != shape[2]:
         raise ValueError(f"{name} must be a {like.dtype} {list(shape)} tensor on {like.device} whose heads "
                          f"follow one another, got {out.dtype} {tuple(out.shape)} strides {out.stride()}")
@@ -54,37 +54,38 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     arguments.  R = 0 only normalises."""
     if qkv.dtype not in _ACT:
         raise NotSupported(f"activations must be bfloat16 or float16, got {qkv.dtype}")
-    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+    if qkv.dim() != 2 or (qkv.stride(1) != 1 and qkv.shape[1] > 1):
         raise NotSupported("qkv must be a 2-D activation with contiguous rows")
     m, width = qkv.shape
-    d = q_weight.numel()
-    if q_weight.dtype not in _WEIGHT or k_weight.dtype != q_weight.dtype or k_weight.numel() != d or d == 0:
+    d, dev = q_weight.numel(), qkv.get_device()
+    wdt = q_weight.dtype
+    if wdt not in _WEIGHT or k_weight.dtype != wdt or k_weight.numel() != d or d == 0:
         raise ValueError(f"q_weight and k_weight must hold one head's values in one bf16/fp16/fp32 type, got "
                          f"{q_weight.dtype} {tuple(q_weight.shape)} and {k_weight.dtype} {tuple(k_weight.shape)}")
     if heads < 0 or kv_heads < 0 or width < (heads + kv_heads) * d:
         raise ValueError(f"qkv rows of {width} values do not hold {heads} + {kv_heads} heads of {d}")
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (m,):
+    wide = positions.dtype == torch.int64
+    if not (wide or positions.dtype == torch.int32) or positions.shape != (m,):
         raise ValueError(f"positions must be {m} int32 or int64 values, got {positions.dtype} "
                          f"{tuple(positions.shape)}")
     if cos_sin.dim() != 2 or cos_sin.dtype not in _WEIGHT or cos_sin.shape[1] > d or cos_sin.shape[1] % 2:
         raise ValueError(f"cos_sin must be a bf16/fp16/fp32 [positions, even rot <= {d}] table, got "
                          f"{cos_sin.dtype} {tuple(cos_sin.shape)}")
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("positions", positions),
-                    ("cos_sin", cos_sin)):
-        if t.device != qkv.device:
-            raise ValueError(f"{name} is on {t.device}, qkv on {qkv.device}")
-    if not qkv.is_cuda:
+    if dev < 0:
         raise ValueError(f"qk_norm_rope runs on a CUDA device, got {qkv.device}")
+    if not (q_weight.get_device() == k_weight.get_device() == positions.get_device() == cos_sin.get_device() == dev):
+        raise ValueError(f"the weights, positions and cos_sin must be on {qkv.device}")
     q = _out(q_out, (m, heads, d), qkv, "q_out")
     k = _out(k_out, (m, kv_heads, d), qkv, "k_out")
     if m == 0 or heads + kv_heads == 0:
         return q, k
-    wq, wk, pos, table = (t if t.is_contiguous() else t.contiguous()
-                          for t in (q_weight, k_weight, positions, cos_sin))
-    dev = qkv.get_device()
-    args = (qkv.data_ptr(), qkv.stride(0), _ACT[qkv.dtype], wq.data_ptr(), wk.data_ptr(), _WEIGHT[wq.dtype],
-            eps, pos.data_ptr(), pos.dtype == torch.int64, table.data_ptr(), _WEIGHT[table.dtype],
-            table.shape[0], q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), m, heads, kv_heads, d,
-            table.shape[1], interleaved, current_stream(dev))
-    _native.on_device(dev, _native.load().i8l_qk_norm_rope, args)
+    wq = q_weight if q_weight.is_contiguous() else q_weight.contiguous()
+    wk = k_weight if k_weight.is_contiguous() else k_weight.contiguous()
+    pos = positions if positions.is_contiguous() else positions.contiguous()
+    table = cos_sin if cos_sin.is_contiguous() else cos_sin.contiguous()
+    length, rot = table.shape
+    _native.on_device(dev, _native.load().i8l_qk_norm_rope, qkv.data_ptr(), qkv.stride(0), _ACT[qkv.dtype],
+                      wq.data_ptr(), wk.data_ptr(), _WEIGHT[wdt], eps, pos.data_ptr(), wide, table.data_ptr(),
+                      _WEIGHT[table.dtype], length, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), m, heads,
+                      kv_heads, d, rot, interleaved, current_stream(dev))
     return q, k
