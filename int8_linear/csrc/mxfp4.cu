@@ -22,6 +22,7 @@
 namespace i8l {
 
 constexpr int kFlatThreads = 256;
+constexpr int64_t kBlockThreadsMin = 148 * 256;  // blocks from which a thread takes a whole one
 
 struct MxOut {
   uint8_t *q;
@@ -63,6 +64,27 @@ __device__ __forceinline__ void load8(const void *base, long long idx, bool vec,
   }
 }
 
+// Eight 16-bit values from any alignment, as they lie in memory.
+__device__ __forceinline__ uint4 load8_raw(const void *base, long long idx, bool vec) {
+  const uint16_t *p = static_cast<const uint16_t *>(base) + idx;
+  if (vec) return *reinterpret_cast<const uint4 *>(p);
+  return make_uint4(p[0] | (static_cast<uint32_t>(p[1]) << 16), p[2] | (static_cast<uint32_t>(p[3]) << 16),
+                    p[4] | (static_cast<uint32_t>(p[5]) << 16), p[6] | (static_cast<uint32_t>(p[7]) << 16));
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack8(const uint4 &w, float (&v)[8]) {
+  unpack2<DT>(w.x, v[0], v[1]);
+  unpack2<DT>(w.y, v[2], v[3]);
+  unpack2<DT>(w.z, v[4], v[5]);
+  unpack2<DT>(w.w, v[6], v[7]);
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7]));
+}
+
 // ------------------------------------------------------------------ SiLU
 
 // float32(g / (1 + exp(-g)) * u) in float64: within 2^-50 of the exact value before its
@@ -70,17 +92,6 @@ __device__ __forceinline__ void load8(const void *base, long long idx, bool vec,
 __device__ __noinline__ float silu_mul_exact(float g, float u) {
   const double gd = g;
   return static_cast<float>(gd / (1.0 + exp(-gd)) * static_cast<double>(u));
-}
-
-// Rounds two floats to the 16-bit type and packs them, v0 low.
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float v0, float v1) {
-  uint32_t p;
-  if constexpr (DT == I8L_BF16)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(v1), "f"(v0));
-  else
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(v1), "f"(v0));
-  return p;
 }
 
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -142,68 +153,138 @@ struct FlatArgs {
   uint32_t vectors;        // rows * blocks * 4
   uint32_t pad_words;      // zero words below the last row
   FastDiv per_row;         // vectors per row
-  int vec;                 // 16-byte loads allowed
+  int vec;                 // 1: 16-byte loads allowed, 2: 32-byte loads
+  int q16;                 // 16-byte stores of codes allowed
 };
 
-// Eight 16-bit values from any alignment, as they lie in memory.
-__device__ __forceinline__ uint4 load8_raw(const void *base, long long idx, bool vec) {
-  const uint16_t *p = static_cast<const uint16_t *>(base) + idx;
-  if (vec) return *reinterpret_cast<const uint4 *>(p);
-  return make_uint4(p[0] | (static_cast<uint32_t>(p[1]) << 16), p[2] | (static_cast<uint32_t>(p[3]) << 16),
-                    p[4] | (static_cast<uint32_t>(p[5]) << 16), p[6] | (static_cast<uint32_t>(p[7]) << 16));
+// 32 bytes at a 32-byte boundary: a whole DRAM sector per lane.
+__device__ __forceinline__ void ld_v8(const void *p, uint32_t *w) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void st_v8(void *p, const uint32_t *w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
-// kSilu: x holds [gate | up] rows of 2K values.  Each thread takes U vectors, a block's
-// width of threads apart, and loads them all before it works on the first.
-template <int DT, bool kSilu, int U>
+// A block of 32 16-bit values, two to a word.
+__device__ __forceinline__ void load_block(const void *base, long long idx, int vec, uint32_t (&w)[16]) {
+  const uint16_t *p = static_cast<const uint16_t *>(base) + idx;
+  if (vec == 2) {
+    ld_v8(p, w);
+    ld_v8(p + 16, w + 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = load8_raw(base, idx + 8 * i, vec);
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+  }
+}
+
+// Largest magnitude, as float32 bits, of 32 16-bit values.  The signed maximum of the bits is
+// that of the positive values, the unsigned one that of the negative values where there are
+// any; with the sign cleared, the larger of both is the block's (NaN and infinity included).
+template <int DT>
+__device__ __forceinline__ uint32_t mx_amax32(const uint32_t (&w)[16]) {
+  uint32_t s = w[0], u = w[0];
+#pragma unroll
+  for (int i = 1; i < 15; i += 2) {
+    s = __vimax3_s16x2(s, w[i], w[i + 1]);
+    u = __vimax3_u16x2(u, w[i], w[i + 1]);
+  }
+  s = __vmaxs2(s, w[15]);
+  u = __vmaxu2(u, w[15]);
+  uint32_t m = __vmaxu2(s & 0x7fff7fffu, u & 0x7fff7fffu);
+  m = max(m & 0xffffu, m >> 16);
+  if constexpr (DT == I8L_BF16) return m << 16;
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+}
+
+// Four lanes a block, one vector of eight values a thread.  kSilu: x holds [gate | up] rows
+// of 2K values.
+template <int DT, bool kSilu>
 __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a) {
   static_assert(!kSilu || DT != I8L_F32, "SiLU takes 16-bit activations");
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t base = blockIdx.x * (kFlatThreads * U) + threadIdx.x;
-  const long long K = static_cast<long long>(a.blocks) * kMxBlock;
-  constexpr bool kWide = DT == I8L_F32;
-  uint4 x[kWide ? 1 : U], up[kSilu ? U : 1];
-  float y[kWide ? U : 1][8];
-  uint32_t row[U], vec[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t id = base + u * kFlatThreads;
-    row[u] = a.per_row.div(id);
-    vec[u] = id - row[u] * a.per_row.d;
-    const bool in = id < a.vectors;
-    const long long at = row[u] * a.ldx + vec[u] * 8u;
-    if constexpr (kWide) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[u][i] = 0.f;
-      if (in) load8<DT>(a.x, at, a.vec, y[u]);
-    } else {
-      x[u] = in ? load8_raw(a.x, at, a.vec) : make_uint4(0u, 0u, 0u, 0u);
-      if constexpr (kSilu) up[u] = in ? load8_raw(a.x, at + K, a.vec) : make_uint4(0u, 0u, 0u, 0u);
+  const uint32_t id = blockIdx.x * kFlatThreads + threadIdx.x;
+  const uint32_t row = a.per_row.div(id), vec = id - row * a.per_row.d;
+  const bool in = id < a.vectors;
+  const long long at = row * a.ldx + vec * 8u;
+  uint32_t byte, w;
+  if constexpr (DT == I8L_F32) {
+    float y[8] = {};
+    if (in) load8<DT>(a.x, at, a.vec, y);
+    w = mx_quantise8(y, byte);
+  } else {
+    uint4 x = in ? load8_raw(a.x, at, a.vec) : make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (kSilu) {
+      const long long K = static_cast<long long>(a.blocks) * kMxBlock;
+      const uint4 up = in ? load8_raw(a.x, at + K, a.vec) : make_uint4(0u, 0u, 0u, 0u);
+      x.x = silu_mul2<DT>(x.x, up.x);
+      x.y = silu_mul2<DT>(x.y, up.y);
+      x.z = silu_mul2<DT>(x.z, up.z);
+      x.w = silu_mul2<DT>(x.w, up.w);
     }
+    w = mx_quantise8<DT>(x, byte);
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t id = base + u * kFlatThreads;
-    uint32_t byte, w;
-    if constexpr (kWide) {
-      w = mx_quantise8(y[u], byte);
-    } else {
-      if constexpr (kSilu) {
-        x[u].x = silu_mul2<DT>(x[u].x, up[u].x);
-        x[u].y = silu_mul2<DT>(x[u].y, up[u].y);
-        x[u].z = silu_mul2<DT>(x[u].z, up[u].z);
-        x[u].w = silu_mul2<DT>(x[u].w, up[u].w);
-      }
-      w = mx_quantise8<DT>(x[u], byte);
-    }
-    if (id < a.vectors) {
-      *reinterpret_cast<uint32_t *>(a.o.q + row[u] * a.o.ldq + vec[u] * 4u) = w;
-      if ((threadIdx.x & 3) == 0) store_sf(a.o, row[u], static_cast<int>(vec[u] >> 2), a.blocks, byte);
-    } else if (id - a.vectors < a.pad_words) {
-      zero_pad_word(a.o, a.rows, id - a.vectors);
-    }
+  if (in) {
+    *reinterpret_cast<uint32_t *>(a.o.q + row * a.o.ldq + vec * 4u) = w;
+    if ((threadIdx.x & 3) == 0) store_sf(a.o, row, static_cast<int>(vec >> 2), a.blocks, byte);
+  } else if (id - a.vectors < a.pad_words) {
+    zero_pad_word(a.o, a.rows, id - a.vectors);
   }
+}
+
+// The flat quantisers for matrices that fill the GPU: one thread takes a whole block, so
+// there is nothing to exchange, and addresses, the scale and the index arithmetic are shared
+// by 32 values instead of 8.  The four-lanes-a-block kernel above was bound by instruction
+// issue (77 % of the slots, 111 instructions per 8 values, 50 % of HBM at 8192 x 8192), but
+// spreads a small matrix over four times as many threads.
+template <int DT, bool kSilu>
+__global__ void __launch_bounds__(kFlatThreads) mx_block_kernel(const FlatArgs a) {
+  static_assert(DT != I8L_F32, "16-bit values");
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t id = blockIdx.x * kFlatThreads + threadIdx.x;
+  const uint32_t total = a.vectors >> 2;
+  if (id >= total) {
+    if (id - total < a.pad_words) zero_pad_word(a.o, a.rows, id - total);
+    return;
+  }
+  const uint32_t row = a.per_row.div(id), block = id - row * a.per_row.d;
+  const long long at = row * a.ldx + block * static_cast<long long>(kMxBlock);
+  uint32_t x[16];
+  load_block(a.x, at, a.vec, x);
+  if constexpr (kSilu) {
+    uint32_t up[16];
+    load_block(a.x, at + static_cast<long long>(a.blocks) * kMxBlock, a.vec, up);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = silu_mul2<DT>(x[i], up[i]);
+  }
+  const uint32_t byte = mx_scale_byte(mx_amax32<DT>(x));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[8];
+    unpack8<DT>(make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]), y);
+    w[i] = byte == 255u ? 0u : mx_pack8(y, mx_inv_scale(byte));
+  }
+  uint8_t *q = a.o.q + row * a.o.ldq + block * 16u;
+  if (a.q16) {
+    *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t *>(q)[i] = w[i];
+  }
+  store_sf(a.o, row, static_cast<int>(block), a.blocks, byte);
 }
 
 // ------------------------------------------------------------------ add + RMSNorm
@@ -224,22 +305,11 @@ struct MxNormArgs {
   int vec;  // 16-byte loads and stores allowed
 };
 
-__device__ __forceinline__ double block_sum_f64(double v, double *red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
-  if (l == 0) red[w] = v;
-  __syncthreads();
-  v = l < nw ? red[l] : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // One row per CTA, the row in registers.  The squares are summed in float64 (a float32
-// squares exactly into one) and 1/sqrt(mean + eps) is rounded once to float32, so the
-// factor does not depend on the order of the sum.
-template <int DT, int NV>
+// squares exactly into one) and 1/sqrt(mean + eps) is rounded once to float32, so the factor
+// does not depend on the order of the sum; the first warp computes it for the row, as the
+// square root and the division are worth a vector's arithmetic to each thread.
+template <int DT, int WDT, int NV>
 __global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -251,54 +321,72 @@ __global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) 
     return;
   }
   __shared__ double red[32];
+  __shared__ float factor;
+  uint4 xr[NV], rr[NV];
   float h[NV][8];
-  double ss = 0.0;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int col = col_of<8>(v);
+    xr[v] = rr[v] = make_uint4(0u, 0u, 0u, 0u);
     if (col < a.K) {
-      load8<DT>(a.x, row * a.ldx + col, a.vec, h[v]);
-      if (a.res) {
-        float r[8];
-        load8<DT>(a.res, row * a.ldr + col, a.vec, r);
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) add2_rn(h[v][i], h[v][i + 1], h[v][i], h[v][i + 1], r[i], r[i + 1]);
-        T *p = static_cast<T *>(a.rout) + row * a.ldro;
-        if (a.vec) {
-          store_vec<DT, 8>(p, col, h[v]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) p[col + i] = ActType<DT>::from_f32(h[v][i]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fma(static_cast<double>(h[v][i]), static_cast<double>(h[v][i]), ss);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[v][i] = 0.f;
+      xr[v] = load8_raw(a.x, row * a.ldx + col, a.vec);
+      if (a.res) rr[v] = load8_raw(a.res, row * a.ldr + col, a.vec);
     }
   }
-  ss = block_sum_f64(ss, red);
-  const float rs = static_cast<float>(1.0 / sqrt(ss / a.K + a.eps));
+  double ss = 0.0;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    unpack8<DT>(xr[v], h[v]);
+    const int col = col_of<8>(v);
+    if (a.res) {
+      float r[8];
+      unpack8<DT>(rr[v], r);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) add2_rn(h[v][i], h[v][i + 1], h[v][i], h[v][i + 1], r[i], r[i + 1]);
+      if (col < a.K) {
+        T *p = static_cast<T *>(a.rout) + row * a.ldro + col;
+        if (a.vec) {
+          *reinterpret_cast<uint4 *>(p) = pack8<DT>(h[v]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] = ActType<DT>::from_f32(h[v][i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double d = h[v][i];
+      ss = fma(d, d, ss);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    ss = threadIdx.x < blockDim.x >> 5 ? red[threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);  // at most 8 warps
+    if (threadIdx.x == 0) factor = static_cast<float>(1.0 / sqrt(ss / a.K + a.eps));
+  }
+  __syncthreads();
+  const float rs = factor;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int col = col_of<8>(v);
     if (col < a.K) {
       float w[8];
-      load_weight_vec<8>(a.w, a.w_dtype, col, a.w_vec != 0, w);
+      load_weight_vec<8>(a.w, WDT, col, a.w_vec != 0, w);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         float n0, n1;
         mul2_rn(n0, n1, h[v][i], h[v][i + 1], rs, rs);
-        n0 = round_to_weight(n0, a.w_dtype);
-        n1 = round_to_weight(n1, a.w_dtype);
+        round2_through<WDT>(n0, n1);
         mul2_rn(h[v][i], h[v][i + 1], n0, n1, w[i], w[i + 1]);
       }
     }
-    const uint4 y = make_uint4(pack2<DT>(h[v][0], h[v][1]), pack2<DT>(h[v][2], h[v][3]), pack2<DT>(h[v][4], h[v][5]),
-                               pack2<DT>(h[v][6], h[v][7]));
     uint32_t byte;
-    const uint32_t packed = mx_quantise8<DT>(y, byte);
+    const uint32_t packed = mx_quantise8<DT>(pack8<DT>(h[v]), byte);
     if (col < a.K) {
       *reinterpret_cast<uint32_t *>(a.o.q + row * a.o.ldq + col / 2) = packed;
       if ((threadIdx.x & 3) == 0) store_sf(a.o, row, col / kMxBlock, a.K / kMxBlock, byte);
@@ -315,49 +403,57 @@ struct DeqArgs {
   int ktiles;
   void *out;
   long long ldo;
-  uint32_t vectors;
+  uint32_t blocks;  // in all
   FastDiv per_row;
-  int vec;
+  int vec;  // 32-byte stores allowed
+  int q16;  // 16-byte loads of codes allowed
 };
 
-template <int DT, int U>
+// One thread per block.
+template <int DT>
 __global__ void __launch_bounds__(kFlatThreads) mx_dequant_kernel(const DeqArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   using T = typename ActType<DT>::T;
-  const uint32_t base = blockIdx.x * (kFlatThreads * U) + threadIdx.x;
-  uint32_t row[U], vec[U], w[U], byte[U];
+  const uint32_t id = blockIdx.x * kFlatThreads + threadIdx.x;
+  if (id >= a.blocks) return;
+  const uint32_t row = a.per_row.div(id), block = id - row * a.per_row.d;
+  const uint8_t *q = a.q + row * a.ldq + block * 16u;
+  uint32_t w[4];
+  if (a.q16) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(q);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  } else {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t id = base + u * kFlatThreads;
-    row[u] = a.per_row.div(id);
-    vec[u] = id - row[u] * a.per_row.d;
-    w[u] = byte[u] = 0u;
-    if (id < a.vectors) {
-      w[u] = *reinterpret_cast<const uint32_t *>(a.q + row[u] * a.ldq + vec[u] * 4u);
-      const int block = static_cast<int>(vec[u] >> 2);
-      byte[u] = a.sf[sf_word_offset(row[u], block >> 2, a.ktiles) + (block & 3)];
-    }
+    for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t *>(q)[i];
   }
+  const float s = mx_scale_value(a.sf[sf_word_offset(row, static_cast<int>(block >> 2), a.ktiles) + (block & 3)]);
+  T *out = static_cast<T *>(a.out) + row * a.ldo + block * static_cast<long long>(kMxBlock);
+  constexpr int kWords = DT == I8L_F32 ? 8 : 4;  // of eight values
+  uint32_t o[2 * kWords];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (base + u * kFlatThreads >= a.vectors) continue;
+  for (int i = 0; i < 4; ++i) {
     float v[8];
-    mx_unpack8(w[u], v);
-    const float s = mx_scale_value(byte[u]);
+    mx_unpack8(w[i], v);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) mul2_rn(v[i], v[i + 1], v[i], v[i + 1], s, s);
-    T *p = static_cast<T *>(a.out) + row[u] * a.ldo + vec[u] * 8u;
-    if (a.vec) {
-      if constexpr (DT == I8L_F32) {
-        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        store_vec<DT, 8>(p, 0, v);
-      }
+    for (int j = 0; j < 8; j += 2) mul2_rn(v[j], v[j + 1], v[j], v[j + 1], s, s);
+    uint32_t *p = o + (i & 1) * kWords;
+    if constexpr (DT == I8L_F32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __float_as_uint(v[j]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = ActType<DT>::from_f32(v[i]);
+      for (int j = 0; j < 4; ++j) p[j] = pack2<DT>(v[2 * j], v[2 * j + 1]);
+    }
+    if (!a.vec) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[8 * i + j] = ActType<DT>::from_f32(v[j]);
+    } else if (i & 1) {
+#pragma unroll
+      for (int j = 0; j < 2 * kWords; j += 8) st_v8(reinterpret_cast<uint32_t *>(out) + (i - 1) * kWords + j, o + j);
     }
   }
 }
@@ -414,21 +510,34 @@ int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uin
     a.blocks = blocks;
     a.vectors = static_cast<uint32_t>(rows) * (blocks * 4u);
     a.pad_words = static_cast<uint32_t>(pad) * ktiles;
-    a.per_row = FastDiv(blocks * 4u);
-    a.vec = vec_rows(x, ldx, dtype) && (!kSilu || (static_cast<int64_t>(K) * act_size(dtype)) % 16 == 0);
-    constexpr int U = kSilu ? 1 : 2;
-    const int64_t work = static_cast<int64_t>(a.vectors) + a.pad_words;
-    const dim3 grid(static_cast<unsigned>((work + kFlatThreads * U - 1) / (kFlatThreads * U)));
+    a.vec = vec_rows(x, ldx, dtype) && (!kSilu || (static_cast<int64_t>(K) * act_size(dtype)) % 16 == 0) ? 1 : 0;
+    a.q16 = aligned16(q) && ldq % 16 == 0 ? 1 : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err;
-    if (dtype == I8L_BF16)
-      err = launch(mx_quant_kernel<I8L_BF16, kSilu, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
-    else if (dtype == I8L_F16)
-      err = launch(mx_quant_kernel<I8L_F16, kSilu, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
-    else if constexpr (!kSilu)
-      err = launch(mx_quant_kernel<I8L_F32, false, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
-    else
-      err = cudaErrorInvalidValue;
+    // A thread per block from 256 threads an SM on: with fewer, four lanes a block finish
+    // sooner (MEASURE).
+    const int64_t total = a.vectors / 4;
+    if (dtype != I8L_F32 && total >= kBlockThreadsMin) {
+      if (a.vec && reinterpret_cast<uintptr_t>(x) % 32 == 0 && (ldx * 2) % 32 == 0) a.vec = 2;
+      a.per_row = FastDiv(blocks);
+      const dim3 grid(static_cast<unsigned>((total + a.pad_words + kFlatThreads - 1) / kFlatThreads));
+      if (dtype == I8L_BF16)
+        err = launch(mx_block_kernel<I8L_BF16, kSilu>, grid, dim3(kFlatThreads), 0, s, 1, a);
+      else
+        err = launch(mx_block_kernel<I8L_F16, kSilu>, grid, dim3(kFlatThreads), 0, s, 1, a);
+    } else {
+      a.per_row = FastDiv(blocks * 4u);
+      const int64_t work = static_cast<int64_t>(a.vectors) + a.pad_words;
+      const dim3 grid(static_cast<unsigned>((work + kFlatThreads - 1) / kFlatThreads));
+      if (dtype == I8L_BF16)
+        err = launch(mx_quant_kernel<I8L_BF16, kSilu>, grid, dim3(kFlatThreads), 0, s, 1, a);
+      else if (dtype == I8L_F16)
+        err = launch(mx_quant_kernel<I8L_F16, kSilu>, grid, dim3(kFlatThreads), 0, s, 1, a);
+      else if constexpr (!kSilu)
+        err = launch(mx_quant_kernel<I8L_F32, false>, grid, dim3(kFlatThreads), 0, s, 1, a);
+      else
+        err = cudaErrorInvalidValue;
+    }
     if (int e = finish_launch(err, what)) return e;
   }
   return I8L_OK;
@@ -503,11 +612,19 @@ extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const voi
   const dim3 grid(static_cast<unsigned>(M) + (a.pad_words + th - 1) / th);
   cudaError_t err = cudaSuccess;
   a.vec = vec ? 1 : 0;
+#define I8L_MX_NORM(ADT, WDTV) \
+  I8L_DISPATCH_NV(nv, (err = launch(mx_norm_quant_kernel<ADT, WDTV, NV>, grid, dim3(th), 0, s, 1, a)))
+#define I8L_MX_NORM_W(ADT)                                              \
+  if (w_dtype == I8L_BF16) { I8L_MX_NORM(ADT, I8L_BF16) }               \
+  else if (w_dtype == I8L_F16) { I8L_MX_NORM(ADT, I8L_F16) }            \
+  else { I8L_MX_NORM(ADT, I8L_F32) }
   if (act_dtype == I8L_BF16) {
-    I8L_DISPATCH_NV(nv, (err = launch(mx_norm_quant_kernel<I8L_BF16, NV>, grid, dim3(th), 0, s, 1, a)))
+    I8L_MX_NORM_W(I8L_BF16)
   } else {
-    I8L_DISPATCH_NV(nv, (err = launch(mx_norm_quant_kernel<I8L_F16, NV>, grid, dim3(th), 0, s, 1, a)))
+    I8L_MX_NORM_W(I8L_F16)
   }
+#undef I8L_MX_NORM_W
+#undef I8L_MX_NORM
   return finish_launch(err, "add_rmsnorm_quant_mxfp4 launch");
 }
 
@@ -530,19 +647,19 @@ extern "C" int i8l_dequant_mxfp4(const uint8_t *q, int64_t ldq, const uint8_t *s
     a.ktiles = ktiles;
     a.out = static_cast<uint8_t *>(out) + r0 * ldo * act_size(out_dtype);
     a.ldo = ldo;
-    a.vectors = static_cast<uint32_t>(rows) * (K / 8u);
-    a.per_row = FastDiv(K / 8u);
-    a.vec = vec_rows(out, ldo, out_dtype);
-    constexpr int U = 4;
-    const dim3 grid((a.vectors + kFlatThreads * U - 1) / (kFlatThreads * U));
+    a.blocks = static_cast<uint32_t>(rows) * (K / kMxBlock);
+    a.per_row = FastDiv(K / kMxBlock);
+    a.vec = reinterpret_cast<uintptr_t>(out) % 32 == 0 && (ldo * act_size(out_dtype)) % 32 == 0 ? 1 : 0;
+    a.q16 = aligned16(q) && ldq % 16 == 0 ? 1 : 0;
+    const dim3 grid((a.blocks + kFlatThreads - 1) / kFlatThreads);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err;
     if (out_dtype == I8L_BF16)
-      err = launch(mx_dequant_kernel<I8L_BF16, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+      err = launch(mx_dequant_kernel<I8L_BF16>, grid, dim3(kFlatThreads), 0, s, 1, a);
     else if (out_dtype == I8L_F16)
-      err = launch(mx_dequant_kernel<I8L_F16, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+      err = launch(mx_dequant_kernel<I8L_F16>, grid, dim3(kFlatThreads), 0, s, 1, a);
     else
-      err = launch(mx_dequant_kernel<I8L_F32, U>, grid, dim3(kFlatThreads), 0, s, 1, a);
+      err = launch(mx_dequant_kernel<I8L_F32>, grid, dim3(kFlatThreads), 0, s, 1, a);
     if (int e = finish_launch(err, "dequant_mxfp4 launch")) return e;
   }
   return I8L_OK;

@@ -263,6 +263,17 @@ __device__ __forceinline__ void unpack2(uint32_t w, float &v0, float &v1) {
   }
 }
 
+// Rounds two floats to the 16-bit type and packs them, v0 low.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float v0, float v1) {
+  uint32_t p;
+  if constexpr (DT == I8L_BF16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(v1), "f"(v0));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(v1), "f"(v0));
+  return p;
+}
+
 // The same for eight bf16 or fp16 values as they lie in memory.  16-bit floats of one sign
 // are ordered as their bits are, NaN and infinity last, so the maximum is taken two at a
 // time on the bits.

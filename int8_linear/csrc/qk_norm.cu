@@ -41,14 +41,15 @@ struct QkArgs {
   int parts;       // groups per token, each with up to P heads
   uint32_t groups;  // tokens * parts, below 2^31
   FastDiv per_token;  // parts
-  float eps;
+  float eps, inv_dim;
   int interleaved;
   int w_vec, cs_vec;
 };
 
-// G lanes per head (a power of two, G * 8 >= dim), P heads per group.  In place is fine: a lane stores the
+// G lanes per head (a power of two, G * 8 >= dim), P heads per group; kFull: every value is
+// rotated (rot == dim).  In place is fine: a lane stores the
 // elements that it alone loaded, after every exchange within its head.
-template <int DT, int G, int P>
+template <int DT, int G, int P, bool kFull>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a
   // The lane of this group that holds the other values of this lane's pairs.
   const int partner = !a.interleaved && turns ? (c0 < half ? lane + half / 8 : lane - half / 8) : lane;
 
-  float w[8];
+  float w[8] = {};
   int loaded = -1;  // which weight `w` holds: 0 queries, 1 keys
 #pragma unroll
   for (int turn = 0; turn < P; ++turn) {
@@ -113,33 +114,30 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a
     if (here && key != loaded) load_weight_vec<8>(key ? a.wk : a.wq, a.w_dtype, c0, a.w_vec != 0, w);
     loaded = key;
     float x[8];
-    const T *h = reinterpret_cast<const T *>(&raw[turn]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ActType<DT>::to_f32(h[i]);
+    unpack2<DT>(raw[turn].x, x[0], x[1]);
+    unpack2<DT>(raw[turn].y, x[2], x[3]);
+    unpack2<DT>(raw[turn].z, x[4], x[5]);
+    unpack2<DT>(raw[turn].w, x[6], x[7]);
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
-    float rs = 1.0f / sqrtf(ss / static_cast<float>(a.dim) + a.eps);
+    float rs = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
     if (!known) rs = __int_as_float(0x7fc00000);
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = here ? x[i] * rs * w[i] : 0.f;
-    if (a.interleaved) {
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * w[i];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = turns ? x[i] * cs[i] + x[i ^ 1] * sn[i] : x[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = __shfl_sync(0xffffffffu, x[i], partner, G);
-        y[i] = turns ? x[i] * cs[i] + other * sn[i] : x[i];
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float other = a.interleaved ? x[i ^ 1] : __shfl_sync(0xffffffffu, x[i], partner, G);
+      y[i] = kFull || turns ? fmaf(x[i], cs[i], other * sn[i]) : x[i];
     }
     if (here) {
       T *dst = key ? static_cast<T *>(a.k) + token * a.ldk + static_cast<long long>(head - a.heads) * a.dim
                    : static_cast<T *>(a.q) + token * a.ldq + static_cast<long long>(head) * a.dim;
-      store_vec<DT, 8>(dst, c0, y);
+      *reinterpret_cast<uint4 *>(dst + c0) =
+          make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
     }
   }
 }
@@ -150,17 +148,17 @@ using namespace i8l;
 
 namespace {
 
-template <int DT, int P>
+template <int DT, int P, bool kFull>
 cudaError_t launch_qk(const QkArgs &a, int lanes, cudaStream_t s) {
   const unsigned per_block = kQkThreads / lanes;
   const dim3 grid((a.groups + per_block - 1) / per_block);
   switch (lanes) {
-    case 1: return launch(qk_norm_rope_kernel<DT, 1, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 2: return launch(qk_norm_rope_kernel<DT, 2, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 4: return launch(qk_norm_rope_kernel<DT, 4, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 8: return launch(qk_norm_rope_kernel<DT, 8, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 16: return launch(qk_norm_rope_kernel<DT, 16, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    default: return launch(qk_norm_rope_kernel<DT, 32, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 1: return launch(qk_norm_rope_kernel<DT, 1, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 2: return launch(qk_norm_rope_kernel<DT, 2, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 4: return launch(qk_norm_rope_kernel<DT, 4, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 8: return launch(qk_norm_rope_kernel<DT, 8, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 16: return launch(qk_norm_rope_kernel<DT, 16, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
+    default: return launch(qk_norm_rope_kernel<DT, 32, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
   }
 }
 
@@ -216,6 +214,7 @@ extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, 
   a.dim = head_dim;
   a.rot = rot_dim;
   a.eps = eps;
+  a.inv_dim = 1.0f / static_cast<float>(head_dim);
   a.interleaved = interleaved ? 1 : 0;
   a.w_vec = (!heads || aligned16(q_weight)) && (!kv_heads || aligned16(k_weight)) ? 1 : 0;
   // every row of angles, and its second half, starts on 16 bytes
@@ -233,11 +232,14 @@ extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, 
   a.groups = static_cast<uint32_t>(groups);
   a.per_token = FastDiv(static_cast<uint32_t>(a.parts));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool full = rot_dim == head_dim;
   cudaError_t err;
   if (act_dtype == I8L_BF16)
-    err = four ? launch_qk<I8L_BF16, 4>(a, lanes, s) : launch_qk<I8L_BF16, 1>(a, lanes, s);
+    err = four ? (full ? launch_qk<I8L_BF16, 4, true>(a, lanes, s) : launch_qk<I8L_BF16, 4, false>(a, lanes, s))
+               : launch_qk<I8L_BF16, 1, false>(a, lanes, s);
   else
-    err = four ? launch_qk<I8L_F16, 4>(a, lanes, s) : launch_qk<I8L_F16, 1>(a, lanes, s);
+    err = four ? (full ? launch_qk<I8L_F16, 4, true>(a, lanes, s) : launch_qk<I8L_F16, 4, false>(a, lanes, s))
+               : launch_qk<I8L_F16, 1, false>(a, lanes, s);
   if (err != cudaSuccess) return cuda_error(err, "qk_norm_rope launch");
   err = cudaGetLastError();
   return err == cudaSuccess ? I8L_OK : cuda_error(err, "qk_norm_rope launch");
