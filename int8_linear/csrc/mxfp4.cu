@@ -105,41 +105,45 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-// One value for which the float32 arithmetic of silu_mul2 does not settle the rounding.
+// Two values of y = round_DT(float32(silu(g) * u)), packed, the float32 rounding being that
+// of the exact product: here in float64.
 template <int DT>
-__device__ __noinline__ uint32_t silu_mul_settle(float g, float u) {
-  const float y = g == 0.f || u == 0.f ? g * u : silu_mul_exact(g, u);
-  return pack2<DT>(y, 0.f) & 0xffffu;
+__device__ __noinline__ uint32_t silu_mul2_exact(uint32_t gw, uint32_t uw) {
+  float g[2], u[2];
+  unpack2<DT>(gw, g[0], g[1]);
+  unpack2<DT>(uw, u[0], u[1]);
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) g[i] = g[i] == 0.f || u[i] == 0.f ? g[i] * u[i] : silu_mul_exact(g[i], u[i]);
+  return pack2<DT>(g[0], g[1]);
 }
 
-// Two values of y = round_DT(float32(silu(g) * u)), packed, the float32 rounding being that
-// of the exact product.
+// The same in float32, with `unsure` set where that does not settle the rounding.
 //
-// v = g * rcp(1 + 2^(-g log2 e)) * u in float32.  In units of 2^-23 relative: the exponent's
-// product and its constant are off by 0.63 |g| at most, ex2.approx by 2, both damped by
-// e/(1 + e) with e = exp(-g), which is below 1 for g < 0 and below 1/2 (times |g|: below 0.3)
-// for g > 0; the sum and the two products add 1/2 each and rcp.approx 1.  So v is within
-// 5 + 0.7 max(-g, 0) of those units, with some margin, and y is right wherever both ends of
-// that interval round alike.  Elsewhere (about one value in 2000 for bf16) it is computed
-// again in float64, and so are values near the end of float32's normal range, which has no
-// such relative bound.
+// v = g * rcp(1 + 2^(-g log2 e)) * u.  In units of 2^-23 relative: the exponent's product and
+// its constant are off by 0.63 |g| at most, ex2.approx by 2, both damped by e/(1 + e) with
+// e = exp(-g), which is below 1 for g < 0 and below 1/2 (times |g|: below 0.3) for g > 0; the
+// sum and the two products add 1/2 each and rcp.approx 1.  So v is within 5 + 0.7 max(-g, 0)
+// of those units, with some margin, and y is right wherever both ends of that interval round
+// alike; about one bf16 value in 5000 is unsure.  Values near the end of float32's normal
+// range have no such relative bound and are unsure for bf16; for fp16 they are zero.
 template <int DT>
-__device__ __forceinline__ uint32_t silu_mul2(uint32_t gw, uint32_t uw) {
+__device__ __forceinline__ uint32_t silu_mul2(uint32_t gw, uint32_t uw, bool &unsure) {
   constexpr float kUnit = 1.0f / 8388608.0f, kTiny = 1e-36f;
-  float g0, g1, u0, u1, p0, p1, d0, d1, v0, v1;
+  float g0, g1, u0, u1, p0, p1, d0, d1, v0, v1, e0, e1, l0, l1, h0, h1;
   unpack2<DT>(gw, g0, g1);
   unpack2<DT>(uw, u0, u1);
   mul2_rn(p0, p1, g0, g1, -1.4426950408889634f, -1.4426950408889634f);
   add2_rn(d0, d1, 1.0f, 1.0f, ex2_approx(p0), ex2_approx(p1));
   mul2_rn(v0, v1, g0, g1, rcp_approx(d0), rcp_approx(d1));
   mul2_rn(v0, v1, v0, v1, u0, u1);
-  const float e0 = fmaf(fmaxf(-g0, 0.f), 0.7f * kUnit, 5.0f * kUnit), e1 = fmaf(fmaxf(-g1, 0.f), 0.7f * kUnit, 5.0f * kUnit);
-  uint32_t low = pack2<DT>(fmaf(v0, -e0, v0), fmaf(v1, -e1, v1));
-  const uint32_t high = pack2<DT>(fmaf(v0, e0, v0), fmaf(v1, e1, v1));
-  if (low != high || fminf(fabsf(v0), fabsf(v1)) < kTiny) {
-    if (((low ^ high) & 0xffffu) || fabsf(v0) < kTiny) low = (low & 0xffff0000u) | silu_mul_settle<DT>(g0, u0);
-    if (((low ^ high) >> 16) || fabsf(v1) < kTiny) low = (low & 0xffffu) | (silu_mul_settle<DT>(g1, u1) << 16);
-  }
+  g0 = fminf(g0, 0.f);
+  g1 = fminf(g1, 0.f);
+  fma2_rn(e0, e1, g0, g1, 0.7f * kUnit, 0.7f * kUnit, -5.0f * kUnit, -5.0f * kUnit);  // minus the bound
+  fma2_rn(l0, l1, v0, v1, e0, e1, v0, v1);
+  fma2_rn(h0, h1, v0, v1, -e0, -e1, v0, v1);
+  const uint32_t low = pack2<DT>(l0, l1), high = pack2<DT>(h0, h1);
+  unsure = low != high;
+  if constexpr (DT == I8L_BF16) unsure = unsure || fminf(fabsf(v0), fabsf(v1)) < kTiny;
   return low;
 }
 
@@ -207,6 +211,28 @@ __device__ __forceinline__ uint32_t mx_amax32(const uint32_t (&w)[16]) {
   return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
 }
 
+// Quantises a block that one thread holds and stores its codes and its scale.
+template <int DT>
+__device__ __forceinline__ void store_block(const MxOut &o, int q16, long long row, int block, int blocks,
+                                            const uint32_t (&x)[16]) {
+  const uint32_t byte = mx_scale_byte(mx_amax32<DT>(x));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float y[8];
+    unpack8<DT>(make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]), y);
+    w[i] = byte == 255u ? 0u : mx_pack8(y, mx_inv_scale(byte));
+  }
+  uint8_t *q = o.q + row * o.ldq + block * 16;
+  if (q16) {
+    *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t *>(q)[i] = w[i];
+  }
+  store_sf(o, row, block, blocks, byte);
+}
+
 // Four lanes a block, one vector of eight values a thread.  kSilu: x holds [gate | up] rows
 // of 2K values.
 template <int DT, bool kSilu>
@@ -228,10 +254,15 @@ __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a
     if constexpr (kSilu) {
       const long long K = static_cast<long long>(a.blocks) * kMxBlock;
       const uint4 up = in ? load8_raw(a.x, at + K, a.vec) : make_uint4(0u, 0u, 0u, 0u);
-      x.x = silu_mul2<DT>(x.x, up.x);
-      x.y = silu_mul2<DT>(x.y, up.y);
-      x.z = silu_mul2<DT>(x.z, up.z);
-      x.w = silu_mul2<DT>(x.w, up.w);
+      auto settle = [](uint32_t &g, uint32_t u) {
+        bool unsure;
+        const uint32_t y = silu_mul2<DT>(g, u, unsure);
+        g = unsure ? silu_mul2_exact<DT>(g, u) : y;
+      };
+      settle(x.x, up.x);
+      settle(x.y, up.y);
+      settle(x.z, up.z);
+      settle(x.w, up.w);
     }
     w = mx_quantise8<DT>(x, byte);
   }
@@ -266,25 +297,27 @@ __global__ void __launch_bounds__(kFlatThreads) mx_block_kernel(const FlatArgs a
   if constexpr (kSilu) {
     uint32_t up[16];
     load_block(a.x, at + static_cast<long long>(a.blocks) * kMxBlock, a.vec, up);
+    // The unsure pairs are few: they are read again and done after all others, which keeps
+    // the slow code out of the unrolled loop.
+    uint32_t todo = 0u;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = silu_mul2<DT>(x[i], up[i]);
-  }
-  const uint32_t byte = mx_scale_byte(mx_amax32<DT>(x));
-  uint32_t w[4];
+    for (int i = 0; i < 16; ++i) {
+      bool unsure;
+      x[i] = silu_mul2<DT>(x[i], up[i], unsure);
+      if (unsure) todo |= 1u << i;
+    }
+    while (todo) {
+      const int i = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const uint16_t *g = static_cast<const uint16_t *>(a.x) + at + 2 * i;
+      const uint16_t *u = g + static_cast<long long>(a.blocks) * kMxBlock;
+      const uint32_t y = silu_mul2_exact<DT>(g[0] | (static_cast<uint32_t>(g[1]) << 16),
+                                             u[0] | (static_cast<uint32_t>(u[1]) << 16));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float y[8];
-    unpack8<DT>(make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]), y);
-    w[i] = byte == 255u ? 0u : mx_pack8(y, mx_inv_scale(byte));
+      for (int j = 0; j < 16; ++j) x[j] = j == i ? y : x[j];
+    }
   }
-  uint8_t *q = a.o.q + row * a.o.ldq + block * 16u;
-  if (a.q16) {
-    *reinterpret_cast<uint4 *>(q) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t *>(q)[i] = w[i];
-  }
-  store_sf(a.o, row, static_cast<int>(block), a.blocks, byte);
+  store_block<DT>(a.o, a.q16, row, static_cast<int>(block), a.blocks, x);
 }
 
 // ------------------------------------------------------------------ add + RMSNorm
@@ -302,7 +335,8 @@ struct MxNormArgs {
   int rows, K;
   double eps;
   uint32_t pad_words;
-  int vec;  // 16-byte loads and stores allowed
+  int vec;  // 1: 16-byte loads and stores allowed, 2: 32-byte ones
+  int q16;  // 16-byte stores of codes allowed
 };
 
 // One row per CTA, the row in registers.  The squares are summed in float64 (a float32
@@ -392,6 +426,89 @@ __global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) 
       if ((threadIdx.x & 3) == 0) store_sf(a.o, row, col / kMxBlock, a.K / kMxBlock, byte);
     }
   }
+}
+
+// The same for batches of many rows of up to 8192 values, with a whole block per thread: the
+// reductions, the scale and the addresses are shared by 32 values.
+template <int DT, int WDT>
+__global__ void __launch_bounds__(256) mx_norm_block_kernel(const MxNormArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  using T = typename ActType<DT>::T;
+  const long long row = blockIdx.x;
+  if (row >= a.rows) {  // zero words of the scale tiles below the last row
+    const long long i = (row - a.rows) * blockDim.x + threadIdx.x;
+    if (i < a.pad_words) zero_pad_word(a.o, a.rows, i);
+    return;
+  }
+  __shared__ double red[8];
+  __shared__ float factor;
+  const int blocks = a.K / kMxBlock, block = static_cast<int>(threadIdx.x);
+  const bool in = block < blocks;
+  uint32_t x[16], r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = r[i] = 0u;
+  if (in) {
+    load_block(a.x, row * a.ldx + block * kMxBlock, a.vec, x);
+    if (a.res) load_block(a.res, row * a.ldr + block * kMxBlock, a.vec, r);
+  }
+  float h[32];
+  double ss = 0.0, ss1 = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    unpack2<DT>(x[i], h[2 * i], h[2 * i + 1]);
+    if (a.res) {
+      float r0, r1;
+      unpack2<DT>(r[i], r0, r1);
+      add2_rn(h[2 * i], h[2 * i + 1], h[2 * i], h[2 * i + 1], r0, r1);
+      r[i] = pack2<DT>(h[2 * i], h[2 * i + 1]);
+    }
+    const double d0 = h[2 * i], d1 = h[2 * i + 1];
+    ss = fma(d0, d0, ss);
+    ss1 = fma(d1, d1, ss1);
+  }
+  if (in && a.res) {
+    T *p = static_cast<T *>(a.rout) + row * a.ldro + block * kMxBlock;
+    if (a.vec == 2) {
+      st_v8(p, r);
+      st_v8(p + 16, r + 8);
+    } else if (a.vec) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<uint4 *>(p)[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) p[i] = ActType<DT>::from_f32(h[i]);
+    }
+  }
+  ss += ss1;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    ss = threadIdx.x < blockDim.x >> 5 ? red[threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (threadIdx.x == 0) factor = static_cast<float>(1.0 / sqrt(ss / a.K + a.eps));
+  }
+  __syncthreads();
+  if (!in) return;
+  const float rs = factor;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    float w[8];
+    load_weight_vec<8>(a.w, WDT, block * kMxBlock + 8 * v, a.w_vec != 0, w);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      float n0, n1;
+      mul2_rn(n0, n1, h[8 * v + i], h[8 * v + i + 1], rs, rs);
+      round2_through<WDT>(n0, n1);
+      mul2_rn(n0, n1, n0, n1, w[i], w[i + 1]);
+      x[4 * v + i / 2] = pack2<DT>(n0, n1);
+    }
+  }
+  store_block<DT>(a.o, a.q16, row, block, blocks, x);
 }
 
 // ------------------------------------------------------------------ dequantisation
@@ -608,12 +725,26 @@ extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const voi
   a.eps = eps;
   a.pad_words = static_cast<uint32_t>((128 - M % 128) % 128) * ktiles;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int nv = rs.nv, th = rs.threads;
+  a.vec = vec ? 1 : 0;
+  a.q16 = aligned16(q) && ldq % 16 == 0 ? 1 : 0;
+  DeviceInfo di;
+  if (int e = device_info(&di)) return e;
+  // A block per thread from 4 rows an SM on; fewer rows finish sooner spread over four times
+  // the threads (MEASURE).
+  const bool blocks = M >= 4 * di.sms && K <= 8192;
+  if (blocks && vec) {
+    auto wide = [](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 32 == 0 && ld % 16 == 0; };
+    if (wide(x, ldx) && (!residual || (wide(residual, ldr) && wide(rout, ldro)))) a.vec = 2;
+  }
+  const int nv = rs.nv, th = blocks ? (K / kMxBlock + 31) / 32 * 32 : rs.threads;
   const dim3 grid(static_cast<unsigned>(M) + (a.pad_words + th - 1) / th);
   cudaError_t err = cudaSuccess;
-  a.vec = vec ? 1 : 0;
-#define I8L_MX_NORM(ADT, WDTV) \
-  I8L_DISPATCH_NV(nv, (err = launch(mx_norm_quant_kernel<ADT, WDTV, NV>, grid, dim3(th), 0, s, 1, a)))
+#define I8L_MX_NORM(ADT, WDTV)                                                                          \
+  if (blocks) {                                                                                         \
+    err = launch(mx_norm_block_kernel<ADT, WDTV>, grid, dim3(th), 0, s, 1, a);                          \
+  } else {                                                                                              \
+    I8L_DISPATCH_NV(nv, (err = launch(mx_norm_quant_kernel<ADT, WDTV, NV>, grid, dim3(th), 0, s, 1, a))) \
+  }
 #define I8L_MX_NORM_W(ADT)                                              \
   if (w_dtype == I8L_BF16) { I8L_MX_NORM(ADT, I8L_BF16) }               \
   else if (w_dtype == I8L_F16) { I8L_MX_NORM(ADT, I8L_F16) }            \

@@ -193,6 +193,19 @@ __device__ __forceinline__ void mma_commit_elected(uint32_t elected, uint32_t ba
         : "memory");
 }
 
+// Two fused multiply-adds in one instruction, each rounded as fmaf rounds.
+__device__ __forceinline__ void fma2_rn(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0,
+                                        float c1) {
+  asm("{\n.reg .b64 ra, rb, rc, rd;\n"
+      "mov.b64 ra, {%2, %3};\n"
+      "mov.b64 rb, {%4, %5};\n"
+      "mov.b64 rc, {%6, %7};\n"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n"
+      "mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+
 // Eight values times `inv`, rounded to e2m1 (nearest, ties to even, saturating), packed
 // with the first value in the lowest nibble.
 __device__ __forceinline__ uint32_t mx_pack8(const float (&y)[8], float inv) {

@@ -118,20 +118,34 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a
     unpack2<DT>(raw[turn].y, x[2], x[3]);
     unpack2<DT>(raw[turn].z, x[4], x[5]);
     unpack2<DT>(raw[turn].w, x[6], x[7]);
-    float ss = 0.f;
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+    for (int i = 0; i < 8; i += 2) fma2_rn(s0, s1, x[i], x[i + 1], x[i], x[i + 1], s0, s1);
+    float ss = s0 + s1;
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
     float rs = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
     if (!known) rs = __int_as_float(0x7fc00000);
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * rs * w[i];
+    for (int i = 0; i < 8; i += 2) {
+      mul2_rn(x[i], x[i + 1], x[i], x[i + 1], rs, rs);
+      mul2_rn(x[i], x[i + 1], x[i], x[i + 1], w[i], w[i + 1]);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = a.interleaved ? x[i ^ 1] : __shfl_sync(0xffffffffu, x[i], partner, G);
-      y[i] = kFull || turns ? fmaf(x[i], cs[i], other * sn[i]) : x[i];
+    for (int i = 0; i < 8; i += 2) {
+      float o0, o1, t0, t1;
+      if (a.interleaved) {
+        o0 = x[i + 1];
+        o1 = x[i];
+      } else {
+        o0 = __shfl_sync(0xffffffffu, x[i], partner, G);
+        o1 = __shfl_sync(0xffffffffu, x[i + 1], partner, G);
+      }
+      mul2_rn(t0, t1, o0, o1, sn[i], sn[i + 1]);
+      fma2_rn(t0, t1, x[i], x[i + 1], cs[i], cs[i + 1], t0, t1);
+      y[i] = kFull || turns ? t0 : x[i];
+      y[i + 1] = kFull || turns ? t1 : x[i + 1];
     }
     if (here) {
       T *dst = key ? static_cast<T *>(a.k) + token * a.ldk + static_cast<long long>(head - a.heads) * a.dim
