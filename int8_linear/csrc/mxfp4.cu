@@ -21,7 +21,7 @@
 
 namespace i8l {
 
-constexpr int kFlatThreads = 256;
+constexpr int kFlatThreads = 128;
 constexpr int64_t kBlockThreadsMin = 148 * 256;  // blocks from which a thread takes a whole one
 
 struct MxOut {

@@ -7,11 +7,14 @@
 // where pair i is (n[i], n[i + rot/2]), or (n[2i], n[2i + 1]) when interleaved.  Everything
 // is float32 between the load and one rounding at the store.
 //
-// A group of lanes, eight values each, holds one head in registers: the sum of squares is
-// a butterfly over the group, and the other half of a pair comes from another lane of the
-// group by a shuffle.  A group takes up to P neighbouring heads of one token: their loads are
-// all in flight together, and the token's angles are read once for them.  The kernel reads
-// and writes each value once and is bound by HBM.
+// A group of lanes holds one head in registers, each lane two chunks of eight values that
+// are rotated with one another: values 8c.. and rot/2 + 8c.. (or, interleaved, two chunks in
+// a row), so that a lane needs eight angles and nothing from another lane but the sum of
+// squares, a butterfly over the group.  (With neighbouring values in a lane and the pairs'
+// other halves shuffled, the kernel took 42 us where this takes 36, 8192 tokens x 40 heads
+// of 128.)  A group takes up to P neighbouring heads of one token: their loads are all in
+// flight together, and the token's angles are read once for them.  The kernel reads and
+// writes each value once.
 #include <algorithm>
 
 #include "common.cuh"
@@ -21,7 +24,8 @@
 
 namespace i8l {
 
-constexpr int kQkThreads = 256;
+constexpr int kQkThreads = 128;
+constexpr int kQkHeads = 4;  // heads per group in a large batch
 
 struct QkArgs {
   const void *qkv;
@@ -46,10 +50,9 @@ struct QkArgs {
   int w_vec, cs_vec;
 };
 
-// G lanes per head (a power of two, G * 8 >= dim), P heads per group; kFull: every value is
-// rotated (rot == dim).  In place is fine: a lane stores the
-// elements that it alone loaded, after every exchange within its head.
-template <int DT, int G, int P, bool kFull>
+// G lanes per head (a power of two, G * 16 >= dim), P heads per group.  In place is fine: a
+// lane stores the elements that it alone loaded.
+template <int DT, int G, int P>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -59,99 +62,107 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a
   const bool live = group < a.groups;
   const long long token = live ? a.per_token.div(group) : 0;
   const int part = live ? static_cast<int>(group - static_cast<uint32_t>(token) * a.parts) : 0;
-  const int c0 = lane * 8;
-  const bool mine = live && c0 < a.dim;
-  const int all = a.heads + a.kv_heads, head0 = part * P;
-  const T *src = static_cast<const T *>(a.qkv) + token * a.ld + static_cast<long long>(head0) * a.dim + c0;
-  uint4 raw[P];
-#pragma unroll
-  for (int i = 0; i < P; ++i)
-    raw[i] = mine && head0 + i < all ? *reinterpret_cast<const uint4 *>(src + i * a.dim) : make_uint4(0u, 0u, 0u, 0u);
   const int half = a.rot / 2;
+  // The lane's chunks begin at c0 and c1; what lies behind the rotated values follows in order.
+  const bool split = !a.interleaved && lane < a.rot / 16;
+  const int c0 = split ? 8 * lane : 16 * lane, c1 = split ? half + 8 * lane : 16 * lane + 8;
+  const bool has0 = live && c0 < a.dim, has1 = live && c1 < a.dim;
+  const int all = a.heads + a.kv_heads, head0 = part * P;
+  const T *src = static_cast<const T *>(a.qkv) + token * a.ld + static_cast<long long>(head0) * a.dim;
+  uint4 raw[P][2];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const bool in = head0 + i < all;
+    raw[i][0] = in && has0 ? *reinterpret_cast<const uint4 *>(src + i * a.dim + c0) : make_uint4(0u, 0u, 0u, 0u);
+    raw[i][1] = in && has1 ? *reinterpret_cast<const uint4 *>(src + i * a.dim + c1) : make_uint4(0u, 0u, 0u, 0u);
+  }
 
   long long pos = 0;
   if (live)
     pos = a.pos64 ? static_cast<const long long *>(a.positions)[token] : static_cast<const int *>(a.positions)[token];
   // A position outside the table has no angles: the token's heads come out as NaN.
   const bool known = a.rot == 0 || (pos >= 0 && pos < a.max_pos);
-  const bool turns = mine && c0 < a.rot;
+  // Angles 8 lane .. 8 lane + 7; those past the last are none.
   float cs[8], sn[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     cs[i] = 1.f;
     sn[i] = 0.f;
   }
-  if (turns && known) {
-    const uint8_t *table = static_cast<const uint8_t *>(a.cos_sin) +
-                           pos * a.rot * (a.cs_dtype == I8L_F32 ? 4 : 2);
-    if (a.interleaved) {
-      // pairs (2i, 2i + 1): both take angle i
+  if (has0 && known && 8 * lane < half) {
+    const uint8_t *table = static_cast<const uint8_t *>(a.cos_sin) + pos * a.rot * (a.cs_dtype == I8L_F32 ? 4 : 2);
+    if (8 * lane + 8 <= half) {
+      load_weight_vec<8>(table, a.cs_dtype, 8 * lane, a.cs_vec != 0, cs);
+      load_weight_vec<8>(table, a.cs_dtype, half + 8 * lane, a.cs_vec != 0, sn);
+    } else {  // interleaved, and four angles left
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        cs[i] = load_weight(table, a.cs_dtype, (c0 + i) / 2);
-        sn[i] = load_weight(table, a.cs_dtype, half + (c0 + i) / 2);
+      for (int i = 0; i < 4; ++i) {
+        cs[i] = load_weight(table, a.cs_dtype, 8 * lane + i);
+        sn[i] = load_weight(table, a.cs_dtype, half + 8 * lane + i);
       }
-    } else {
-      const int j = c0 < half ? c0 : c0 - half;
-      load_weight_vec<8>(table, a.cs_dtype, j, a.cs_vec != 0, cs);
-      load_weight_vec<8>(table, a.cs_dtype, half + j, a.cs_vec != 0, sn);
     }
-    // the first value of a pair subtracts its partner's share
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (a.interleaved ? i % 2 == 0 : c0 < half) sn[i] = -sn[i];
   }
-  // The lane of this group that holds the other values of this lane's pairs.
-  const int partner = !a.interleaved && turns ? (c0 < half ? lane + half / 8 : lane - half / 8) : lane;
 
-  float w[8] = {};
+  float w[16] = {};
   int loaded = -1;  // which weight `w` holds: 0 queries, 1 keys
 #pragma unroll
   for (int turn = 0; turn < P; ++turn) {
     const int head = head0 + turn;
-    const bool here = mine && head < all;
+    const bool here = live && head < all;
     const int key = head >= a.heads ? 1 : 0;
-    if (here && key != loaded) load_weight_vec<8>(key ? a.wk : a.wq, a.w_dtype, c0, a.w_vec != 0, w);
+    if (here && key != loaded) {
+      const void *weight = key ? a.wk : a.wq;
+      if (has0) load_weight_vec<8>(weight, a.w_dtype, c0, a.w_vec != 0, *reinterpret_cast<float(*)[8]>(w));
+      if (has1) load_weight_vec<8>(weight, a.w_dtype, c1, a.w_vec != 0, *reinterpret_cast<float(*)[8]>(w + 8));
+    }
     loaded = key;
-    float x[8];
-    unpack2<DT>(raw[turn].x, x[0], x[1]);
-    unpack2<DT>(raw[turn].y, x[2], x[3]);
-    unpack2<DT>(raw[turn].z, x[4], x[5]);
-    unpack2<DT>(raw[turn].w, x[6], x[7]);
+    float x[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      unpack2<DT>(raw[turn][h].x, x[8 * h], x[8 * h + 1]);
+      unpack2<DT>(raw[turn][h].y, x[8 * h + 2], x[8 * h + 3]);
+      unpack2<DT>(raw[turn][h].z, x[8 * h + 4], x[8 * h + 5]);
+      unpack2<DT>(raw[turn][h].w, x[8 * h + 6], x[8 * h + 7]);
+    }
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) fma2_rn(s0, s1, x[i], x[i + 1], x[i], x[i + 1], s0, s1);
+    for (int i = 0; i < 16; i += 2) fma2_rn(s0, s1, x[i], x[i + 1], x[i], x[i + 1], s0, s1);
     float ss = s0 + s1;
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
     float rs = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
     if (!known) rs = __int_as_float(0x7fc00000);
-    float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
+    for (int i = 0; i < 16; i += 2) {
       mul2_rn(x[i], x[i + 1], x[i], x[i + 1], rs, rs);
       mul2_rn(x[i], x[i + 1], x[i], x[i + 1], w[i], w[i + 1]);
     }
+    if (a.interleaved) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      float o0, o1, t0, t1;
-      if (a.interleaved) {
-        o0 = x[i + 1];
-        o1 = x[i];
-      } else {
-        o0 = __shfl_sync(0xffffffffu, x[i], partner, G);
-        o1 = __shfl_sync(0xffffffffu, x[i + 1], partner, G);
+      for (int i = 0; i < 8; ++i) {
+        const float u = x[2 * i], v = x[2 * i + 1];
+        x[2 * i] = fmaf(u, cs[i], -(v * sn[i]));
+        x[2 * i + 1] = fmaf(v, cs[i], u * sn[i]);
       }
-      mul2_rn(t0, t1, o0, o1, sn[i], sn[i + 1]);
-      fma2_rn(t0, t1, x[i], x[i + 1], cs[i], cs[i + 1], t0, t1);
-      y[i] = kFull || turns ? t0 : x[i];
-      y[i + 1] = kFull || turns ? t1 : x[i + 1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        float t0, t1, r0, r1;
+        mul2_rn(t0, t1, x[8 + i], x[9 + i], -sn[i], -sn[i + 1]);
+        mul2_rn(r0, r1, x[i], x[i + 1], sn[i], sn[i + 1]);
+        fma2_rn(x[i], x[i + 1], x[i], x[i + 1], cs[i], cs[i + 1], t0, t1);
+        fma2_rn(x[8 + i], x[9 + i], x[8 + i], x[9 + i], cs[i], cs[i + 1], r0, r1);
+      }
     }
     if (here) {
       T *dst = key ? static_cast<T *>(a.k) + token * a.ldk + static_cast<long long>(head - a.heads) * a.dim
                    : static_cast<T *>(a.q) + token * a.ldq + static_cast<long long>(head) * a.dim;
-      *reinterpret_cast<uint4 *>(dst + c0) =
-          make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
+      if (has0)
+        *reinterpret_cast<uint4 *>(dst + c0) = make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]),
+                                                          pack2<DT>(x[4], x[5]), pack2<DT>(x[6], x[7]));
+      if (has1)
+        *reinterpret_cast<uint4 *>(dst + c1) = make_uint4(pack2<DT>(x[8], x[9]), pack2<DT>(x[10], x[11]),
+                                                          pack2<DT>(x[12], x[13]), pack2<DT>(x[14], x[15]));
     }
   }
 }
@@ -162,17 +173,16 @@ using namespace i8l;
 
 namespace {
 
-template <int DT, int P, bool kFull>
+template <int DT, int P>
 cudaError_t launch_qk(const QkArgs &a, int lanes, cudaStream_t s) {
   const unsigned per_block = kQkThreads / lanes;
   const dim3 grid((a.groups + per_block - 1) / per_block);
   switch (lanes) {
-    case 1: return launch(qk_norm_rope_kernel<DT, 1, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 2: return launch(qk_norm_rope_kernel<DT, 2, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 4: return launch(qk_norm_rope_kernel<DT, 4, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 8: return launch(qk_norm_rope_kernel<DT, 8, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 16: return launch(qk_norm_rope_kernel<DT, 16, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
-    default: return launch(qk_norm_rope_kernel<DT, 32, P, kFull>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 1: return launch(qk_norm_rope_kernel<DT, 1, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 2: return launch(qk_norm_rope_kernel<DT, 2, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 4: return launch(qk_norm_rope_kernel<DT, 4, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 8: return launch(qk_norm_rope_kernel<DT, 8, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    default: return launch(qk_norm_rope_kernel<DT, 16, P>, grid, dim3(kQkThreads), 0, s, 1, a);
   }
 }
 
@@ -234,26 +244,23 @@ extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, 
   // every row of angles, and its second half, starts on 16 bytes
   a.cs_vec = aligned16(cos_sin) && (rot_dim / 2 * (cs_dtype == I8L_F32 ? 4 : 2)) % 16 == 0 ? 1 : 0;
   int lanes = 1;
-  while (lanes * 8 < head_dim) lanes *= 2;
-  // One head per group until the groups fill the SMs twice over, then four.
+  while (lanes * 16 < head_dim) lanes *= 2;
+  // One head per group until the groups fill the SMs twice over, then kQkHeads.
   DeviceInfo di;
   if (int e = device_info(&di)) return e;
-  const bool four = static_cast<int64_t>(tokens) * all > 2LL * di.sms * (2048 / lanes);
-  a.parts = static_cast<int>(four ? (all + 3) / 4 : all);
+  const bool many = static_cast<int64_t>(tokens) * all > 2LL * di.sms * (2048 / lanes);
+  a.parts = static_cast<int>(many ? (all + kQkHeads - 1) / kQkHeads : all);
   const int64_t groups = static_cast<int64_t>(tokens) * a.parts;
   if (groups > INT32_MAX - kQkThreads)
     return set_error(I8L_ENOTSUP, "%d tokens x %lld heads is too large", tokens, static_cast<long long>(all));
   a.groups = static_cast<uint32_t>(groups);
   a.per_token = FastDiv(static_cast<uint32_t>(a.parts));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool full = rot_dim == head_dim;
   cudaError_t err;
   if (act_dtype == I8L_BF16)
-    err = four ? (full ? launch_qk<I8L_BF16, 4, true>(a, lanes, s) : launch_qk<I8L_BF16, 4, false>(a, lanes, s))
-               : launch_qk<I8L_BF16, 1, false>(a, lanes, s);
+    err = many ? launch_qk<I8L_BF16, kQkHeads>(a, lanes, s) : launch_qk<I8L_BF16, 1>(a, lanes, s);
   else
-    err = four ? (full ? launch_qk<I8L_F16, 4, true>(a, lanes, s) : launch_qk<I8L_F16, 4, false>(a, lanes, s))
-               : launch_qk<I8L_F16, 1, false>(a, lanes, s);
+    err = many ? launch_qk<I8L_F16, kQkHeads>(a, lanes, s) : launch_qk<I8L_F16, 1>(a, lanes, s);
   if (err != cudaSuccess) return cuda_error(err, "qk_norm_rope launch");
   err = cudaGetLastError();
   return err == cudaSuccess ? I8L_OK : cuda_error(err, "qk_norm_rope launch");
