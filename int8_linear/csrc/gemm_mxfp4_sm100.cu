@@ -55,6 +55,7 @@ struct MxGemmArgs {
 // ------------------------------------------------------------------ split tiles
 
 constexpr int kSplitThreads = 128;
+constexpr int kMaxCluster = 8;
 
 template <int TN>
 struct SplitLayout {
@@ -151,6 +152,13 @@ __global__ void __launch_bounds__(kSplitThreads)
   const int tx = tile % a.tiles_n, ty = tile / a.tiles_n;
   const int kb0 = a.kblocks * rank / a.cluster, kb1 = a.kblocks * (rank + 1) / a.cluster;
 
+  const uint64_t pol_w = policy_evict_first(), pol_a = policy_evict_last();
+  auto load_w = [&](int st, int kb) {
+    mbar_arrive_expect_tx(&full[st], L::kStageBytes);
+    tma_load_2d(sx + st * L::kXBytes, &map_x, &full[st], kb * kMxRowBytes, tx * kMxRows, pol_w);
+    tma_load_2d(ssx + st * kSfStageBytes, &map_sfx, &full[st], kb * 2 * kSfWords, tx, pol_w);
+  };
+  const int pre = min(S, kb1 - kb0);
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);
@@ -160,10 +168,10 @@ __global__ void __launch_bounds__(kSplitThreads)
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    tma_prefetch_desc(&map_x);
-    tma_prefetch_desc(&map_sfx);
-    tma_prefetch_desc(&map_y);
-    tma_prefetch_desc(&map_sfy);
+    fence_proxy_async_smem();
+    // The weight tiles of the first stages wait neither for the other warps nor for the
+    // previous kernel.
+    for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, L::kTmemCols);
@@ -176,15 +184,6 @@ __global__ void __launch_bounds__(kSplitThreads)
   pdl_launch_dependents();
 
   if (warp == 0 && lane == 0) {
-    // Weight tiles of the first stages do not wait for the previous kernel.
-    const uint64_t pol_w = policy_evict_first(), pol_a = policy_evict_last();
-    auto load_w = [&](int st, int kb) {
-      mbar_arrive_expect_tx(&full[st], L::kStageBytes);
-      tma_load_2d(sx + st * L::kXBytes, &map_x, &full[st], kb * kMxRowBytes, tx * kMxRows, pol_w);
-      tma_load_2d(ssx + st * kSfStageBytes, &map_sfx, &full[st], kb * 2 * kSfWords, tx, pol_w);
-    };
-    const int pre = min(S, kb1 - kb0);
-    for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
     pdl_wait();
     bool ok = true;
     int issued = 0, st = 0;
@@ -271,16 +270,21 @@ __global__ void __launch_bounds__(kSplitThreads)
       const int m = u / (kMxRows / 4), c = (u % (kMxRows / 4)) * 4;
       const int n0 = tx * kMxRows + c;
       if (n0 >= a.N) continue;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      // Every CTA's partial sums are on their way together and added in rank order.
       const uint32_t at = smem_u32(red + m * kMxRows + c);
-      for (int p = 0; p < a.cluster; ++p) {
-        const float4 f = a.cluster > 1 ? ld_cluster_v4(map_to_rank(at, static_cast<uint32_t>(p)))
-                                       : *reinterpret_cast<const float4 *>(red + m * kMxRows + c);
-        v[0] += f.x;
-        v[1] += f.y;
-        v[2] += f.z;
-        v[3] += f.w;
-      }
+      float4 f[kMaxCluster];
+#pragma unroll
+      for (int p = 0; p < kMaxCluster; ++p)
+        if (p < a.cluster) f[p] = ld_cluster_v4(a.cluster > 1 ? map_to_rank(at, static_cast<uint32_t>(p)) : at);
+      float v[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
+#pragma unroll
+      for (int p = 1; p < kMaxCluster; ++p)
+        if (p < a.cluster) {
+          v[0] += f[p].x;
+          v[1] += f[p].y;
+          v[2] += f[p].z;
+          v[3] += f[p].w;
+        }
       if (a.bias)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -689,6 +693,9 @@ static int launch_pair(const CUtensorMap &mx, const CUtensorMap &my, const CUten
   return e == cudaSuccess ? I8L_OK : cuda_error(e, "mxfp4 gemm launch");
 }
 
+// Shared memory of one of two CTAs on an SM (228 KB, 1 KB of it reserved per CTA).
+constexpr int kHalfSmem = 233472 / 2 - 1024;
+
 static int split_stage_bytes(int tn) { return kMxRows * kMxRowBytes + tn * kMxRowBytes + 2 * kSfStageBytes; }
 
 static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
@@ -718,11 +725,13 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   int c = 1;
   while (c < 8 && 2 * c * tiles <= di.sms && kblocks / (2 * c) >= 1) c *= 2;
   if (tile && tile->cluster) c = tile->cluster;
-  if (c < 1 || c > 8 || c > kblocks)
+  if (c < 1 || c > kMaxCluster || c > kblocks)
     return set_error(I8L_ENOTSUP, "cluster size %d outside [1, min(8, k-blocks=%d)]", c, kblocks);
   p->cluster = c;
   const int most = std::min(16, (di.max_smem_optin - 1024 - 256) / split_stage_bytes(p->tn));
-  int s = std::min((kblocks + c - 1) / c, p->tn <= 64 ? 5 : 6);
+  // More CTAs than SMs share an SM in twos.
+  const int two = (kHalfSmem - 1024 - 256) / split_stage_bytes(p->tn);
+  int s = std::min((kblocks + c - 1) / c, tiles * c > di.sms ? std::min(two, 5) : 6);
   if (tile && tile->stages) s = tile->stages;
   if (s < 1 || s > most) return set_error(I8L_ENOTSUP, "stages %d outside [1, %d] for this tile", s, most);
   p->stages = s;
