@@ -106,29 +106,6 @@ __device__ __forceinline__ void store_out4(const MxGemmArgs &a, int m, int n0, c
   }
 }
 
-// The MMAs of one stage: its scale tiles into TMEM, then up to four steps of 64 values.
-// Steps past K are left out, so a scale tile past the end is never used.
-template <int TN>
-__device__ __forceinline__ void split_stage_mmas(uint32_t elected, uint32_t d, uint32_t sf, uint32_t x, uint32_t y,
-                                                 uint32_t sfx, uint32_t sfy, int k_left, bool first) {
-  const int steps = min(4, (k_left + 63) / 64);
-  const uint64_t ad = sw128_kmajor_desc(x), bd = sw128_kmajor_desc(y);
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    if (2 * t < steps) {
-      sf_to_tmem<false>(elected, sf + 4 * t, sf_desc(sfx + t * kSfTileBytes));
-      sf_to_tmem<false>(elected, sf + 8 + 4 * t, sf_desc(sfy + t * kSfTileBytes));
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (k < steps)
-      mma_mxf4<false>(elected, d, ad + 2 * k, bd + 2 * k,
-                      k & 1 ? idesc_mxf4(kMxRows, TN, 2) : idesc_mxf4(kMxRows, TN, 0), sf + 4 * (k >> 1),
-                      sf + 8 + 4 * (k >> 1), first && k == 0 ? 0u : 1u);
-  }
-}
-
 template <int TN>
 __global__ void __launch_bounds__(kSplitThreads)
     mx_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
@@ -217,6 +194,8 @@ __global__ void __launch_bounds__(kSplitThreads)
     }
   } else if (warp == 1) {
     const uint32_t elected = elect_one();
+    const uint32_t x_lo = desc_lo(smem_u32(sx)), y_lo = desc_lo(smem_u32(sy)), sfx_lo = desc_lo(smem_u32(ssx)),
+                   sfy_lo = desc_lo(smem_u32(ssy));
     bool ok = true, any = false;
     int st = 0;
     uint32_t phase = 0;
@@ -224,9 +203,14 @@ __global__ void __launch_bounds__(kSplitThreads)
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[st], phase, abort_flag, a.status, kStatusMmaWait));
       if (!ok) break;
       tc_fence_after();
-      split_stage_mmas<TN>(elected, tmem, tmem + TN, smem_u32(sx + st * L::kXBytes), smem_u32(sy + st * L::kYBytes),
-                           smem_u32(ssx + st * kSfStageBytes), smem_u32(ssy + st * kSfStageBytes),
-                           a.K - kb * kMxStageK, !any);
+      const uint32_t al = x_lo + st * (L::kXBytes >> 4), bl = y_lo + st * (L::kYBytes >> 4),
+                     xl = sfx_lo + st * (kSfStageBytes >> 4), yl = sfy_lo + st * (kSfStageBytes >> 4);
+      const int left = a.K - kb * kMxStageK;  // steps of 64 values past K are left out
+      constexpr uint32_t kId0 = idesc_mxf4(kMxRows, TN, 0), kId2 = idesc_mxf4(kMxRows, TN, 2);
+      single_half_stage(elected, tmem, al, bl, xl, yl, tmem + TN, tmem + TN + 8, kId0, kId2, any ? 1u : 0u, left > 64);
+      if (left > 128)
+        single_half_stage(elected, tmem, al + 4, bl + 4, xl + (kSfTileBytes >> 4), yl + (kSfTileBytes >> 4),
+                          tmem + TN + 4, tmem + TN + 12, kId0, kId2, 1u, left > 192);
       any = true;
       mma_commit_elected<false>(elected, smem_u32(&empty[st]));
       if (++st == S) {
@@ -265,31 +249,49 @@ __global__ void __launch_bounds__(kSplitThreads)
   pdl_wait();  // this thread's outputs and bias follow the stream's order
   if (*abort_flag == 0) {
     const int units = live * (kMxRows / 4);  // four consecutive outputs each
-    const int u1 = units * (rank + 1) / a.cluster;
-    for (int u = units * rank / a.cluster + static_cast<int>(threadIdx.x); u < u1; u += kSplitThreads) {
-      const int m = u / (kMxRows / 4), c = (u % (kMxRows / 4)) * 4;
-      const int n0 = tx * kMxRows + c;
-      if (n0 >= a.N) continue;
-      // Every CTA's partial sums are on their way together and added in rank order.
-      const uint32_t at = smem_u32(red + m * kMxRows + c);
-      float4 f[kMaxCluster];
-#pragma unroll
-      for (int p = 0; p < kMaxCluster; ++p)
-        if (p < a.cluster) f[p] = ld_cluster_v4(a.cluster > 1 ? map_to_rank(at, static_cast<uint32_t>(p)) : at);
-      float v[4] = {f[0].x, f[0].y, f[0].z, f[0].w};
-#pragma unroll
-      for (int p = 1; p < kMaxCluster; ++p)
-        if (p < a.cluster) {
-          v[0] += f[p].x;
-          v[1] += f[p].y;
-          v[2] += f[p].z;
-          v[3] += f[p].w;
-        }
+    const int u0 = units * rank / a.cluster, u1 = units * (rank + 1) / a.cluster;
+    auto finish = [&](int u, float4 f) {
+      const int m = u / (kMxRows / 4), n0 = tx * kMxRows + (u % (kMxRows / 4)) * 4;
+      if (n0 >= a.N) return;
+      float v[4] = {f.x, f.y, f.z, f.w};
       if (a.bias)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (n0 + j < a.N) v[j] += load_scalar_f(a.bias, a.bias_dtype, n0 + j);
       store_out4(a, ty * TN + m, n0, v);
+    };
+    if (a.cluster == 1) {
+#pragma unroll 4
+      for (int u = u0 + static_cast<int>(threadIdx.x); u < u1; u += kSplitThreads)
+        finish(u, reinterpret_cast<const float4 *>(red)[u]);
+    } else {
+      // A read of another CTA's shared memory takes some 700 cycles: those of kAhead units
+      // and every CTA are on their way together, then added in rank order.
+      constexpr int kAhead = 2;
+      const uint32_t at = smem_u32(red);
+      for (int u = u0 + static_cast<int>(threadIdx.x); u < u1; u += kAhead * kSplitThreads) {
+        float4 f[kAhead][kMaxCluster];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+          for (int p = 0; p < kMaxCluster; ++p)
+            if (p < a.cluster && u + i * kSplitThreads < u1)
+              f[i][p] = ld_cluster_v4(map_to_rank(at + (u + i * kSplitThreads) * 16, static_cast<uint32_t>(p)));
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (u + i * kSplitThreads >= u1) break;
+          float4 sum = f[i][0];
+#pragma unroll
+          for (int p = 1; p < kMaxCluster; ++p)
+            if (p < a.cluster) {
+              sum.x += f[i][p].x;
+              sum.y += f[i][p].y;
+              sum.z += f[i][p].z;
+              sum.w += f[i][p].w;
+            }
+          finish(u + i * kSplitThreads, sum);
+        }
+      }
     }
   }
   // No CTA leaves while another may still read its partial sums.
@@ -722,8 +724,13 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   if (p->tn < 128 && M > p->tn)
     return set_error(I8L_ENOTSUP, "a %d-token tile holds the whole batch, %d tokens given", p->tn, M);
   const int tiles = ((N + kMxRows - 1) / kMxRows) * ((M + p->tn - 1) / p->tn);
+  // Double the CTAs of a tile while they have SMs of their own and two stages each, or, of a
+  // long K, half an SM and 14 stages each (us with c and 2c: 16 x 2048 x 2048 c = 4 5.1 and
+  // 5.4; 64 x 4096 x 14336 c = 4 11.6 and 12.0; 256 x 4096 x 14336 c = 2 18.5 and 17.0).
   int c = 1;
-  while (c < 8 && 2 * c * tiles <= di.sms && kblocks / (2 * c) >= 1) c *= 2;
+  while (c < kMaxCluster && ((2 * c * tiles <= di.sms && kblocks >= 4 * c) ||
+                             (2 * c * tiles <= 2 * di.sms && kblocks >= 28 * c)))
+    c *= 2;
   if (tile && tile->cluster) c = tile->cluster;
   if (c < 1 || c > kMaxCluster || c > kblocks)
     return set_error(I8L_ENOTSUP, "cluster size %d outside [1, min(8, k-blocks=%d)]", c, kblocks);

@@ -48,7 +48,7 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
 // and a shift (the round-up method: m = ceil(2^(32+s) / d), s = ceil(log2 d)).
 struct FastDiv {
   uint32_t d, m, s;
-  __host__ explicit FastDiv(uint32_t div = 1) : d(div), m(0), s(0) {
+  __host__ FastDiv(uint32_t div = 1) : d(div), m(0), s(0) {
     while ((1ull << s) < d) ++s;
     m = static_cast<uint32_t>(((1ull << 32) * ((1ull << s) - d)) / d + 1);
   }
@@ -80,30 +80,6 @@ __device__ __forceinline__ uint32_t elect_one() {
   return r;
 }
 
-// One 512-byte scale tile from shared memory into four TMEM columns, replicated to the
-// lanes of all four warps; in order with this thread's later tcgen05.mma.  kPair: in both
-// CTAs of a pair, each from its own shared memory.
-template <bool kPair>
-__device__ __forceinline__ void sf_to_tmem(uint32_t elected, uint32_t taddr, uint64_t desc) {
-  if constexpr (kPair)
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
-        "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
-        "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(elected)
-        : "memory");
-}
-
-// Shared-memory descriptor of a scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups
-// 128 bytes apart.
-__device__ __forceinline__ uint64_t sf_desc(uint32_t smem_addr) {
-  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(1) << 16) |
-         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
-}
-
 // Instruction descriptor: e2m1 x e2m1 with e8m0 scales, both K-major; `sf_id` (0 or 2) is
 // the first of the two scale bytes, the same in both operands.
 __host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int sf_id) {
@@ -111,28 +87,9 @@ __host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n, int sf_id) {
          (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) | (static_cast<uint32_t>(sf_id) << 29);
 }
 
-// D[tmem] (+)= A * B, 64 values of K.
-template <bool kPair>
-__device__ __forceinline__ void mma_mxf4(uint32_t elected, uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  if constexpr (kPair)
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
-        "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
-            d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb), "r"(elected)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
-            d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb), "r"(elected)
-        : "memory");
-}
-
-// High words of the descriptors: those of sw128_kmajor_desc and sf_desc do not depend on the
-// address.
+// Shared-memory descriptors: the low word holds the address, the high word what does not
+// change: 128-byte swizzled K-major rows in groups of eight 1024 bytes apart (as
+// sw128_kmajor_desc), or a scale tile's 32 rows of 16 bytes, no swizzle, eight 128 bytes apart.
 constexpr uint32_t kSw128DescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 constexpr uint32_t kSfDescHi = (128u >> 4) | (1u << 14);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
@@ -171,6 +128,34 @@ __device__ __forceinline__ void pair_half_stage(uint32_t elected, uint32_t third
         "add.u32 t, %1, 2;\n\tadd.u32 w, %2, 2;\n\tmov.b64 u, {t, %7};\n\tmov.b64 v, {w, %7};\n\t"
         "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], u, v, %5, [%3], [%4], p;\n\t}" ::"r"(d),
         "r"(alo), "r"(blo), "r"(sfx), "r"(sfy_at), "r"(idesc2), "r"(elected), "r"(kSw128DescHi)
+        : "memory");
+}
+
+// The same for one CTA, whose second operand lies in one 128-row scale group.
+__device__ __forceinline__ void single_half_stage(uint32_t elected, uint32_t d, uint32_t alo, uint32_t blo,
+                                                  uint32_t xlo, uint32_t ylo, uint32_t sfx, uint32_t sfy,
+                                                  uint32_t idesc0, uint32_t idesc2, uint32_t accumulate, bool second) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      ".reg .b64 u, v;\n\t"
+      "setp.ne.b32 p, %8, 0;\n\tsetp.ne.b32 q, %9, 0;\n\t"
+      "mov.b64 u, {%3, %11};\n\t"
+      "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%5], u;\n\t"
+      "mov.b64 u, {%4, %11};\n\t"
+      "@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%6], u;\n\t"
+      "mov.b64 u, {%1, %10};\n\tmov.b64 v, {%2, %10};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], u, v, %7, [%5], [%6], p;\n\t}" ::"r"(d),
+      "r"(alo), "r"(blo), "r"(xlo), "r"(ylo), "r"(sfx), "r"(sfy), "r"(idesc0), "r"(accumulate), "r"(elected),
+      "r"(kSw128DescHi), "r"(kSfDescHi)
+      : "memory");
+  if (second)
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        ".reg .b64 u, v;\n\t.reg .b32 t, w;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\tsetp.eq.u32 p, 0, 0;\n\t"
+        "add.u32 t, %1, 2;\n\tadd.u32 w, %2, 2;\n\tmov.b64 u, {t, %7};\n\tmov.b64 v, {w, %7};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], u, v, %5, [%3], [%4], p;\n\t}" ::"r"(d),
+        "r"(alo), "r"(blo), "r"(sfx), "r"(sfy), "r"(idesc2), "r"(elected), "r"(kSw128DescHi)
         : "memory");
 }
 
