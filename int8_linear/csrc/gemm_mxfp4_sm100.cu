@@ -700,48 +700,67 @@ constexpr int kHalfSmem = 233472 / 2 - 1024;
 
 static int split_stage_bytes(int tn) { return kMxRows * kMxRowBytes + tn * kMxRowBytes + 2 * kSfStageBytes; }
 
+// CTAs that share a split tile's K.  Doubled while they have SMs of their own and two stages
+// each, or, of a long K, half an SM and 14 stages each (us with c and 2c: 16 x 2048 x 2048
+// c = 4 5.1 and 5.4; 64 x 4096 x 14336 c = 4 11.6 and 12.0; 256 x 4096 x 14336 c = 2 18.5
+// and 17.0).
+static int split_cluster(int64_t tiles, int kblocks, int sms) {
+  int c = 1;
+  while (c < kMaxCluster &&
+         ((2 * c * tiles <= sms && kblocks >= 4 * c) || (2 * c * tiles <= 2 * sms && kblocks >= 28 * c)))
+    c *= 2;
+  return c;
+}
+
 static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   DeviceInfo di;
   if (int e = device_info(&di)) return e;
   const int kblocks = (K + kMxStageK - 1) / kMxStageK;
   *p = MxPlan{};
-  if (tile && tile->split == 4 ? true : !(tile && (tile->tok_tile || tile->split)) && M > 256) {
-    if (tile && tile->split == 4 && (tile->swap_ab || tile->tok_tile != 128 || tile->w_tile != kWide))
+  const i8l_tile t = tile ? *tile : i8l_tile{};
+  if (t.split != 0 && t.split != 1 && t.split != 3 && t.split != 4)
+    return set_error(I8L_ENOTSUP, "split mode %d unknown to 4-bit products (0 auto, 1 whole, 3 cluster, 4 CTA pairs)",
+                     t.split);
+  auto count = [&](int tn) { return (static_cast<int64_t>(N) + kMxRows - 1) / kMxRows * ((static_cast<int64_t>(M) + tn - 1) / tn); };
+  p->pair = t.split == 4;
+  if (t.split == 0 && t.tok_tile == 0 && M > 64) {
+    // Pairs where 128-token split tiles would fill more than a quarter of the SMs, but for a
+    // long K that two CTAs a tile can share (us by split tiles and by pairs: 128 x 4096 x 4096
+    // 9.6 and 11.3, 128 x 12288 x 2048 10.6 and 10.1, 256 x 12288 x 2048 13.1 and 11.2,
+    // 512 x 4096 x 14336 23.4 and 25.2).
+    const int64_t tiles = count(128);
+    p->pair = tiles > di.sms / 4 && !(kblocks >= 24 && tiles <= di.sms && split_cluster(tiles, kblocks, di.sms) > 1);
+  }
+  if (p->pair) {
+    if (t.split == 4 && (t.swap_ab || t.tok_tile != 128 || t.w_tile != kWide))
       return set_error(I8L_ENOTSUP, "CTA pairs (split 4) take tok_tile 128 x w_tile %d tiles without swap_ab", kWide);
-    p->pair = 1;
     p->tn = 2 * kMxRows;
     p->cluster = 2;
     const int most = (di.max_smem_optin - static_cast<int>(pair_smem(0))) / (kPairStageBytes + 16);
-    p->stages = tile && tile->stages ? tile->stages : most;
+    p->stages = t.stages ? t.stages : most;
     if (p->stages < 2 || p->stages > most)
       return set_error(I8L_ENOTSUP, "stages %d outside [2, %d] for this tile", p->stages, most);
     return I8L_OK;
   }
-  p->tn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  if (tile && tile->tok_tile) p->tn = tile->tok_tile;
+  p->tn = t.tok_tile ? t.tok_tile : M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   if (p->tn != 16 && p->tn != 32 && p->tn != 64 && p->tn != 128)
     return set_error(I8L_ENOTSUP, "token tile %d is none of 16, 32, 64, 128", p->tn);
   if (p->tn < 128 && M > p->tn)
     return set_error(I8L_ENOTSUP, "a %d-token tile holds the whole batch, %d tokens given", p->tn, M);
-  const int tiles = ((N + kMxRows - 1) / kMxRows) * ((M + p->tn - 1) / p->tn);
-  // Double the CTAs of a tile while they have SMs of their own and two stages each, or, of a
-  // long K, half an SM and 14 stages each (us with c and 2c: 16 x 2048 x 2048 c = 4 5.1 and
-  // 5.4; 64 x 4096 x 14336 c = 4 11.6 and 12.0; 256 x 4096 x 14336 c = 2 18.5 and 17.0).
-  int c = 1;
-  while (c < kMaxCluster && ((2 * c * tiles <= di.sms && kblocks >= 4 * c) ||
-                             (2 * c * tiles <= 2 * di.sms && kblocks >= 28 * c)))
-    c *= 2;
-  if (tile && tile->cluster) c = tile->cluster;
+  if (t.tok_tile && (!t.swap_ab || t.w_tile != 128))
+    return set_error(I8L_ENOTSUP, "token tiles of 4-bit products take w_tile 128 with swap_ab");
+  const int64_t tiles = count(p->tn);
+  const int c = t.split == 1 ? 1 : t.cluster ? t.cluster : split_cluster(tiles, kblocks, di.sms);
   if (c < 1 || c > kMaxCluster || c > kblocks)
     return set_error(I8L_ENOTSUP, "cluster size %d outside [1, min(8, k-blocks=%d)]", c, kblocks);
   p->cluster = c;
-  const int most = std::min(16, (di.max_smem_optin - 1024 - 256) / split_stage_bytes(p->tn));
+  const int stage = split_stage_bytes(p->tn);
+  const int most = std::min(16, (di.max_smem_optin - 1024 - 256) / stage);
   // More CTAs than SMs share an SM in twos.
-  const int two = (kHalfSmem - 1024 - 256) / split_stage_bytes(p->tn);
-  int s = std::min((kblocks + c - 1) / c, tiles * c > di.sms ? std::min(two, 5) : 6);
-  if (tile && tile->stages) s = tile->stages;
-  if (s < 1 || s > most) return set_error(I8L_ENOTSUP, "stages %d outside [1, %d] for this tile", s, most);
-  p->stages = s;
+  const int share = tiles * c > di.sms ? std::min(5, (kHalfSmem - 1024 - 256) / stage) : 6;
+  p->stages = t.stages ? t.stages : std::min((kblocks + c - 1) / c, share);
+  if (p->stages < 1 || p->stages > most)
+    return set_error(I8L_ENOTSUP, "stages %d outside [1, %d] for this tile", p->stages, most);
   return I8L_OK;
 }
 
@@ -770,6 +789,8 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
   if (K == 0) return set_error(I8L_ENOTSUP, "K=0 is not supported");
   if (K % kMxBlock) return set_error(I8L_ENOTSUP, "K=%d must be a multiple of 32 (whole blocks)", K);
   if (K > kMxMaxK) return set_error(I8L_ENOTSUP, "K=%d is above %d", K, kMxMaxK);
+  constexpr int32_t kMost = INT32_MAX - 1024;  // tile coordinates stay inside 32 bits
+  if (M > kMost || N > kMost) return set_error(I8L_ENOTSUP, "M=%d or N=%d is above %d", M, N, kMost);
   if (!A || !W || !sa || !sw || !out) return set_error(I8L_EINVAL, "NULL operand pointer");
   if (lda < K / 2 || ldw < K / 2 || ldc < N)
     return set_error(I8L_EINVAL, "leading dimensions lda=%lld ldw=%lld ldc=%lld too small",
@@ -781,8 +802,6 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
     return set_error(I8L_ENOTSUP, "bias dtype code %d not supported", bias_dtype);
   MxPlan p;
   if (int e = make_mx_plan(M, N, K, tile, &p)) return e;
-  DeviceInfo di;
-  if (int e = device_info(&di)) return e;
   MxGemmArgs a{};
   a.M = M;
   a.N = N;
@@ -825,8 +844,11 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
       a.tma_out = 1;
     }
     a.per_col = FastDiv(static_cast<uint32_t>(a.tiles_m));
+    DeviceInfo di;
+    if (int e = device_info(&di)) return e;
+    const int ctas = tile && tile->ctas ? tile->ctas : di.sms;
     const int64_t tiles = static_cast<int64_t>(a.tiles_m) * ((N + kBoth - 1) / kBoth + (N + kBoth - 1 - kWide) / kBoth);
-    const int pairs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, (tile && tile->ctas ? tile->ctas : di.sms) / 2)));
+    const int pairs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, ctas / 2)));
     return out_dtype == I8L_BF16  ? launch_pair<I8L_BF16>(mx, my, mn, msx, msy, mo, a, pairs, s)
            : out_dtype == I8L_F16 ? launch_pair<I8L_F16>(mx, my, mn, msx, msy, mo, a, pairs, s)
                                   : launch_pair<I8L_F32>(mx, my, mn, msx, msy, mo, a, pairs, s);

@@ -19,6 +19,9 @@ launch with the same bits as the two it replaces (a batch the fused kernel decli
 the two steps).  With fuse_o_proj, o_proj's quantiser also runs inside tensor-core tilings
 that have direct activation loads (w8a8_mm_quant_act); off by default, as those tilings
 were measured slower on B200 than the quantiser followed by the tuned tiling.
+
+MXFP4StandinDecoder is the same decoder with 4-bit linears and with the query/key norm and
+position rotation that a Qwen3 layer has after qkv_proj.
 """
 
 from __future__ import annotations
@@ -29,6 +32,8 @@ import torch
 
 from int8_linear.fused_quant import add_rmsnorm_quant, per_token_quant, silu_mul_quant
 from int8_linear import kernel
+from int8_linear.mxfp4 import add_rmsnorm_quant_mxfp4, quant_mxfp4, silu_mul_quant_mxfp4, w4a4_mm
+from int8_linear.qk_norm import qk_norm_rope
 from int8_linear.kernel import (Config, choose_config, rmsnorm_w8a8_mm, silu_mul_w8a8_mm, w8a8_mm,
                                 w8a8_mm_quant_act)
 
@@ -43,6 +48,7 @@ FUSE_DEFAULT: dict[int, tuple[str, ...]] = {1: ("o_proj", "gate_up_proj"), 2: ("
 # (K, N) of each linear, as vLLM runs Qwen3-1.7B (merged qkv and gate_up).
 SHAPES = {"qkv_proj": (2048, 4096), "o_proj": (2048, 2048),
           "gate_up_proj": (2048, 12288), "down_proj": (6144, 2048)}
+Q_HEADS, KV_HEADS, HEAD_DIM, ROPE_BASE = 16, 8, 128, 1e6
 
 
 @dataclass
@@ -247,6 +253,79 @@ class StandinDecoder:
     def weight_bytes(self) -> int:
         return sum(lin.w_t.numel() + lin.scale.numel() * 4 for layer in self.layers
                    for lin in layer.values())
+
+
+@dataclass
+class MXFP4Linear:
+    q_t: torch.Tensor    # [K/2, N] view of the [N, K/2] codes
+    scale: torch.Tensor  # scale tiles, as quant_mxfp4 gives them
+
+
+class MXFP4StandinDecoder:
+    """The decoder's step for m tokens with 4-bit (MXFP4) linears, per layer
+
+        add_rmsnorm_quant_mxfp4 -> qkv product -> qk_norm_rope -> quant_mxfp4 of the queries
+        -> o_proj product -> add_rmsnorm_quant_mxfp4 -> gate_up product
+        -> silu_mul_quant_mxfp4 -> down product
+
+    with the queries standing in for attention's output.  Weights are normal values of
+    standard deviation 0.02 quantised by quant_mxfp4, drawn from one seeded generator in
+    layer order; `positions` [m] (int64) are the tokens' places and may be changed between
+    steps, in place for a captured one."""
+
+    def __init__(self, m: int, layers: int = LAYERS, seed: int = 0, device="cuda", max_positions: int = 4096):
+        g = torch.Generator(device=device).manual_seed(seed)
+        self.x = torch.randn((m, HIDDEN), generator=g, device=device).to(torch.bfloat16)
+        self.w = torch.ones(HIDDEN, device=device, dtype=torch.bfloat16)
+        self.q_w = torch.ones(HEAD_DIM, device=device, dtype=torch.bfloat16)
+        self.k_w = torch.ones(HEAD_DIM, device=device, dtype=torch.bfloat16)
+        self.positions = torch.arange(m, device=device) % max_positions
+        freq = ROPE_BASE ** (-torch.arange(0, HEAD_DIM, 2, device=device, dtype=torch.float64) / HEAD_DIM)
+        angle = torch.arange(max_positions, device=device, dtype=torch.float64)[:, None] * freq
+        self.cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float()
+        self.layers: list[dict[str, MXFP4Linear]] = []
+        for _ in range(layers):
+            layer = {}
+            for name, (k, n) in SHAPES.items():
+                w = (torch.randn((n, k), generator=g, device=device) * 0.02).to(torch.bfloat16)
+                q, s = quant_mxfp4(w)
+                layer[name] = MXFP4Linear(q.t(), s)
+            self.layers.append(layer)
+        self.graph: torch.cuda.CUDAGraph | None = None
+        self.out: torch.Tensor | None = None
+
+    def step(self, record: list | None = None) -> torch.Tensor:
+        """One step.  With `record` (a list), every op appends (layer, op name, inputs,
+        outputs), so a test can check each op on its own inputs."""
+
+        def rec(i, name, ins, outs):
+            if record is not None:
+                record.append((i, name, ins, outs))
+            return outs
+
+        def mm(i, name, q, s):
+            lin = self.layers[i][name]
+            return rec(i, name, (q, s, lin), w4a4_mm(q, lin.q_t, s, lin.scale))
+
+        h, res = self.x, None
+        for i in range(len(self.layers)):
+            q, s, rout = rec(i, "norm", (h, res, self.w), add_rmsnorm_quant_mxfp4(h, res, self.w, EPS))
+            res = h if rout is None else rout
+            qkv = mm(i, "qkv_proj", q, s)
+            queries, _ = rec(i, "qk_norm", (qkv, self.q_w, self.k_w, self.positions, self.cos_sin),
+                             qk_norm_rope(qkv, self.q_w, self.k_w, EPS, self.positions, self.cos_sin, Q_HEADS,
+                                          KV_HEADS))
+            queries = queries.view(-1, Q_HEADS * HEAD_DIM)
+            h = mm(i, "o_proj", *rec(i, "quant", (queries,), quant_mxfp4(queries)))
+            q, s, res = rec(i, "post_norm", (h, res, self.w), add_rmsnorm_quant_mxfp4(h, res, self.w, EPS))
+            gu = mm(i, "gate_up_proj", q, s)
+            h = mm(i, "down_proj", *rec(i, "silu_mul_quant", (gu,), silu_mul_quant_mxfp4(gu)))
+        return h
+
+    capture = StandinDecoder.capture
+
+    def weight_bytes(self) -> int:
+        return sum(lin.q_t.numel() + lin.scale.numel() for layer in self.layers for lin in layer.values())
 
 
 class TPStandinDecoder:
