@@ -54,7 +54,7 @@ struct MxGemmArgs {
 
 // ------------------------------------------------------------------ split tiles
 
-constexpr int kSplitThreads = 128;
+constexpr int kSplitThreads = 256;  // two warps for each quarter of the TMEM lanes
 constexpr int kMaxCluster = 8;
 
 template <int TN>
@@ -78,6 +78,37 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
+}
+
+// Units u0..u1-1 (four floats each) of the partial tiles at `red` in every CTA of a cluster of
+// at most C, added in rank order and handed to finish(unit, sum).  A read of another CTA's
+// shared memory takes some 700 cycles, so those of kAhead units and all CTAs are on their way
+// together.
+template <int C, int kAhead, typename Finish>
+__device__ __forceinline__ void add_partials(uint32_t red, int u0, int u1, int cluster, Finish finish) {
+  for (int u = u0 + static_cast<int>(threadIdx.x); u < u1; u += kAhead * kSplitThreads) {
+    float4 f[kAhead][C];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int p = 0; p < C; ++p)
+        if (p < cluster && u + i * kSplitThreads < u1)
+          f[i][p] = ld_cluster_v4(map_to_rank(red + (u + i * kSplitThreads) * 16, static_cast<uint32_t>(p)));
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (u + i * kSplitThreads >= u1) break;
+      float4 sum = f[i][0];
+#pragma unroll
+      for (int p = 1; p < C; ++p)
+        if (p < cluster) {
+          sum.x += f[i][p].x;
+          sum.y += f[i][p].y;
+          sum.z += f[i][p].z;
+          sum.w += f[i][p].w;
+        }
+      finish(u + i * kSplitThreads, sum);
+    }
+  }
 }
 
 // Stores outputs n0..n0+3 of token row m.
@@ -232,13 +263,13 @@ __global__ void __launch_bounds__(kSplitThreads)
   const int live = min(TN, a.M - ty * TN);  // tokens of this tile
   // Every MMA has read its operands: the ring holds the partial tile now, [token][128 n].
   if (__syncthreads_and(ok)) {
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    for (int c = 0; c < live; c += 16) {
+    const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    for (int c = (warp >> 2) * 16; c < live; c += 32) {
       uint32_t r[16];
       tmem_ld16(taddr + c, r);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) red[(c + j) * kMxRows + threadIdx.x] = __uint_as_float(r[j]);
+      for (int j = 0; j < 16; ++j) red[(c + j) * kMxRows + (warp & 3) * 32 + lane] = __uint_as_float(r[j]);
     }
   }
   tc_fence_before();
@@ -264,34 +295,10 @@ __global__ void __launch_bounds__(kSplitThreads)
 #pragma unroll 4
       for (int u = u0 + static_cast<int>(threadIdx.x); u < u1; u += kSplitThreads)
         finish(u, reinterpret_cast<const float4 *>(red)[u]);
+    } else if (a.cluster <= 4) {
+      add_partials<4, 4>(smem_u32(red), u0, u1, a.cluster, finish);
     } else {
-      // A read of another CTA's shared memory takes some 700 cycles: those of kAhead units
-      // and every CTA are on their way together, then added in rank order.
-      constexpr int kAhead = 2;
-      const uint32_t at = smem_u32(red);
-      for (int u = u0 + static_cast<int>(threadIdx.x); u < u1; u += kAhead * kSplitThreads) {
-        float4 f[kAhead][kMaxCluster];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-          for (int p = 0; p < kMaxCluster; ++p)
-            if (p < a.cluster && u + i * kSplitThreads < u1)
-              f[i][p] = ld_cluster_v4(map_to_rank(at + (u + i * kSplitThreads) * 16, static_cast<uint32_t>(p)));
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (u + i * kSplitThreads >= u1) break;
-          float4 sum = f[i][0];
-#pragma unroll
-          for (int p = 1; p < kMaxCluster; ++p)
-            if (p < a.cluster) {
-              sum.x += f[i][p].x;
-              sum.y += f[i][p].y;
-              sum.z += f[i][p].z;
-              sum.w += f[i][p].w;
-            }
-          finish(u + i * kSplitThreads, sum);
-        }
-      }
+      add_partials<kMaxCluster, 2>(smem_u32(red), u0, u1, a.cluster, finish);
     }
   }
   // No CTA leaves while another may still read its partial sums.
@@ -701,13 +708,14 @@ constexpr int kHalfSmem = 233472 / 2 - 1024;
 static int split_stage_bytes(int tn) { return kMxRows * kMxRowBytes + tn * kMxRowBytes + 2 * kSfStageBytes; }
 
 // CTAs that share a split tile's K.  Doubled while they have SMs of their own and two stages
-// each, or, of a long K, half an SM and 14 stages each (us with c and 2c: 16 x 2048 x 2048
-// c = 4 5.1 and 5.4; 64 x 4096 x 14336 c = 4 11.6 and 12.0; 256 x 4096 x 14336 c = 2 18.5
-// and 17.0).
-static int split_cluster(int64_t tiles, int kblocks, int sms) {
+// each, or, of a long K, half an SM and 14 stages each; four at most on 128-token tiles, whose
+// partial sums are the larger part of the work (us with c and 2c: 16 x 2048 x 2048 c = 4 5.1
+// and 5.4; 64 x 4096 x 14336 c = 4 11.4 and 12.4; 512 x 4096 x 14336 c = 1 24.7 and 21.8;
+// 128 x 2048 x 6144 c = 4 8.9 and 10.6).
+static int split_cluster(int64_t tiles, int kblocks, int sms, int tn) {
+  const int most = tn == 128 ? 4 : kMaxCluster;
   int c = 1;
-  while (c < kMaxCluster &&
-         ((2 * c * tiles <= sms && kblocks >= 4 * c) || (2 * c * tiles <= 2 * sms && kblocks >= 28 * c)))
+  while (c < most && ((2 * c * tiles <= sms && kblocks >= 4 * c) || (2 * c * tiles <= 2 * sms && kblocks >= 28 * c)))
     c *= 2;
   return c;
 }
@@ -723,14 +731,10 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
                      t.split);
   auto count = [&](int tn) { return (static_cast<int64_t>(N) + kMxRows - 1) / kMxRows * ((static_cast<int64_t>(M) + tn - 1) / tn); };
   p->pair = t.split == 4;
-  if (t.split == 0 && t.tok_tile == 0 && M > 64) {
-    // Pairs where 128-token split tiles would fill more than a quarter of the SMs, but for a
-    // long K that two CTAs a tile can share (us by split tiles and by pairs: 128 x 4096 x 4096
-    // 9.6 and 11.3, 128 x 12288 x 2048 10.6 and 10.1, 256 x 12288 x 2048 13.1 and 11.2,
-    // 512 x 4096 x 14336 23.4 and 25.2).
-    const int64_t tiles = count(128);
-    p->pair = tiles > di.sms / 4 && !(kblocks >= 24 && tiles <= di.sms && split_cluster(tiles, kblocks, di.sms) > 1);
-  }
+  // Pairs where 128-token split tiles are more than the SMs (us by split tiles and by pairs:
+  // 128 x 12288 x 2048, 96 tiles, 9.4 and 10.0; 1024 x 2048 x 2048, 128 tiles, 8.8 and 9.6;
+  // 256 x 12288 x 2048, 192 tiles, 13.1 and 11.2).
+  if (t.split == 0 && t.tok_tile == 0 && M > 64) p->pair = count(128) > di.sms;
   if (p->pair) {
     if (t.split == 4 && (t.swap_ab || t.tok_tile != 128 || t.w_tile != kWide))
       return set_error(I8L_ENOTSUP, "CTA pairs (split 4) take tok_tile 128 x w_tile %d tiles without swap_ab", kWide);
@@ -750,7 +754,7 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   if (t.tok_tile && (!t.swap_ab || t.w_tile != 128))
     return set_error(I8L_ENOTSUP, "token tiles of 4-bit products take w_tile 128 with swap_ab");
   const int64_t tiles = count(p->tn);
-  const int c = t.split == 1 ? 1 : t.cluster ? t.cluster : split_cluster(tiles, kblocks, di.sms);
+  const int c = t.split == 1 ? 1 : t.cluster ? t.cluster : split_cluster(tiles, kblocks, di.sms, p->tn);
   if (c < 1 || c > kMaxCluster || c > kblocks)
     return set_error(I8L_ENOTSUP, "cluster size %d outside [1, min(8, k-blocks=%d)]", c, kblocks);
   p->cluster = c;
