@@ -340,7 +340,8 @@ int i8l_dequant_mxfp4(const uint8_t *q, int64_t ldq, const uint8_t *scale, void 
  * at ldc elements of out_dtype (I8L_BF16/F16/F32).  The result of a shape and tile does
  * not vary from run to run.  tile: NULL or zeroed for the library's choice; of a given
  * one, split 0, 1 or 3 with tok_tile {16,32,64,128}, cluster and stages, or split 4 (CTA
- * pairs, tok_tile 128, w_tile 256) with stages and ctas.
+ * pairs, tok_tile 128, w_tile 256) with stages and ctas, or split 5 (CUDA cores, at most
+ * tok_tile in {1,2,4} tokens, w_tile 0).
  */
 int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, const uint8_t *W, int64_t ldw,
                 const uint8_t *sw, const void *bias, int32_t bias_dtype, void *out,

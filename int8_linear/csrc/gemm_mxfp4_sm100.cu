@@ -727,7 +727,7 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   *p = MxPlan{};
   const i8l_tile t = tile ? *tile : i8l_tile{};
   if (t.split != 0 && t.split != 1 && t.split != 3 && t.split != 4)
-    return set_error(I8L_ENOTSUP, "split mode %d unknown to 4-bit products (0 auto, 1 whole, 3 cluster, 4 CTA pairs)",
+    return set_error(I8L_ENOTSUP, "split mode %d unknown to 4-bit products (0 auto, 1 whole, 3 cluster, 4 CTA pairs, 5 CUDA cores)",
                      t.split);
   auto count = [&](int tn) { return (static_cast<int64_t>(N) + kMxRows - 1) / kMxRows * ((static_cast<int64_t>(M) + tn - 1) / tn); };
   p->pair = t.split == 4;
@@ -804,6 +804,11 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
     return set_error(I8L_ENOTSUP, "4-bit operands, their row strides and their scales must be 16-byte aligned");
   if (bias && (bias_dtype < I8L_BF16 || bias_dtype > I8L_F32))
     return set_error(I8L_ENOTSUP, "bias dtype code %d not supported", bias_dtype);
+  if (tile ? tile->split == 5 : mx_gemv_holds(M)) {
+    if (!mx_gemv_holds(M) || (tile && (tile->swap_ab || tile->w_tile || (tile->tok_tile && tile->tok_tile < M))))
+      return set_error(I8L_ENOTSUP, "CUDA-core tiles (split 5) of 4-bit products take at most 4 tokens, w_tile 0, no swap_ab");
+    return mx_gemv_run(A, lda, sa, W, ldw, sw, bias, bias_dtype, out, out_dtype, ldc, M, N, K, stream);
+  }
   MxPlan p;
   if (int e = make_mx_plan(M, N, K, tile, &p)) return e;
   MxGemmArgs a{};

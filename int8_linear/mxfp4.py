@@ -155,12 +155,14 @@ SPLIT_TILES = (16, 32, 64, 128)
 
 def _tile(config: Config) -> _native.I8LTile:
     """The C tile of a Config for the 4-bit product: swap_ab token tiles with split 0, 1 or 3,
-    or CTA pairs (split 4)."""
+    CTA pairs (split 4) or CUDA cores (split 5)."""
+    if config.split == 5 and config.bm in (1, 2, 4) and config.bn == 0:
+        return _native.I8LTile(tok_tile=config.bm, split=5)
     if config.split == 4 and not config.swapped and config.bm == 128 and config.bn == 256:
         return _native.I8LTile(tok_tile=128, w_tile=256, stages=config.stages, ctas=config.ctas, split=4)
     if config.split not in (0, 1, 3) or not config.swapped or config.bm not in SPLIT_TILES or config.bn != 128:
-        raise NotSupported(f"{config.name}: 4-bit tiles are bm in {SPLIT_TILES} x bn 128 with swap_ab, or pairs "
-                           "(128 x 256, split 4)")
+        raise NotSupported(f"{config.name}: 4-bit tiles are bm in {SPLIT_TILES} x bn 128 with swap_ab, pairs "
+                           "(128 x 256, split 4) or CUDA cores (bm 1, 2 or 4, bn 0, split 5)")
     return _native.I8LTile(swap_ab=1, tok_tile=config.bm, w_tile=128, stages=config.stages, split=config.split,
                            cluster=1 if config.split == 1 else config.cluster)
 
@@ -175,8 +177,9 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
     as quant_mxfp4 gives them.  The sum is float32 on the tensor cores, bias (bf16, fp16 or
     fp32, [N]) is added in float32, and one rounding makes the bf16, fp16 or fp32 output.
     `out` is an [M, N] tensor with contiguous rows to write into.  `config` picks a tiling
-    (swap_ab token tiles of 16 to 128 with split 1 or 3, cluster and stages, or CTA pairs:
-    bm 128, bn 256, split 4) in place of the library's choice.  Raises NotSupported for what the kernel does not take and ValueError
+    (swap_ab token tiles of 16 to 128 with split 1 or 3, cluster and stages; CTA pairs: bm
+    128, bn 256, split 4; or CUDA cores for at most four tokens: bm 1, 2 or 4, bn 0, split 5)
+    in place of the library's choice.  Raises NotSupported for what the kernel does not take and ValueError
     for inconsistent arguments."""
     if a_q.dtype != torch.uint8 or b_q.dtype != torch.uint8:
         raise NotSupported(f"uint8 4-bit codes only, got {a_q.dtype} and {b_q.dtype}")

@@ -64,6 +64,13 @@ def test_every_split_tile(tn, cluster, stages):
         exact(200, 200, 2336, cfg, seed=cluster)
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 4])
+@pytest.mark.parametrize("n,k", [(1, 32), (33, 96), (130, 160), (257, 2048), (515, 2080), (100, 4128), (4096, 2048),
+                                 (12300, 544)])
+def test_cuda_core_tiles(m, n, k):
+    exact(m, n, k, Config(4 if m == 3 else m, 0, split=5), seed=m)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (128, 256, 256), (256, 256, 64), (257, 513, 1056), (300, 40, 2336),
                                    (1000, 1000, 992), (2600, 3000, 288)])
 @pytest.mark.parametrize("stages,ctas", [(0, 0), (2, 0), (3, 6)])
@@ -105,7 +112,7 @@ def test_quantised_operands(m, n, k, dtype):
     near(a, sa, va, b, sb, vb, dtype, rand((n,), 3, 0.1, dtype))
 
 
-@pytest.mark.parametrize("m,n,k", [(9, 130, 320), (130, 70, 320), (300, 270, 320)])
+@pytest.mark.parametrize("m,n,k", [(3, 130, 320), (9, 130, 320), (130, 70, 320), (300, 270, 320)])
 def test_strides_pointers_and_out(m, n, k):
     """Rows of wider matrices, pointers that TMA cannot take (copied), an unaligned or
     strided out, whose other bytes stay as they were."""
@@ -139,6 +146,8 @@ def test_nan_blocks_reach_their_rows_and_columns_only():
     got = mxfp4.w4a4_mm(a, b.t(), sa, sb)
     pair = mxfp4.w4a4_mm(a, b.t(), sa, sb, config=Config(128, 256, split=4))
     assert torch.equal(got.isnan(), pair.isnan())
+    few = mxfp4.w4a4_mm(a[5:9], b.t(), mxfp4.quant_mxfp4(x[5:9])[1], sb, config=Config(4, 0, split=5))
+    assert torch.equal(few.isnan(), got[5:9].isnan())
     want = torch.zeros((40, 200), dtype=torch.bool, device="cuda")
     want[7], want[:, 150] = True, True
     assert torch.equal(got.isnan(), want) and torch.isfinite(got[~want]).all()
@@ -146,7 +155,7 @@ def test_nan_blocks_reach_their_rows_and_columns_only():
 
 def test_scales_of_all_sizes():
     """Blocks from 2^-127 up: sums of very small and very large products."""
-    for m in (4, 150):
+    for m in (4, 20, 150):
         a, sa, va = operand(m, 256, 5, spread=60)
         b, sb, vb = operand(140, 256, 6, spread=60)
         near(a, sa, va, b, sb, vb, torch.float32)
@@ -200,7 +209,7 @@ def test_refusals_and_empty():
         mxfp4.w4a4_mm(a, b.t(), sa, sb, bias=torch.zeros(5, device="cuda"))
     with pytest.raises(ValueError):
         mxfp4.w4a4_mm(a, b.t(), sa, sb, out=torch.zeros((4, 5), device="cuda"))
-    for cfg in (Config(256, 128), Config(16, 0, split=5), Config(16, 128, split=3, cluster=2),
+    for cfg in (Config(256, 128), Config(16, 0, split=5), Config(2, 0, split=5), Config(16, 128, split=3, cluster=2),
                 Config(16, 128, split=1, stages=99)):
         with pytest.raises(NotSupported):
             mxfp4.w4a4_mm(a, b.t(), sa, sb, config=cfg)
