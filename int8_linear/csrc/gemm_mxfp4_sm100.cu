@@ -18,7 +18,11 @@
 // of its 128 rows, the whole weight tile's.  TMEM's 512 columns do not hold two accumulators
 // of 256 and the scales, so every other tile has 192 weight rows: 256 + 192 columns of
 // accumulators leave 64 for the scales, and one tile's epilogue runs beside the next tile's
-// MMAs.  XXXPAIR
+// MMAs.  4096 x 12288 x 2048 takes 49 us (4.2 PFLOP/s; 5.8 at K = 8192).  What bounds it is
+// the operands' way from L2: with the loads left out the same MMAs ran at 8.3 PFLOP/s, and
+// 36 KB a stage and SM is 97 bytes a ns and SM.  Other tilings measured: 256 x 256 with two
+// accumulators sharing 32 columns 53 us (each tile waits for the last one's shared columns),
+// 256 x 192 throughout 53 us (a 256-row MMA takes the same time for 192 and 256 columns).
 #include <algorithm>
 
 #include "common.cuh"
@@ -804,8 +808,9 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
     return set_error(I8L_ENOTSUP, "4-bit operands, their row strides and their scales must be 16-byte aligned");
   if (bias && (bias_dtype < I8L_BF16 || bias_dtype > I8L_F32))
     return set_error(I8L_ENOTSUP, "bias dtype code %d not supported", bias_dtype);
-  if (tile ? tile->split == 5 : mx_gemv_holds(M)) {
-    if (!mx_gemv_holds(M) || (tile && (tile->swap_ab || tile->w_tile || (tile->tok_tile && tile->tok_tile < M))))
+  const bool chosen = tile && (tile->split || tile->tok_tile);
+  if (chosen ? tile->split == 5 : mx_gemv_wins(M, N, K)) {
+    if (M > kMxGemvTokens || (chosen && (tile->swap_ab || tile->w_tile || (tile->tok_tile && tile->tok_tile < M))))
       return set_error(I8L_ENOTSUP, "CUDA-core tiles (split 5) of 4-bit products take at most 4 tokens, w_tile 0, no swap_ab");
     return mx_gemv_run(A, lda, sa, W, ldw, sw, bias, bias_dtype, out, out_dtype, ldc, M, N, K, stream);
   }

@@ -12,8 +12,10 @@
 // Here a CTA owns eight whole output columns: the weight rows that share the 32-byte sectors
 // of their scale tiles (rows 2j, 2j+1 and those 32, 64 and 96 further on).  A thread takes
 // one 16-byte load, a whole block, of four of the rows at a time, all in flight together and,
-// as weights do not depend on the previous kernel, before the dependency wait.
-// MEASURE
+// as weights do not depend on the previous kernel, before the dependency wait.  Measured at
+// 2048 x 2048 (2.2 MB): 2.7 us for one token, 3.9 for four, a launch of an empty kernel being
+// about 1.5; a tensor-core tile takes 4.8 to 5.0.  The permutes and dot products, half-rate
+// instructions, bound it from about 4096 x 2048 on (4.0 us).
 #include <algorithm>
 
 #include "common.cuh"
@@ -154,7 +156,13 @@ __global__ void __launch_bounds__(2 * kSpan) mx_gemv_kernel(const MxGemvArgs a) 
   }
 }
 
-bool mx_gemv_holds(int M) { return M <= 4; }
+// The arithmetic grows with the tokens, two, four or eight dot products a word, where a
+// tensor-core tile's time does not (us here and there: 1 x 8192 x 2048 5.1 and 5.9,
+// 1 x 12288 x 2048 7.1 and 6.3; 2 x 4096 x 2048 4.7 and 5.4, 2 x 2048 x 6144 6.9 and 5.9;
+// 4 x 2048 x 2048 3.9 and 5.0, 4 x 4096 x 2048 6.1 and 5.5).
+bool mx_gemv_wins(int M, int N, int K) {
+  return M <= kMxGemvTokens && static_cast<int64_t>(N) * K * (M <= 2 ? M : 4) <= 1 << 24;
+}
 
 int mx_gemv_run(const uint8_t *A, int64_t lda, const uint8_t *sa, const uint8_t *W, int64_t ldw, const uint8_t *sw,
                 const void *bias, int32_t bias_dtype, void *out, int32_t out_dtype, int64_t ldc, int32_t M, int32_t N,

@@ -60,9 +60,11 @@ int gemv_run(const int8_t *A, int64_t lda, const int8_t *W, int64_t ldw, const f
              int32_t bias_dtype, void *out, int32_t out_dtype, int64_t ldc, int32_t M, int32_t N,
              int32_t K, const i8l_tile *tile, void *stream, const GemvPro *pro = nullptr);
 
-// The CUDA-core form of w4a4_mm (split mode 5, gemv_mxfp4.cu): whether it takes a batch of M
-// tokens, and its launch (arguments as i8l_w4a4_mm, checked there).
-bool mx_gemv_holds(int M);
+// The CUDA-core form of w4a4_mm (split mode 5, gemv_mxfp4.cu): the most tokens it takes,
+// whether it is the faster form of a product, and its launch (arguments as i8l_w4a4_mm,
+// checked there).
+constexpr int kMxGemvTokens = 4;
+bool mx_gemv_wins(int M, int N, int K);
 int mx_gemv_run(const uint8_t *A, int64_t lda, const uint8_t *sa, const uint8_t *W, int64_t ldw, const uint8_t *sw,
                 const void *bias, int32_t bias_dtype, void *out, int32_t out_dtype, int64_t ldc, int32_t M, int32_t N,
                 int32_t K, void *stream);

@@ -7,7 +7,10 @@
 // what y is stored in differs.  A block's scale depends on its own 32 values, so there is
 // no row reduction in the plain and SiLU quantisers: a lane takes eight values, four
 // neighbouring lanes share a block (two shuffles), and the matrix is walked as one flat
-// list of eight-value vectors.  All four kernels move each byte once and are bound by HBM.
+// list of eight-value vectors or of blocks.  All four kernels move each byte once and are
+// bound by HBM: at 8192 rows (inputs larger than L2) quant_mxfp4 and dequant_mxfp4 take 26 us
+// of 8192 values, the measured copy rate; SiLU takes 42 us of 6144 (84 %, the rest is its
+// arithmetic and 48 % occupancy) and the norm 40 of 4096 with a residual (84 %).
 //
 // A 4-bit value next to the border between two steps flips on the last bit of y, so y is
 // computed to the bit: the norm's mean in float64, and SiLU in float32 with a second, exact
@@ -22,7 +25,6 @@
 namespace i8l {
 
 constexpr int kFlatThreads = 128;
-constexpr int64_t kBlockThreadsMin = 148 * 256;  // blocks from which a thread takes a whole one
 
 struct MxOut {
   uint8_t *q;
@@ -594,7 +596,7 @@ int check_mx(int32_t M, int32_t K, const void *q, int64_t ldq, const void *sf) {
   if (K > kMxMaxK) return set_error(I8L_ENOTSUP, "K=%d is above %d", K, kMxMaxK);
   if (M == 0 || K == 0) return I8L_OK;
   if (!q || !sf) return set_error(I8L_EINVAL, "NULL pointer argument");
-  if (ldq < K / 2) return set_error(I8L_EINVAL, "packed row stride %lld < K/2", static_cast<long long>(ldq));
+  if (M > 1 && ldq < K / 2) return set_error(I8L_EINVAL, "packed row stride %lld < K/2", static_cast<long long>(ldq));
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(sf)) % 4 || ldq % 4)
     return set_error(I8L_ENOTSUP, "packed rows and scales must be 4-byte aligned");
   return I8L_OK;
@@ -614,6 +616,8 @@ int64_t flat_rows(int32_t K) {
 template <bool kSilu>
 int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uint8_t *sf, int32_t M, int32_t K,
              void *stream, const char *what) {
+  DeviceInfo di;
+  if (int e = device_info(&di)) return e;
   const int blocks = K / kMxBlock, ktiles = (K + 127) / 128;
   const int64_t step = flat_rows(K);
   for (int64_t r0 = 0; r0 < M; r0 += step) {
@@ -631,10 +635,11 @@ int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uin
     a.q16 = aligned16(q) && ldq % 16 == 0 ? 1 : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err;
-    // A thread per block from 256 threads an SM on: with fewer, four lanes a block finish
-    // sooner (MEASURE).
+    // A thread per block from 256 blocks an SM on (SiLU: 512); with fewer, four lanes a block
+    // finish sooner (us by threads and by lanes: 18944 blocks 1.88 and 1.80, 75776 2.28 and
+    // 3.12, 303104 4.19 and 10.6; SiLU 37888 4.09 and 3.91, 151552 6.88 and 7.53).
     const int64_t total = a.vectors / 4;
-    if (dtype != I8L_F32 && total >= kBlockThreadsMin) {
+    if (dtype != I8L_F32 && total >= (kSilu ? 512 : 256) * di.sms) {
       if (a.vec && reinterpret_cast<uintptr_t>(x) % 32 == 0 && (ldx * 2) % 32 == 0) a.vec = 2;
       a.per_row = FastDiv(blocks);
       const dim3 grid(static_cast<unsigned>((total + a.pad_words + kFlatThreads - 1) / kFlatThreads));
@@ -675,6 +680,7 @@ extern "C" int i8l_quant_mxfp4(const void *x, int64_t ldx, int32_t dtype, uint8_
   if (int e = check_mx(M, K, q, ldq, scale)) return e;
   if (M == 0 || K == 0) return I8L_OK;
   if (!x) return set_error(I8L_EINVAL, "NULL pointer argument");
+  if (M == 1) ldx = std::max<int64_t>(ldx, K);  // a single row's stride is never used
   if (ldx < K) return set_error(I8L_EINVAL, "row stride smaller than K");
   return run_flat<false>(x, ldx, dtype, q, ldq, scale, M, K, stream, "quant_mxfp4 launch");
 }
@@ -686,6 +692,7 @@ extern "C" int i8l_silu_mul_quant_mxfp4(const void *gate_up, int64_t ld, int32_t
   if (int e = check_mx(M, I, q, ldq, scale)) return e;
   if (M == 0 || I == 0) return I8L_OK;
   if (!gate_up) return set_error(I8L_EINVAL, "NULL pointer argument");
+  if (M == 1) ld = std::max<int64_t>(ld, 2LL * I);
   if (ld < 2LL * I) return set_error(I8L_EINVAL, "row stride too small");
   return run_flat<true>(gate_up, ld, act_dtype, q, ldq, scale, M, I, stream, "silu_mul_quant_mxfp4 launch");
 }
@@ -703,6 +710,10 @@ extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const voi
   if (!x || !weight) return set_error(I8L_EINVAL, "NULL pointer argument");
   if ((residual == nullptr) != (rout == nullptr))
     return set_error(I8L_EINVAL, "residual and residual_out must be given together");
+  if (M == 1) {
+    ldx = std::max<int64_t>(ldx, K);
+    ldr = std::max<int64_t>(ldr, K);
+  }
   if (ldx < K || (residual && (ldr < K || ldro < K))) return set_error(I8L_EINVAL, "row stride smaller than K");
   const bool vec = vec_rows(x, ldx, act_dtype) &&
                    (!residual || (vec_rows(residual, ldr, act_dtype) && vec_rows(rout, ldro, act_dtype)));
@@ -729,9 +740,10 @@ extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const voi
   a.q16 = aligned16(q) && ldq % 16 == 0 ? 1 : 0;
   DeviceInfo di;
   if (int e = device_info(&di)) return e;
-  // A block per thread from 4 rows an SM on; fewer rows finish sooner spread over four times
-  // the threads (MEASURE).
-  const bool blocks = M >= 4 * di.sms && K <= 8192;
+  // A block per thread from 16 rows an SM on; fewer rows finish sooner spread over four times
+  // the threads (us by block and by vector: 592 rows of 2048 3.77 and 3.57, 1184 rows of 4096
+  // 8.22 and 8.02, 2368 rows of 4096 14.1 and 14.6).
+  const bool blocks = M >= 16 * di.sms && K <= 8192;
   if (blocks && vec) {
     auto wide = [](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 32 == 0 && ld % 16 == 0; };
     if (wide(x, ldx) && (!residual || (wide(residual, ldr) && wide(rout, ldro)))) a.vec = 2;

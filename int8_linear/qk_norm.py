@@ -5,7 +5,8 @@ B200 (sm_100a).
 
 is the step between the qkv linear of a Qwen3-shaped layer and its attention: each head is
 normalised over its own values, scaled by its weight and rotated by its token's position.
-The kernel is csrc/qk_norm.cu behind the C ABI; float32 inside, one rounding at the end.
+The kernel is csrc/qk_norm.cu behind the C ABI; float32 inside, one rounding at the end; also
+torch.ops.int8_linear.qk_norm_rope.
 The reference package (AshrithaG/int8-linear) leaves this step to vLLM.
 """
 
@@ -86,6 +87,20 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     length, rot = table.shape
     _native.on_device(dev, _native.load().i8l_qk_norm_rope, qkv.data_ptr(), qkv.stride(0), _ACT[qkv.dtype],
                       wq.data_ptr(), wk.data_ptr(), _WEIGHT[wdt], eps, pos.data_ptr(), wide, table.data_ptr(),
-                      _WEIGHT[table.dtype], length, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), m, heads,
+                      _WEIGHT[table.dtype], length, q.data_ptr(), q.stride(0) if m > 1 else heads * d, k.data_ptr(),
+                      k.stride(0) if m > 1 else kv_heads * d, m, heads,
                       kv_heads, d, rot, interleaved, current_stream(dev))
     return q, k
+
+
+@torch.library.custom_op("int8_linear::qk_norm_rope", mutates_args=())
+def qk_norm_rope_op(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
+                    positions: torch.Tensor, cos_sin: torch.Tensor, heads: int, kv_heads: int,
+                    interleaved: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return qk_norm_rope(qkv, q_weight, k_weight, eps, positions, cos_sin, heads, kv_heads, interleaved=interleaved)
+
+
+@qk_norm_rope_op.register_fake
+def _(qkv, q_weight, k_weight, eps, positions, cos_sin, heads, kv_heads, interleaved):
+    m, d = qkv.shape[0], q_weight.numel()
+    return qkv.new_empty((m, heads, d)), qkv.new_empty((m, kv_heads, d))

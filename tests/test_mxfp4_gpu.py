@@ -49,6 +49,44 @@ def test_quant_of_unaligned_and_strided_rows():
     check(*mxfp4.quant_mxfp4(x), np_(x))
 
 
+def test_one_row_may_have_any_stride():
+    flat = spread((512,), 3, torch.bfloat16)
+    w = torch.ones(256, dtype=torch.bfloat16, device="cuda")
+    for stride in (0, 1, 7, 300):
+        x = torch.as_strided(flat, (1, 256), (stride, 1))
+        check(*mxfp4.quant_mxfp4(x), np_(x))
+        check(*mxfp4.silu_mul_quant_mxfp4(x), om.silu_rows(np_(x), "bf16"))
+        q, s, r = mxfp4.add_rmsnorm_quant_mxfp4(x, x, w, EPS)
+        check(q, s, om.norm_rows(np_(x), np_(x), np_(w), EPS, "bf16", "bf16")[0])
+        back = mxfp4.dequant_mxfp4(torch.as_strided(q, q.shape, (stride, 1)), s)
+        assert torch.equal(back, mxfp4.dequant_mxfp4(q, s))
+    with pytest.raises(ValueError):
+        mxfp4.quant_mxfp4(flat[:256].expand(4, 256))       # rows on top of one another
+
+
+@pytest.mark.parametrize("m,k", [(600, 2048), (2500, 64), (2369, 4096), (2368, 8192), (3000, 8224)])
+@pytest.mark.parametrize("lo", [0, 8, 16, 3])
+def test_large_batches(m, k, lo):
+    """The forms that large batches take (a block per thread), 32-byte, 16-byte and unaligned
+    rows, against the same rows in small batches."""
+    wide, res = rand((m, 2 * k + 16), 7), rand((m, k + 16), 8)
+    w = rand((k,), 9, 0.1) + 1.0
+    x, r, gu = wide[:, lo:lo + k], res[:, lo:lo + k], wide[:, lo:lo + 2 * k]
+    for fn in (lambda rows: mxfp4.quant_mxfp4(x[rows]), lambda rows: mxfp4.silu_mul_quant_mxfp4(gu[rows]),
+               lambda rows: mxfp4.add_rmsnorm_quant_mxfp4(x[rows], r[rows], w, EPS),
+               lambda rows: mxfp4.add_rmsnorm_quant_mxfp4(x[rows], None, w, EPS)):
+        full = fn(slice(None))
+        for begin, end in ((0, 128), (m // 128 * 128 - 128, m)):
+            part = fn(slice(begin, end))
+            assert torch.equal(full[0][begin:end], part[0])
+            assert torch.equal(full[1][begin // 128:], part[1]) if end == m else torch.equal(full[1][:1], part[1])
+            if len(full) == 3 and full[2] is not None:
+                assert torch.equal(full[2][begin:end], part[2])
+    y, _ = om.norm_rows(np_(x[-40:]), np_(r[-40:]), np_(w), EPS, "bf16", "bf16")
+    codes, _ = om.quantise(y)
+    assert np.array_equal(np_(mxfp4.add_rmsnorm_quant_mxfp4(x, r, w, EPS)[0][-40:]), om.pack(codes))
+
+
 def test_rounding_borders_and_signs():
     """Every border between two steps, the values just beside it and their negatives, at
     scales across the range; the block's largest value fixes the scale at 4 to 8 steps."""
@@ -226,6 +264,9 @@ def test_custom_ops_opcheck():
     torch.library.opcheck(mxfp4.rmsnorm_quant_mxfp4_op, (x, w, EPS))
     torch.library.opcheck(mxfp4.add_rmsnorm_quant_mxfp4_op, (x, r, w, EPS))
     torch.library.opcheck(mxfp4.silu_mul_quant_mxfp4_op, (x,))
+    a, sa = mxfp4.quant_mxfp4(x)
+    b, sb = mxfp4.quant_mxfp4(r)
+    torch.library.opcheck(mxfp4.w4a4_mm_op, (a, b.t(), sa, sb, torch.bfloat16, None))
 
 
 def test_two_streams_and_graph_replay():

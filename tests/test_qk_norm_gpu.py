@@ -15,7 +15,7 @@ import pytest
 import torch
 
 from int8_linear import NotSupported
-from int8_linear.qk_norm import qk_norm_rope
+from int8_linear.qk_norm import qk_norm_rope, qk_norm_rope_op
 from tests.gpu_util import np_, rand
 
 pytestmark = pytest.mark.gpu
@@ -122,6 +122,16 @@ def test_positions_outside_the_table_give_nan_and_no_others_do():
     assert torch.equal(k.isnan().all(-1).all(-1), bad) and torch.equal(k.isnan().any(-1).any(-1), bad)
     q, _ = qk_norm_rope(qkv, w, w, EPS, pos, table(0, 0), 2, 1)      # no rotation: no angles needed
     assert torch.isfinite(q).all()
+
+
+def test_one_token_may_have_any_stride_and_the_op_checks():
+    flat, w, cs = rand((400,), 1), torch.ones(64, dtype=torch.bfloat16, device="cuda"), table(9, 64)
+    pos = torch.tensor([4], device="cuda")
+    want = qk_norm_rope(flat[:256].view(1, 256), w, w, EPS, pos, cs, 3, 1)
+    for stride in (0, 3):
+        got = qk_norm_rope(torch.as_strided(flat, (1, 256), (stride, 1)), w, w, EPS, pos, cs, 3, 1)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    torch.library.opcheck(qk_norm_rope_op, (flat[:256].view(1, 256), w, w, EPS, pos, cs, 3, 1, False))
 
 
 def test_special_heads_keep_to_themselves():

@@ -14,6 +14,7 @@ import numpy as np
 import pytest
 import torch
 
+import int8_linear
 from int8_linear import Config, NotSupported, _native, mxfp4
 from oracle import mxfp4 as om
 from tests.gpu_util import np_, rand
@@ -186,6 +187,39 @@ def test_runs_repeat_bit_for_bit_and_graphs_replay():
     torch.cuda.synchronize()
     assert all(torch.equal(o, first) for o in outs)
     assert _native.read_status() == 0
+
+
+def test_one_row_may_have_any_stride():
+    a, sa, va = operand(1, 96, 1)
+    b, sb, vb = operand(1, 96, 2)
+    for cfg in (None, Config(1, 0, split=5), Config(16, 128, split=1), Config(128, 256, split=4)):
+        for stride in (0, 5):
+            x, w = torch.as_strided(a, (1, 48), (stride, 1)), torch.as_strided(b, (1, 48), (stride, 1))
+            out = torch.as_strided(torch.empty(8, device="cuda"), (1, 1), (0, 1))
+            got = mxfp4.w4a4_mm(x, w.t(), sa, sb, torch.float32, config=cfg, out=out)
+            assert torch.equal(got.double(), va @ vb.t())
+
+
+def test_weights_to_copy_are_refused_under_programmatic_launch():
+    a, sa, va = operand(3, 64, 1)
+    b, sb, vb = operand(40, 64, 2)
+    odd = torch.zeros((40, 48), dtype=torch.uint8, device="cuda")
+    odd[:, 3:35] = b
+    int8_linear.set_pdl(True)
+    try:
+        with pytest.raises(NotSupported):
+            mxfp4.w4a4_mm(a, odd[:, 3:35].t(), sa, sb)
+        flat = torch.zeros(513, dtype=torch.uint8, device="cuda")
+        flat[1:] = sb.reshape(-1)
+        with pytest.raises(NotSupported):
+            mxfp4.w4a4_mm(a, b.t(), sa, flat[1:].view(1, 1, 512))
+        flat[1:] = sa.reshape(-1)
+        mxfp4.w4a4_mm(a, b.t(), flat[1:].view(1, 1, 512), sb)       # an activation is copied
+        mxfp4.w4a4_mm(a, b.t(), sa, torch.cat([sb, sb], 2)[:, :, :512])   # one tile: contiguous
+        got = mxfp4.w4a4_mm(a, b.t(), torch.cat([sa, sa], 2)[:, :, :512], sb, torch.float32)
+        assert torch.equal(got.double(), va @ vb.t())
+    finally:
+        int8_linear.set_pdl(False)
 
 
 def test_refusals_and_empty():
