@@ -39,6 +39,7 @@ from int8_linear.kernel import Config, current_stream
 
 BLOCK = 32
 _FLOAT = _WEIGHT  # bf16, fp16 and fp32
+_U8 = torch.uint8
 
 __all__ = ["w4a4_mm", "quant_mxfp4", "add_rmsnorm_quant_mxfp4", "silu_mul_quant_mxfp4", "dequant_mxfp4"]
 
@@ -47,19 +48,19 @@ def _rows(x: torch.Tensor, name: str, kinds: dict) -> tuple[int, int, int]:
     """(rows, columns, device index) of a quantiser's input, or the refusal of it."""
     if x.dtype not in kinds:
         raise NotSupported(f"{name} must be one of {[str(k) for k in kinds]}, got {x.dtype}")
-    if x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+    shape = x.shape
+    if len(shape) != 2 or (x.stride(1) != 1 and shape[1] > 1):
         raise NotSupported(f"{name} must be a 2-D tensor with contiguous rows")
     dev = x.get_device()
     if dev < 0:
         raise ValueError(f"the 4-bit quantisers run on a CUDA device, got {x.device}")
-    m, k = x.shape
-    return m, k, dev
+    return shape[0], shape[1], dev
 
 
 def _empty(x: torch.Tensor, m: int, k: int) -> tuple[torch.Tensor, torch.Tensor]:
     if k % BLOCK:
         raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks)")
-    q = x.new_empty((m, k >> 1), dtype=torch.uint8)
+    q = x.new_empty((m, k >> 1), dtype=_U8)
     return q, q.new_empty(((m + 127) >> 7, (k + 127) >> 7, 512))
 
 
@@ -118,7 +119,7 @@ def silu_mul_quant_mxfp4(gate_up: torch.Tensor) -> tuple[torch.Tensor, torch.Ten
 def _scales(s: torch.Tensor, rows: int, k: int, dev: int, name: str) -> torch.Tensor:
     """The scale tiles s of a [rows, k] operand on device `dev`, copied if the kernels cannot
     read them where they lie; raises if they are not that."""
-    if s.dtype != torch.uint8:
+    if s.dtype != _U8:
         raise NotSupported(f"{name} must be uint8 scale bytes, got {s.dtype}")
     if s.shape != ((rows + 127) >> 7, (k + 127) >> 7, 512) or s.get_device() != dev:
         raise ValueError(f"{name} must be the {[-(-rows // 128), -(-k // 128), 512]} scale tiles of [{rows}, {k}] on "
@@ -138,12 +139,13 @@ def _copied(t: torch.Tensor, name: str) -> torch.Tensor:
 
 def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """[M, K] values that codes q [M, K/2] and scales s stand for, in bf16, fp16 or fp32."""
-    if q.dtype != torch.uint8 or out_dtype not in _FLOAT:
+    if q.dtype != _U8 or out_dtype not in _FLOAT:
         raise NotSupported(f"uint8 codes to bf16, fp16 or fp32 only, got {q.dtype} to {out_dtype}")
-    if q.dim() != 2 or (q.stride(1) != 1 and q.shape[1] > 1):
+    shape, stride = q.shape, q.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise NotSupported("q must be a 2-D tensor with contiguous rows")
-    m, half = q.shape
-    k, dev = 2 * half, q.get_device()
+    m, half = shape
+    k, dev, ldq = 2 * half, q.get_device(), stride[0]
     if k % BLOCK:
         raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks)")
     if dev < 0:
@@ -151,9 +153,9 @@ def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = tor
     s = _scales(s, m, k, dev, "s")
     out = q.new_empty((m, k), dtype=out_dtype)
     if m and k:
-        if q.data_ptr() % 4 or q.stride(0) % 4 or q.stride(0) < half:
-            q = q.clone(memory_format=torch.contiguous_format)
-        _native.on_device(dev, _native.load().i8l_dequant_mxfp4, q.data_ptr(), q.stride(0), s.data_ptr(),
+        if q.data_ptr() % 4 or ldq % 4 or ldq < half:
+            q, ldq = q.clone(memory_format=torch.contiguous_format), half
+        _native.on_device(dev, _native.load().i8l_dequant_mxfp4, q.data_ptr(), ldq, s.data_ptr(),
                           out.data_ptr(), k, _FLOAT[out_dtype], m, k, current_stream(dev))
     return out
 
@@ -190,15 +192,18 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
     in place of the library's choice.  Raises NotSupported for what the kernel does not take and ValueError
     for inconsistent arguments.  With programmatic dependent launch (set_pdl) the weight must
     not have been written by the kernel just before, as for w8a8_mm."""
-    if a_q.dtype != torch.uint8 or b_q.dtype != torch.uint8:
+    if a_q.dtype != _U8 or b_q.dtype != _U8:
         raise NotSupported(f"uint8 4-bit codes only, got {a_q.dtype} and {b_q.dtype}")
-    if a_q.dim() != 2 or b_q.dim() != 2 or a_q.shape[1] != b_q.shape[0]:
-        raise ValueError(f"cannot multiply {tuple(a_q.shape)} by {tuple(b_q.shape)}")
-    m, half = a_q.shape
-    n, k, dev = b_q.shape[1], 2 * half, a_q.get_device()
+    shape_a, shape_b = a_q.shape, b_q.shape
+    if len(shape_a) != 2 or len(shape_b) != 2 or shape_a[1] != shape_b[0]:
+        raise ValueError(f"cannot multiply {tuple(shape_a)} by {tuple(shape_b)}")
+    m, half = shape_a
+    n, k, dev = shape_b[1], 2 * half, a_q.get_device()
     if k == 0 or k % BLOCK:
         raise NotSupported(f"K={k} must be a positive multiple of {BLOCK} (whole blocks)")
-    if b_q.stride(0) != 1 and n > 1:
+    lda, unit_a = a_q.stride()
+    unit_b, ldw = b_q.stride()
+    if unit_b != 1 and n > 1:
         raise NotSupported("b_q must be the K-contiguous [K/2, N] view of an [N, K/2] weight")
     if dev < 0 or b_q.get_device() != dev:
         raise ValueError(f"w4a4_mm runs on one CUDA device; got tensors on {a_q.device} and {b_q.device}")
@@ -213,27 +218,28 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
         bias_ptr, bias_code = bias.data_ptr(), _FLOAT[bias.dtype]
     if out_dtype not in _FLOAT:
         raise NotSupported(f"output dtype {out_dtype} not supported")
+    ldc = n
     if out is None:
         out = a_q.new_empty((m, n), dtype=out_dtype)
     elif out.shape != (m, n) or out.dtype != out_dtype or out.get_device() != dev \
             or (out.stride(1) != 1 and n > 1):
         raise ValueError(f"out must be a {out_dtype} [{m}, {n}] tensor with contiguous rows on "
                          f"{a_q.device}, got {out.dtype} {tuple(out.shape)} strides {out.stride()}")
+    elif m > 1:
+        ldc = out.stride(0)
     tile = ctypes.byref(_tile(config)) if config is not None else None
     if m == 0 or n == 0:
         return out
     # TMA reads rows that start on 16-byte boundaries; others are copied.
-    lda = a_q.stride(0) if m > 1 else half
-    if a_q.data_ptr() % 16 or lda % 16 or lda < half or a_q.stride(1) != 1:
+    ap, wp = a_q.data_ptr(), b_q.data_ptr()
+    if ap % 16 or lda % 16 or lda < half or unit_a != 1:
         a_q = a_q.clone(memory_format=torch.contiguous_format)
-        lda = half
-    wp, ldw = b_q.data_ptr(), b_q.stride(1) if n > 1 else half
-    if wp % 16 or ldw % 16 or ldw < half or b_q.stride(0) != 1:
+        ap, lda = a_q.data_ptr(), half
+    if wp % 16 or ldw % 16 or ldw < half or unit_b != 1:
         w = _copied(b_q.t(), "b_q")
         wp, ldw = w.data_ptr(), half
-    _native.on_device(dev, _native.load().i8l_w4a4_mm, a_q.data_ptr(), lda, sa.data_ptr(), wp, ldw,
-                      sb.data_ptr(), bias_ptr, bias_code, out.data_ptr(), _FLOAT[out_dtype], out.stride(0) if m > 1 else n, m, n, k,
-                      tile, current_stream(dev))
+    _native.on_device(dev, _native.load().i8l_w4a4_mm, ap, lda, sa.data_ptr(), wp, ldw, sb.data_ptr(), bias_ptr,
+                      bias_code, out.data_ptr(), _FLOAT[out_dtype], ldc, m, n, k, tile, current_stream(dev))
     return out
 
 
