@@ -322,7 +322,8 @@ constexpr int kPairBufBytes = 4096;  // an epilogue warp's staging: 32 rows of 1
 constexpr int kPairStaging = kPairEpi * kPairBufBytes;
 
 // Weight rows of the two kinds of tile; each CTA holds half of a tile's rows.  Along N they
-// take turns: 256 rows, 192, 256, ...
+// take turns: 256 rows, 192, 256, ...  Both are multiples of 64, so that a tile's scales begin
+// at an even TMEM column: the MMA's scale address takes no odd one.
 constexpr int kWide = 256, kNarrow = 192, kBoth = kWide + kNarrow;
 constexpr int kPairSfGroups = 3;  // 128-row scale groups that a tile's rows can lie in
 constexpr int kPairXBytes = kMxRows * kMxRowBytes;
@@ -486,61 +487,61 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
   int kind, tm, n0;
   if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t pol = policy_evict_last();
-      // Every load of a stage, of both CTAs, is counted on the even CTA's barrier.
-      auto load_w = [&](int st, int kb) {
-        if (leader)
-          mbar_arrive_expect_tx(&full[st], 2u * (kPairStageBytes - (kind ? (kWide - kNarrow) / 2 * kMxRowBytes : 0)));
-        const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
-        const int half = (kind ? kNarrow : kWide) / 2;
-        tma_load_2d_pair(sy + st * kPairYBytes, kind ? &map_narrow : &map_wide, bar, kb * kMxRowBytes,
-                         n0 + rank * half, pol);
-        tma_load_2d_pair(ssy + st * kPairSfGroups * kSfStageBytes, &map_sfy, bar, kb * 2 * kSfWords, n0 / 128, pol);
-      };
-      auto load_a = [&](int st, int kb) {
-        const uint32_t bar = map_to_rank(smem_u32(&full[st]), 0);
-        tma_load_2d_pair(sx + st * kPairXBytes, &map_x, bar, kb * kMxRowBytes, (2 * tm + rank) * kMxRows, pol);
-        tma_load_2d_pair(ssx + st * kSfStageBytes, &map_sfx, bar, kb * 2 * kSfWords, 2 * tm + rank, pol);
-      };
-      PairWalk walk;
-      bool more = walk.next(a, kind, tm, n0);
-      // The first tile's weight stages do not wait for the previous kernel.
-      int pre = 0;
-      if (more)
-        for (; pre < min(S, a.kblocks); ++pre) load_w(pre, pre);
-      pdl_wait();
-      bool ok = true;
-      int st = 0;
-      uint32_t phase = 0;
-      long long issued = 0;
-      for (; ok && more; more = walk.next(a, kind, tm, n0)) {
-        for (int kb = 0; kb < a.kblocks; ++kb) {
-          if (issued >= pre) {
-            if (!mbar_wait_bounded(&empty[st], phase ^ 1u, abort_flag, a.status, kStatusProducerWait)) {
-              ok = false;
-              break;
-            }
-            load_w(st, kb);
-          }
-          load_a(st, kb);
-          ++issued;
-          if (++st == S) {
-            st = 0;
-            phase ^= 1u;
-          }
+    // The whole warp runs the producer's loop, one elected lane issues (see elect_one).  Every
+    // load of a stage, of both CTAs, is counted on the even CTA's barrier.
+    const uint32_t elected = elect_one(), arms = leader ? elected : 0u;
+    const uint64_t pol = policy_evict_last();
+    const uint32_t x0 = smem_u32(sx), y0 = smem_u32(sy), sfx0 = smem_u32(ssx), sfy0 = smem_u32(ssy);
+    const uint32_t full0 = smem_u32(full), bar0 = map_to_rank(full0, 0);
+    auto load_w = [&](int st, int kb) {
+      mbar_expect_tx_elected(arms, full0 + 8 * st,
+                             2u * (kPairStageBytes - (kind ? (kWide - kNarrow) / 2 * kMxRowBytes : 0)));
+      tma_load_2d_pair_elected(elected, y0 + st * kPairYBytes, kind ? &map_narrow : &map_wide, bar0 + 8 * st,
+                               kb * kMxRowBytes, n0 + rank * ((kind ? kNarrow : kWide) / 2), pol);
+      tma_load_2d_pair_elected(elected, sfy0 + st * kPairSfGroups * kSfStageBytes, &map_sfy, bar0 + 8 * st,
+                               kb * 2 * kSfWords, n0 / 128, pol);
+    };
+    auto load_a = [&](int st, int kb) {
+      tma_load_2d_pair_elected(elected, x0 + st * kPairXBytes, &map_x, bar0 + 8 * st, kb * kMxRowBytes,
+                               (2 * tm + rank) * kMxRows, pol);
+      tma_load_2d_pair_elected(elected, sfx0 + st * kSfStageBytes, &map_sfx, bar0 + 8 * st, kb * 2 * kSfWords,
+                               2 * tm + rank, pol);
+    };
+    PairWalk walk;
+    bool more = walk.next(a, kind, tm, n0);
+    // The first tile's weight stages do not wait for the previous kernel.
+    int pre = 0;
+    if (more)
+      for (; pre < min(S, a.kblocks); ++pre) load_w(pre, pre);
+    pdl_wait();
+    bool ok = true;
+    int st = 0;
+    uint32_t phase = 0;
+    int issued = 0;  // up to S
+    for (; ok && more; more = walk.next(a, kind, tm, n0)) {
+      for (int kb = 0; kb < a.kblocks; ++kb) {
+        if (issued >= pre) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], phase ^ 1u, abort_flag, a.status, kStatusProducerWait));
+          if (!ok) break;
+          load_w(st, kb);
+        }
+        load_a(st, kb);
+        issued = min(issued + 1, S);
+        if (++st == S) {
+          st = 0;
+          phase ^= 1u;
         }
       }
-      if (!ok && leader) {
-        // Let the loads already issued land; the odd CTA stays until the even one leaves.
-        for (long long i = 0; i < (issued < S ? issued : S); ++i) {
-          if (--st < 0) {
-            st = S - 1;
-            phase ^= 1u;
-          }
-          volatile int no_abort = 0;
-          mbar_wait_bounded(&full[st], phase, &no_abort, a.status, kStatusDrainWait);
+    }
+    if (!ok && leader) {
+      // Let the loads already issued land; the odd CTA stays until the even one leaves.
+      for (int i = 0; i < issued; ++i) {
+        if (--st < 0) {
+          st = S - 1;
+          phase ^= 1u;
         }
+        volatile int no_abort = 0;
+        mbar_wait_bounded(&full[st], phase, &no_abort, a.status, kStatusDrainWait);
       }
     }
   } else if (warp == 1) {

@@ -160,6 +160,25 @@ __device__ __forceinline__ void single_half_stage(uint32_t elected, uint32_t d, 
         : "memory");
 }
 
+// A pair's TMA load (tma_load_2d_pair) and the arming of its barrier, likewise from a converged
+// warp with one elected lane.
+__device__ __forceinline__ void tma_load_2d_pair_elected(uint32_t elected, uint32_t dst, const void *map,
+                                                         uint32_t bar_cluster, int32_t x, int32_t y, uint64_t policy) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "l"(policy), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_elected(uint32_t elected, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(elected)
+      : "memory");
+}
+
 // Arrive once when every tcgen05 operation this thread issued so far has completed: on this
 // CTA's mbarrier (its shared-memory address), or with kPair on those at the same offset in both CTAs of the pair.
 template <bool kPair>

@@ -90,7 +90,7 @@ def add_rmsnorm_quant_mxfp4(x: torch.Tensor, residual: torch.Tensor | None, weig
                                  or residual.get_device() != dev or (residual.stride(1) != 1 and k > 1)):
         raise ValueError("residual must match x in shape, dtype and device and have contiguous rows")
     q, s = _empty(x, m, k)
-    rout = x.new_empty((m, k)) if residual is not None else None
+    rout = torch.empty_like(x) if residual is not None else None
     if m and k:
         w = weight if weight.is_contiguous() else weight.contiguous()
         has = residual is not None
