@@ -165,11 +165,6 @@ __global__ void __launch_bounds__(kSplitThreads)
   const int kb0 = a.kblocks * rank / a.cluster, kb1 = a.kblocks * (rank + 1) / a.cluster;
 
   const uint64_t pol_w = policy_evict_first(), pol_a = policy_evict_last();
-  auto load_w = [&](int st, int kb) {
-    mbar_arrive_expect_tx(&full[st], L::kStageBytes);
-    tma_load_2d(sx + st * L::kXBytes, &map_x, &full[st], kb * kMxRowBytes, tx * kMxRows, pol_w);
-    tma_load_2d(ssx + st * kSfStageBytes, &map_sfx, &full[st], kb * 2 * kSfWords, tx, pol_w);
-  };
   const int pre = min(S, kb1 - kb0);
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
@@ -183,8 +178,13 @@ __global__ void __launch_bounds__(kSplitThreads)
     fence_proxy_async_smem();
     // The weight tiles of the first stages wait neither for the other warps nor for the
     // previous kernel.
-    for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
+    for (int i = 0; i < pre; ++i) {
+      mbar_arrive_expect_tx(&full[i], L::kStageBytes);
+      tma_load_2d(sx + i * L::kXBytes, &map_x, &full[i], (kb0 + i) * kMxRowBytes, tx * kMxRows, pol_w);
+      tma_load_2d(ssx + i * kSfStageBytes, &map_sfx, &full[i], (kb0 + i) * 2 * kSfWords, tx, pol_w);
+    }
   }
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
@@ -195,21 +195,26 @@ __global__ void __launch_bounds__(kSplitThreads)
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_launch_dependents();
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
+    // The whole warp runs the producer's loop, one elected lane issues (see elect_one).
+    const uint32_t elected = elect_one();
+    const uint32_t x0 = smem_u32(sx), y0 = smem_u32(sy), sfx0 = smem_u32(ssx), sfy0 = smem_u32(ssy),
+                   full0 = smem_u32(full);
     pdl_wait();
     bool ok = true;
     int issued = 0, st = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
       if (issued >= pre) {
-        if (!mbar_wait_bounded(&empty[st], phase ^ 1u, abort_flag, a.status, kStatusProducerWait)) {
-          ok = false;
-          break;
-        }
-        load_w(st, kb);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[st], phase ^ 1u, abort_flag, a.status, kStatusProducerWait));
+        if (!ok) break;
+        mbar_expect_tx_elected(elected, full0 + 8 * st, L::kStageBytes);
+        tma_load_2d_elected(elected, x0 + st * L::kXBytes, &map_x, full0 + 8 * st, kb * kMxRowBytes, tx * kMxRows, pol_w);
+        tma_load_2d_elected(elected, sfx0 + st * kSfStageBytes, &map_sfx, full0 + 8 * st, kb * 2 * kSfWords, tx, pol_w);
       }
-      tma_load_2d(sy + st * L::kYBytes, &map_y, &full[st], kb * kMxRowBytes, ty * TN, pol_a);
-      tma_load_2d(ssy + st * kSfStageBytes, &map_sfy, &full[st], kb * 2 * kSfWords, ty * TN / kMxRows, pol_a);
+      tma_load_2d_elected(elected, y0 + st * L::kYBytes, &map_y, full0 + 8 * st, kb * kMxRowBytes, ty * TN, pol_a);
+      tma_load_2d_elected(elected, sfy0 + st * kSfStageBytes, &map_sfy, full0 + 8 * st, kb * 2 * kSfWords,
+                          ty * TN / kMxRows, pol_a);
       ++issued;
       if (++st == S) {
         st = 0;

@@ -160,8 +160,8 @@ __device__ __forceinline__ void single_half_stage(uint32_t elected, uint32_t d, 
         : "memory");
 }
 
-// A pair's TMA load (tma_load_2d_pair) and the arming of its barrier, likewise from a converged
-// warp with one elected lane.
+// TMA loads (as tma_load_2d_pair and tma_load_2d) and the arming of their barriers, likewise
+// from a converged warp with one elected lane.
 __device__ __forceinline__ void tma_load_2d_pair_elected(uint32_t elected, uint32_t dst, const void *map,
                                                          uint32_t bar_cluster, int32_t x, int32_t y, uint64_t policy) {
   asm volatile(
@@ -169,6 +169,15 @@ __device__ __forceinline__ void tma_load_2d_pair_elected(uint32_t elected, uint3
       "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
       ".L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;\n\t}" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "l"(policy), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_elected(uint32_t elected, uint32_t dst, const void *map, uint32_t bar,
+                                                    int32_t x, int32_t y, uint64_t policy) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "l"(policy), "r"(elected)
       : "memory");
 }
 __device__ __forceinline__ void mbar_expect_tx_elected(uint32_t elected, uint32_t bar, uint32_t bytes) {
