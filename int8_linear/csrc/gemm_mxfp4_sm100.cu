@@ -717,16 +717,13 @@ constexpr int kHalfSmem = 233472 / 2 - 1024;
 
 static int split_stage_bytes(int tn) { return kMxRows * kMxRowBytes + tn * kMxRowBytes + 2 * kSfStageBytes; }
 
-// CTAs that share a split tile's K.  Doubled while they have SMs of their own and two stages
-// each, or, of a long K, half an SM and 14 stages each; four at most on 128-token tiles, whose
-// partial sums are the larger part of the work (us with c and 2c: 16 x 2048 x 2048 c = 4 5.1
-// and 5.4; 64 x 4096 x 14336 c = 4 11.4 and 12.4; 512 x 4096 x 14336 c = 1 24.7 and 21.8;
-// 128 x 2048 x 6144 c = 4 8.9 and 10.6).
-static int split_cluster(int64_t tiles, int kblocks, int sms, int tn) {
-  const int most = tn == 128 ? 4 : kMaxCluster;
+// CTAs that share a split tile's K: doubled, to four at most, while they have SMs of their own
+// and two stages each (us by CTAs: 16 x 2048 x 2048 4 5.1, 8 5.4; 64 x 2048 x 6144 4 7.3, 8
+// 7.8; 256 x 4096 x 14336, 64 tiles, 2 14.7, 4 16.7; 512 x 4096 x 14336, 128 tiles, 1 19.2,
+// 2 21.2).
+static int split_cluster(int64_t tiles, int kblocks, int sms) {
   int c = 1;
-  while (c < most && ((2 * c * tiles <= sms && kblocks >= 4 * c) || (2 * c * tiles <= 2 * sms && kblocks >= 28 * c)))
-    c *= 2;
+  while (c < 4 && 2 * c * tiles <= sms && kblocks >= 4 * c) c *= 2;
   return c;
 }
 
@@ -742,8 +739,8 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   auto count = [&](int tn) { return (static_cast<int64_t>(N) + kMxRows - 1) / kMxRows * ((static_cast<int64_t>(M) + tn - 1) / tn); };
   p->pair = t.split == 4;
   // Pairs where 128-token split tiles are more than the SMs (us by split tiles and by pairs:
-  // 128 x 12288 x 2048, 96 tiles, 9.4 and 10.0; 1024 x 2048 x 2048, 128 tiles, 8.8 and 9.6;
-  // 256 x 12288 x 2048, 192 tiles, 13.1 and 11.2).
+  // 128 x 12288 x 2048, 96 tiles, 9.4 and 9.9; 333 x 6144 x 4096, 144 tiles, 11.3 and 12.5;
+  // 256 x 12288 x 2048, 192 tiles, 11.6 and 11.0).
   if (t.split == 0 && t.tok_tile == 0 && M > 64) p->pair = count(128) > di.sms;
   if (p->pair) {
     if (t.split == 4 && (t.swap_ab || t.tok_tile != 128 || t.w_tile != kWide))
@@ -764,7 +761,7 @@ static int make_mx_plan(int M, int N, int K, const i8l_tile *tile, MxPlan *p) {
   if (t.tok_tile && (!t.swap_ab || t.w_tile != 128))
     return set_error(I8L_ENOTSUP, "token tiles of 4-bit products take w_tile 128 with swap_ab");
   const int64_t tiles = count(p->tn);
-  const int c = t.split == 1 ? 1 : t.cluster ? t.cluster : split_cluster(tiles, kblocks, di.sms, p->tn);
+  const int c = t.split == 1 ? 1 : t.cluster ? t.cluster : split_cluster(tiles, kblocks, di.sms);
   if (c < 1 || c > kMaxCluster || c > kblocks)
     return set_error(I8L_ENOTSUP, "cluster size %d outside [1, min(8, k-blocks=%d)]", c, kblocks);
   p->cluster = c;
