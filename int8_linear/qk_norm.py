@@ -24,7 +24,7 @@ __all__ = ["qk_norm_rope"]
 
 def _out(out: torch.Tensor | None, shape: tuple, like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
-        return like.new_empty(shape)
+        return like.new_empty(*shape)  # a tuple takes 0.4 us more
     if out.shape != shape or out.dtype != like.dtype or out.get_device() != like.get_device() \
             or out.stride(2) != 1 or out.stride(1) != shape[2]:
         raise ValueError(f"{name} must be a {like.dtype} {list(shape)} tensor on {like.device} whose heads "
@@ -55,9 +55,10 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     arguments.  R = 0 only normalises."""
     if qkv.dtype not in _ACT:
         raise NotSupported(f"activations must be bfloat16 or float16, got {qkv.dtype}")
-    if qkv.dim() != 2 or (qkv.stride(1) != 1 and qkv.shape[1] > 1):
+    shape, stride = qkv.shape, qkv.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise NotSupported("qkv must be a 2-D activation with contiguous rows")
-    m, width = qkv.shape
+    m, width = shape
     d, dev = q_weight.numel(), qkv.get_device()
     wdt = q_weight.dtype
     if wdt not in _WEIGHT or k_weight.dtype != wdt or k_weight.numel() != d or d == 0:
@@ -69,7 +70,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     if not (wide or positions.dtype == torch.int32) or positions.shape != (m,):
         raise ValueError(f"positions must be {m} int32 or int64 values, got {positions.dtype} "
                          f"{tuple(positions.shape)}")
-    if cos_sin.dim() != 2 or cos_sin.dtype not in _WEIGHT or cos_sin.shape[1] > d or cos_sin.shape[1] % 2:
+    angles = cos_sin.shape
+    if len(angles) != 2 or cos_sin.dtype not in _WEIGHT or angles[1] > d or angles[1] % 2:
         raise ValueError(f"cos_sin must be a bf16/fp16/fp32 [positions, even rot <= {d}] table, got "
                          f"{cos_sin.dtype} {tuple(cos_sin.shape)}")
     if dev < 0:
@@ -84,8 +86,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     wk = k_weight if k_weight.is_contiguous() else k_weight.contiguous()
     pos = positions if positions.is_contiguous() else positions.contiguous()
     table = cos_sin if cos_sin.is_contiguous() else cos_sin.contiguous()
-    length, rot = table.shape
-    _native.on_device(dev, _native.load().i8l_qk_norm_rope, qkv.data_ptr(), qkv.stride(0), _ACT[qkv.dtype],
+    length, rot = angles
+    _native.on_device(dev, _native.load().i8l_qk_norm_rope, qkv.data_ptr(), stride[0], _ACT[qkv.dtype],
                       wq.data_ptr(), wk.data_ptr(), _WEIGHT[wdt], eps, pos.data_ptr(), wide, table.data_ptr(),
                       _WEIGHT[table.dtype], length, q.data_ptr(), q.stride(0) if m > 1 else heads * d, k.data_ptr(),
                       k.stride(0) if m > 1 else kv_heads * d, m, heads,
