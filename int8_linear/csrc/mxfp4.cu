@@ -9,13 +9,14 @@
 // neighbouring lanes share a block (two shuffles), and the matrix is walked as one flat
 // list of eight-value vectors or of blocks.  All four kernels move each byte once and are
 // bound by HBM: at 8192 rows (inputs larger than L2) quant_mxfp4 and dequant_mxfp4 take 26 us
-// of 8192 values, the measured copy rate; SiLU takes 42 us of 6144 (84 %, the rest is its
-// arithmetic and 48 % occupancy) and the norm 40 of 4096 with a residual (84 %).
+// of 8192 values, the measured copy rate; SiLU takes 38 us of 6144 (92 %; its arithmetic is
+// what is left) and the norm 40 of 4096 with a residual (84 %).
 //
 // A 4-bit value next to the border between two steps flips on the last bit of y, so y is
 // computed to the bit: the norm's mean in float64, and SiLU in float32 with a second, exact
 // pass for the few values where the float32 error could change the rounding.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -89,11 +90,38 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 
 // ------------------------------------------------------------------ SiLU
 
-// float32(g / (1 + exp(-g)) * u) in float64: within 2^-50 of the exact value before its
-// one rounding.  Kept out of line: few values come here.
-__device__ __noinline__ float silu_mul_exact(float g, float u) {
-  const double gd = g;
-  return static_cast<float>(gd / (1.0 + exp(-gd)) * static_cast<double>(u));
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// ln(2)^k / k!
+__host__ __device__ constexpr double exp2_term(int k) { return k == 0 ? 1. : exp2_term(k - 1) * (0.6931471805599453 / k); }
+
+// float32(g / (1 + exp(-g)) * u) in float64, for g and u that are 16-bit values: within 2^-50
+// of the exact value before its one rounding.  exp(-g) = 2^n 2^r with n the nearest integer to
+// -g log2 e (adding 1.5 * 2^52 rounds to it and leaves it in the low bits) and 2^r its Taylor
+// sum up to r^13 (|r| <= 1/2: the rest is below 2^-56), summed in pairs of pairs; the
+// reciprocal is an approximation and two Newton steps.  g is held within +-690, beyond which
+// 1 + exp(-g) is 1 or the product below float32's range.  An infinite g comes out as an
+// infinity or a NaN, either of which makes its block NaN.  (With exp and a division the 4096 x
+// 6144 kernel took 0.6 us more.)
+__device__ __forceinline__ float silu_mul_exact(float g, float u) {
+  constexpr double kLog2e = 1.4426950408889634, kRest = 2.0355273740931033e-17, kRound = 6755399441055744.;
+  const double a = -static_cast<double>(fminf(fmaxf(g, -690.f), 690.f));
+  const double t = fma(a, kLog2e, kRound), n = t - kRound;
+  const double r = fma(a, kRest, fma(a, kLog2e, -n)), r2 = r * r, r4 = r2 * r2;
+  auto pair = [&](auto k) {
+    constexpr double lo = exp2_term(decltype(k)::value), hi = exp2_term(decltype(k)::value + 1);
+    return fma(r, hi, lo);
+  };
+  const double c0 = fma(pair(Int<2>{}), r2, pair(Int<0>{})), c4 = fma(pair(Int<6>{}), r2, pair(Int<4>{}));
+  const double c8 = fma(pair(Int<10>{}), r2, pair(Int<8>{})), c12 = pair(Int<12>{});
+  const double e = fma(fma(c12, r4, c8), r4 * r4, fma(c4, r4, c0));
+  const double d = fma(e, __hiloint2double((__double2loint(t) + 1023) << 20, 0), 1.);
+  double q;
+  asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(q) : "d"(d));
+  q = fma(q, fma(-d, q, 1.), q);
+  q = fma(q, fma(-d, q, 1.), q);
+  return static_cast<float>(static_cast<double>(g) * static_cast<double>(u) * q);
 }
 
 __device__ __forceinline__ float ex2_approx(float x) {
@@ -114,23 +142,26 @@ __device__ __noinline__ uint32_t silu_mul2_exact(uint32_t gw, uint32_t uw) {
   float g[2], u[2];
   unpack2<DT>(gw, g[0], g[1]);
   unpack2<DT>(uw, u[0], u[1]);
-#pragma unroll 1
-  for (int i = 0; i < 2; ++i) g[i] = g[i] == 0.f || u[i] == 0.f ? g[i] * u[i] : silu_mul_exact(g[i], u[i]);
+  const bool zero0 = g[0] == 0.f || u[0] == 0.f, zero1 = g[1] == 0.f || u[1] == 0.f;
+  if (zero0 && zero1) return pack2<DT>(g[0] * u[0], g[1] * u[1]);
+  g[0] = zero0 ? g[0] * u[0] : silu_mul_exact(g[0], u[0]);
+  g[1] = zero1 ? g[1] * u[1] : silu_mul_exact(g[1], u[1]);
   return pack2<DT>(g[0], g[1]);
 }
 
 // The same in float32, with `unsure` set where that does not settle the rounding.
 //
 // v = g * rcp(1 + 2^(-g log2 e)) * u.  In units of 2^-23 relative: the exponent's product and
-// its constant are off by 0.63 |g| at most, ex2.approx by 2, both damped by e/(1 + e) with
-// e = exp(-g), which is below 1 for g < 0 and below 1/2 (times |g|: below 0.3) for g > 0; the
-// sum and the two products add 1/2 each and rcp.approx 1.  So v is within 5 + 0.7 max(-g, 0)
-// of those units, with some margin, and y is right wherever both ends of that interval round
-// alike; about one bf16 value in 5000 is unsure.  Values near the end of float32's normal
-// range have no such relative bound and are unsure for bf16; for fp16 they are zero.
+// its constant are off by 0.61 |g| and ex2.approx by 2, both times s = e/(1 + e) with
+// e = exp(-g); the sum, the two products and the ends of the interval below add 1/2 each and
+// rcp.approx 1: 3 + (2 + 0.61 |g|) s.  For g > 0, s < 1/2 and |g| s < 0.28, so that is below
+// 4.2; for g = -1, -2, -3, -4 it is 4.9, 5.8, 6.7 and 7.4 and grows by 0.61 from there on.  So
+// v is within 4.25 + 0.83 max(-g, 0) of those units, and y is right wherever both ends of that
+// interval round alike; about one bf16 value in 4000 is unsure.  Where v is below float32's
+// normal range it has no such bound: see mx_tiny.
 template <int DT>
 __device__ __forceinline__ uint32_t silu_mul2(uint32_t gw, uint32_t uw, bool &unsure) {
-  constexpr float kUnit = 1.0f / 8388608.0f, kTiny = 1e-36f;
+  constexpr float kUnit = 1.0f / 8388608.0f;
   float g0, g1, u0, u1, p0, p1, d0, d1, v0, v1, e0, e1, l0, l1, h0, h1;
   unpack2<DT>(gw, g0, g1);
   unpack2<DT>(uw, u0, u1);
@@ -140,13 +171,21 @@ __device__ __forceinline__ uint32_t silu_mul2(uint32_t gw, uint32_t uw, bool &un
   mul2_rn(v0, v1, v0, v1, u0, u1);
   g0 = fminf(g0, 0.f);
   g1 = fminf(g1, 0.f);
-  fma2_rn(e0, e1, g0, g1, 0.7f * kUnit, 0.7f * kUnit, -5.0f * kUnit, -5.0f * kUnit);  // minus the bound
+  fma2_rn(e0, e1, g0, g1, 0.83f * kUnit, 0.83f * kUnit, -4.25f * kUnit, -4.25f * kUnit);  // minus the bound
   fma2_rn(l0, l1, v0, v1, e0, e1, v0, v1);
   fma2_rn(h0, h1, v0, v1, -e0, -e1, v0, v1);
   const uint32_t low = pack2<DT>(l0, l1), high = pack2<DT>(h0, h1);
   unsure = low != high;
-  if constexpr (DT == I8L_BF16) unsure = unsure || fminf(fabsf(v0), fabsf(v1)) < kTiny;
   return low;
+}
+
+// Whether a block's largest y is so small that values below float32's normal range may decide
+// its codes, from the magnitude's float32 bits.  In any other block such a value is far below
+// half a step and only its sign is stored, which is right.  (fp16 has no such values: what is
+// below float32's normal range rounds to zero.)
+template <int DT>
+__device__ __forceinline__ bool mx_tiny(uint32_t amax_bits) {
+  return DT == I8L_BF16 && amax_bits < (127u - 110u) << 23;
 }
 
 // ------------------------------------------------------------------ flat quantisers
@@ -213,11 +252,12 @@ __device__ __forceinline__ uint32_t mx_amax32(const uint32_t (&w)[16]) {
   return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
 }
 
-// Quantises a block that one thread holds and stores its codes and its scale.
+// Quantises a block that one thread holds, its largest magnitude given, and stores its codes
+// and its scale.
 template <int DT>
 __device__ __forceinline__ void store_block(const MxOut &o, int q16, long long row, int block, int blocks,
-                                            const uint32_t (&x)[16]) {
-  const uint32_t byte = mx_scale_byte(mx_amax32<DT>(x));
+                                            const uint32_t (&x)[16], uint32_t amax) {
+  const uint32_t byte = mx_scale_byte(amax);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -256,15 +296,16 @@ __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a
     if constexpr (kSilu) {
       const long long K = static_cast<long long>(a.blocks) * kMxBlock;
       const uint4 up = in ? load8_raw(a.x, at + K, a.vec) : make_uint4(0u, 0u, 0u, 0u);
-      auto settle = [](uint32_t &g, uint32_t u) {
+      const uint4 gate = x;
+      auto settle = [](uint32_t g, uint32_t u) {
         bool unsure;
         const uint32_t y = silu_mul2<DT>(g, u, unsure);
-        g = unsure ? silu_mul2_exact<DT>(g, u) : y;
+        return unsure ? silu_mul2_exact<DT>(g, u) : y;
       };
-      settle(x.x, up.x);
-      settle(x.y, up.y);
-      settle(x.z, up.z);
-      settle(x.w, up.w);
+      x = make_uint4(settle(gate.x, up.x), settle(gate.y, up.y), settle(gate.z, up.z), settle(gate.w, up.w));
+      if (mx_tiny<DT>(mx_amax8<DT>(x)))
+        x = make_uint4(silu_mul2_exact<DT>(gate.x, up.x), silu_mul2_exact<DT>(gate.y, up.y),
+                       silu_mul2_exact<DT>(gate.z, up.z), silu_mul2_exact<DT>(gate.w, up.w));
     }
     w = mx_quantise8<DT>(x, byte);
   }
@@ -281,12 +322,17 @@ __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a
 // by 32 values instead of 8.  The four-lanes-a-block kernel above was bound by instruction
 // issue (77 % of the slots, 111 instructions per 8 values, 50 % of HBM at 8192 x 8192), but
 // spreads a small matrix over four times as many threads.
+// Threads: 128 (4096 x 4096 7.6 us, with 64 9.7); with SiLU 64, as a CTA stays as long as the
+// last of its warps that has unsure values (4096 x 6144 22.0 us, with 128 22.8, with 32 26.4).
+template <bool kSilu>
+constexpr int kBlockThreads = kSilu ? 64 : 128;
+
 template <int DT, bool kSilu>
-__global__ void __launch_bounds__(kFlatThreads) mx_block_kernel(const FlatArgs a) {
+__global__ void __launch_bounds__(kBlockThreads<kSilu>) mx_block_kernel(const FlatArgs a) {
   static_assert(DT != I8L_F32, "16-bit values");
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t id = blockIdx.x * kFlatThreads + threadIdx.x;
+  const uint32_t id = blockIdx.x * kBlockThreads<kSilu> + threadIdx.x;
   const uint32_t total = a.vectors >> 2;
   if (id >= total) {
     if (id - total < a.pad_words) zero_pad_word(a.o, a.rows, id - total);
@@ -296,6 +342,7 @@ __global__ void __launch_bounds__(kFlatThreads) mx_block_kernel(const FlatArgs a
   const long long at = row * a.ldx + block * static_cast<long long>(kMxBlock);
   uint32_t x[16];
   load_block(a.x, at, a.vec, x);
+  uint32_t amax;
   if constexpr (kSilu) {
     uint32_t up[16];
     load_block(a.x, at + static_cast<long long>(a.blocks) * kMxBlock, a.vec, up);
@@ -308,18 +355,35 @@ __global__ void __launch_bounds__(kFlatThreads) mx_block_kernel(const FlatArgs a
       x[i] = silu_mul2<DT>(x[i], up[i], unsure);
       if (unsure) todo |= 1u << i;
     }
-    while (todo) {
-      const int i = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const uint16_t *g = static_cast<const uint16_t *>(a.x) + at + 2 * i;
-      const uint16_t *u = g + static_cast<long long>(a.blocks) * kMxBlock;
-      const uint32_t y = silu_mul2_exact<DT>(g[0] | (static_cast<uint32_t>(g[1]) << 16),
-                                             u[0] | (static_cast<uint32_t>(u[1]) << 16));
+    for (bool all = false;; all = true) {
+      while (todo) {
+        const int i = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const uint16_t *g = static_cast<const uint16_t *>(a.x) + at + 2 * i;
+        const uint16_t *u = g + static_cast<long long>(a.blocks) * kMxBlock;
+        const uint32_t y = silu_mul2_exact<DT>(g[0] | (static_cast<uint32_t>(g[1]) << 16),
+                                               u[0] | (static_cast<uint32_t>(u[1]) << 16));
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = j == i ? y : x[j];
+        for (int j = 0; j < 16; ++j) x[j] = j == i ? y : x[j];
+      }
+      amax = mx_amax32<DT>(x);
+      if (all || !mx_tiny<DT>(amax)) break;
+      // Zero rows, as padding has them, need no second look (4096 x 6144 zeros 101 us with it).
+      uint32_t g[16], any_g = 0u, any_u = 0u;
+      load_block(a.x, at, a.vec, g);
+      load_block(a.x, at + static_cast<long long>(a.blocks) * kMxBlock, a.vec, up);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        any_g |= g[i];
+        any_u |= up[i];
+      }
+      if (((any_g & 0x7fff7fffu) == 0u) || ((any_u & 0x7fff7fffu) == 0u)) break;
+      todo = 0xffffu;
     }
+  } else {
+    amax = mx_amax32<DT>(x);
   }
-  store_block<DT>(a.o, a.q16, row, static_cast<int>(block), a.blocks, x);
+  store_block<DT>(a.o, a.q16, row, static_cast<int>(block), a.blocks, x, amax);
 }
 
 // ------------------------------------------------------------------ add + RMSNorm
@@ -510,7 +574,7 @@ __global__ void __launch_bounds__(256) mx_norm_block_kernel(const MxNormArgs a) 
       x[4 * v + i / 2] = pack2<DT>(n0, n1);
     }
   }
-  store_block<DT>(a.o, a.q16, row, block, blocks, x);
+  store_block<DT>(a.o, a.q16, row, block, blocks, x, mx_amax32<DT>(x));
 }
 
 // ------------------------------------------------------------------ dequantisation
@@ -636,17 +700,18 @@ int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uin
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err;
     // A thread per block from 256 blocks an SM on (SiLU: 512); with fewer, four lanes a block
-    // finish sooner (us by threads and by lanes: 18944 blocks 1.88 and 1.80, 75776 2.28 and
-    // 3.12, 303104 4.19 and 10.6; SiLU 37888 4.09 and 3.91, 151552 6.88 and 7.53).
+    // finish sooner (us by threads and by lanes: 18944 blocks 1.85 and 1.77, 75776 2.27 and
+    // 3.18, 151552 2.8 and 5.7; SiLU 37888 3.6 and 3.3, 56832 4.1 and 4.1, 75776 4.5 and 4.7).
     const int64_t total = a.vectors / 4;
     if (dtype != I8L_F32 && total >= (kSilu ? 512 : 256) * di.sms) {
       if (a.vec && reinterpret_cast<uintptr_t>(x) % 32 == 0 && (ldx * 2) % 32 == 0) a.vec = 2;
       a.per_row = FastDiv(blocks);
-      const dim3 grid(static_cast<unsigned>((total + a.pad_words + kFlatThreads - 1) / kFlatThreads));
+      constexpr int kThreads = kBlockThreads<kSilu>;
+      const dim3 grid(static_cast<unsigned>((total + a.pad_words + kThreads - 1) / kThreads));
       if (dtype == I8L_BF16)
-        err = launch(mx_block_kernel<I8L_BF16, kSilu>, grid, dim3(kFlatThreads), 0, s, 1, a);
+        err = launch(mx_block_kernel<I8L_BF16, kSilu>, grid, dim3(kThreads), 0, s, 1, a);
       else
-        err = launch(mx_block_kernel<I8L_F16, kSilu>, grid, dim3(kFlatThreads), 0, s, 1, a);
+        err = launch(mx_block_kernel<I8L_F16, kSilu>, grid, dim3(kThreads), 0, s, 1, a);
     } else {
       a.per_row = FastDiv(blocks * 4u);
       const int64_t work = static_cast<int64_t>(a.vectors) + a.pad_words;

@@ -305,17 +305,19 @@ __device__ __forceinline__ uint32_t pack2(float v0, float v1) {
 // are ordered as their bits are, NaN and infinity last, so the maximum is taken two at a
 // time on the bits.
 template <int DT>
-__device__ __forceinline__ uint32_t mx_quantise8(const uint4 &w, uint32_t &byte) {
+__device__ __forceinline__ uint32_t mx_amax8(const uint4 &w) {
   constexpr uint32_t kAbs = 0x7fff7fffu;
   uint32_t m = __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs), __vmaxu2(w.z & kAbs, w.w & kAbs));
   m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
   m = max(m & 0xffffu, m >> 16);
-  if constexpr (DT == I8L_BF16)
-    m <<= 16;
-  else
-    m = __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
-  byte = mx_scale_byte(m);
+  if constexpr (DT == I8L_BF16) return m << 16;
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t mx_quantise8(const uint4 &w, uint32_t &byte) {
+  byte = mx_scale_byte(mx_amax8<DT>(w));
   float y[8];
   unpack2<DT>(w.x, y[0], y[1]);
   unpack2<DT>(w.y, y[2], y[3]);

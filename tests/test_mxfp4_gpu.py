@@ -219,6 +219,44 @@ def test_silu_of_all_gates(act):
         check(*mxfp4.silu_mul_quant_mxfp4(gu), om.silu_rows(np_(gu), DT[act]))
 
 
+@pytest.mark.parametrize("lo", [0, 16, 8, 1])
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+def test_silu_of_large_batches(act, lo):
+    """Enough blocks for the kernel with a thread per block, at each alignment of its loads."""
+    gu = rand((401, 2 * 6144 + 32), 3, 2.0, dtype=act)[:, lo:lo + 2 * 6144]
+    check(*mxfp4.silu_mul_quant_mxfp4(gu), om.silu_rows(np_(gu), DT[act]))
+
+
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+def test_silu_of_all_gates_in_a_large_batch(act):
+    """Every 16-bit gate in the kernel with a thread per block, against ups from zero over the
+    smallest to the largest: blocks of zeros, blocks whose values all lie below float32's
+    normal range, and such values beside normal ones."""
+    gates = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(act).view(-1, 32)
+    top = 126 if act == torch.bfloat16 else 15
+    ups = [0.0, -0.0, *(1.3125 * 2.0**e * (-1) ** e for e in torch.linspace(-top, top, 36).round().int().tolist())]
+    rows = []
+    for i, up in enumerate(ups):
+        u = torch.full(gates.shape, up, dtype=torch.float64)
+        if i % 3 == 0:
+            u[:, 1::2] *= 2.0**-20
+        rows.append(torch.cat([gates, u.to(act)], 1))
+    gu = torch.cat(rows).cuda()
+    assert gu.shape[0] >= 512 * torch.cuda.get_device_properties(0).multi_processor_count
+    check(*mxfp4.silu_mul_quant_mxfp4(gu), om.silu_rows(np_(gu), DT[act]))
+
+
+@pytest.mark.parametrize("rows", [20, 410])
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+def test_silu_of_padded_batches(act, rows):
+    """Rows of zeros, of zero gates and of zero ups, by turns with others."""
+    gu = rand((rows, 2 * 6144), 5, 2.0, dtype=act)
+    gu[1::4] = 0.0
+    gu[2::4, :6144] = -0.0
+    gu[3::4, 6144:] = 0.0
+    check(*mxfp4.silu_mul_quant_mxfp4(gu), om.silu_rows(np_(gu), DT[act]))
+
+
 def test_empty_batches():
     for k in (0, 64):
         q, s = mxfp4.quant_mxfp4(torch.empty((0, k), dtype=torch.bfloat16, device="cuda"))
