@@ -10,7 +10,7 @@
 // list of eight-value vectors or of blocks.  All four kernels move each byte once and are
 // bound by HBM: at 8192 rows (inputs larger than L2) quant_mxfp4 and dequant_mxfp4 take 26 us
 // of 8192 values, the measured copy rate; SiLU takes 38 us of 6144 (92 %; its arithmetic is
-// what is left) and the norm 40 of 4096 with a residual (84 %).
+// what is left) and the norm 39 of 4096 with a residual (86 %).
 //
 // A 4-bit value next to the border between two steps flips on the last bit of y, so y is
 // computed to the bit: the norm's mean in float64, and SiLU in float32 with a second, exact
@@ -399,16 +399,57 @@ struct MxNormArgs {
   long long ldro;
   MxOut o;
   int rows, K;
-  double eps;
+  double inv_k, eps;
   uint32_t pad_words;
   int vec;  // 1: 16-byte loads and stores allowed, 2: 32-byte ones
   int q16;  // 16-byte stores of codes allowed
 };
 
-// One row per CTA, the row in registers.  The squares are summed in float64 (a float32
-// squares exactly into one) and 1/sqrt(mean + eps) is rounded once to float32, so the factor
-// does not depend on the order of the sum; the first warp computes it for the row, as the
-// square root and the division are worth a vector's arithmetic to each thread.
+// sum + x^2 in float64, which holds a float32's square exactly.  kFast: the float64 is put
+// together from x's bits, an integer multiplication, as the conversion unit is slow (8192 rows of
+// 4096 39.5 us with it, 38.8 so); infinities, NaN, zeros and values below float32's normal range
+// come out as others, which plain_sum tells from the row's sum.
+template <bool kFast>
+__device__ __forceinline__ double add_square(double sum, float x) {
+  const double d = kFast ? __longlong_as_double(static_cast<long long>(
+                               static_cast<unsigned long long>(__float_as_uint(x) & 0x7fffffffu) * 0x20000000ull +
+                               0x3800000000000000ull))
+                         : static_cast<double>(x);
+  return fma(d, d, sum);
+}
+
+// Whether a sum from add_square<true> is that of the values.  An infinity or NaN puts it above
+// 2^255; the value that stands for a zero or a smaller one is below 2^-126, so that 2^18 of
+// their squares change a sum from 2^-180 on by less than 2^-53 of it.
+__device__ __forceinline__ bool plain_sum(double sum) { return sum > 0x1p-180 && sum < 0x1p255; }
+
+// The sum of every thread's `sum`, for CTAs of at most eight warps.
+__device__ __forceinline__ double cta_sum(double sum, double *red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  double part[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[i] = i < static_cast<int>(blockDim.x >> 5) ? red[i] : 0.0;
+  return ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+}
+
+// float32(1 / sqrt(m)): an approximation and two Newton steps, within 2^-51 before the
+// rounding, so that every thread of a row has it sooner than one could hand it round.
+__device__ __forceinline__ float norm_factor(double m) {
+  double r;
+  asm("rsqrt.approx.ftz.f64 %0, %1;" : "=d"(r) : "d"(m));
+  if (m >= 0x1p-1022 && m < 0x1p1023) {  // not zero, an infinity or NaN
+    r = fma(0.5 * r, fma(-m * r, r, 1.), r);
+    r = fma(0.5 * r, fma(-m * r, r, 1.), r);
+  }
+  return static_cast<float>(r);
+}
+
+// One row per CTA, the row in registers.  The squares are summed in float64 and
+// 1/sqrt(mean + eps) is rounded once to float32, so the factor does not depend on the order of
+// the sum.
 template <int DT, int WDT, int NV>
 __global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) {
   pdl_launch_dependents();
@@ -420,8 +461,7 @@ __global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) 
     if (i < a.pad_words) zero_pad_word(a.o, a.rows, i);
     return;
   }
-  __shared__ double red[32];
-  __shared__ float factor;
+  __shared__ double red[8];
   uint4 xr[NV], rr[NV];
   float h[NV][8];
 #pragma unroll
@@ -454,23 +494,10 @@ __global__ void __launch_bounds__(256) mx_norm_quant_kernel(const MxNormArgs a) 
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double d = h[v][i];
-      ss = fma(d, d, ss);
-    }
+    for (int i = 0; i < 8; ++i) ss = add_square<false>(ss, h[v][i]);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    ss = threadIdx.x < blockDim.x >> 5 ? red[threadIdx.x] : 0.0;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);  // at most 8 warps
-    if (threadIdx.x == 0) factor = static_cast<float>(1.0 / sqrt(ss / a.K + a.eps));
-  }
-  __syncthreads();
-  const float rs = factor;
+  ss = cta_sum(ss, red);
+  const float rs = norm_factor(fma(ss, a.inv_k, a.eps));
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int col = col_of<8>(v);
@@ -508,7 +535,6 @@ __global__ void __launch_bounds__(256) mx_norm_block_kernel(const MxNormArgs a) 
     return;
   }
   __shared__ double red[8];
-  __shared__ float factor;
   const int blocks = a.K / kMxBlock, block = static_cast<int>(threadIdx.x);
   const bool in = block < blocks;
   uint32_t x[16], r[16];
@@ -529,9 +555,8 @@ __global__ void __launch_bounds__(256) mx_norm_block_kernel(const MxNormArgs a) 
       add2_rn(h[2 * i], h[2 * i + 1], h[2 * i], h[2 * i + 1], r0, r1);
       r[i] = pack2<DT>(h[2 * i], h[2 * i + 1]);
     }
-    const double d0 = h[2 * i], d1 = h[2 * i + 1];
-    ss = fma(d0, d0, ss);
-    ss1 = fma(d1, d1, ss1);
+    ss = add_square<true>(ss, h[2 * i]);
+    ss1 = add_square<true>(ss1, h[2 * i + 1]);
   }
   if (in && a.res) {
     T *p = static_cast<T *>(a.rout) + row * a.ldro + block * kMxBlock;
@@ -547,20 +572,16 @@ __global__ void __launch_bounds__(256) mx_norm_block_kernel(const MxNormArgs a) 
       for (int i = 0; i < 32; ++i) p[i] = ActType<DT>::from_f32(h[i]);
     }
   }
-  ss += ss1;
+  ss = cta_sum(ss + ss1, red);
+  if (!plain_sum(ss)) {
+    __syncthreads();  // `red` has been read
+    ss = 0.0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    ss = threadIdx.x < blockDim.x >> 5 ? red[threadIdx.x] : 0.0;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (threadIdx.x == 0) factor = static_cast<float>(1.0 / sqrt(ss / a.K + a.eps));
+    for (int i = 0; i < 32; ++i) ss = add_square<false>(ss, h[i]);
+    ss = cta_sum(ss, red);
   }
-  __syncthreads();
   if (!in) return;
-  const float rs = factor;
+  const float rs = norm_factor(fma(ss, a.inv_k, a.eps));
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     float w[8];
@@ -798,6 +819,7 @@ extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const voi
   a.o = MxOut{q, ldq, scale, ktiles};
   a.rows = M;
   a.K = K;
+  a.inv_k = 1.0 / K;
   a.eps = eps;
   a.pad_words = static_cast<uint32_t>((128 - M % 128) % 128) * ktiles;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -805,10 +827,11 @@ extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const voi
   a.q16 = aligned16(q) && ldq % 16 == 0 ? 1 : 0;
   DeviceInfo di;
   if (int e = device_info(&di)) return e;
-  // A block per thread from 16 rows an SM on; fewer rows finish sooner spread over four times
-  // the threads (us by block and by vector: 592 rows of 2048 3.77 and 3.57, 1184 rows of 4096
-  // 8.22 and 8.02, 2368 rows of 4096 14.1 and 14.6).
-  const bool blocks = M >= 16 * di.sms && K <= 8192;
+  // A block per thread from 384 of them an SM on; fewer finish sooner spread over four times the
+  // threads, and so do rows that leave half a warp idle (us by block and by vector: 592 rows of
+  // 2048 3.6 and 3.5, 888 4.1 and 4.4; 296 rows of 4096 3.8 and 3.9, 1184 7.2 and 8.0; 8192
+  // rows of 512 10.5 and 9.3, of 1024 12.2 and 13.7).
+  const bool blocks = static_cast<int64_t>(M) * K >= 384 * kMxBlock * static_cast<int64_t>(di.sms) && K >= 1024 && K <= 8192;
   if (blocks && vec) {
     auto wide = [](const void *p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 32 == 0 && ld % 16 == 0; };
     if (wide(x, ldx) && (!residual || (wide(residual, ldr) && wide(rout, ldro)))) a.vec = 2;

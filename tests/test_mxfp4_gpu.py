@@ -193,6 +193,30 @@ def test_norm_of_special_rows():
     assert np.isnan(back[4]).all() and np.isnan(back[5]).any()
 
 
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+@pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k", [(40, 2048), (1900, 1024), (1200, 4096), (300, 8192)])
+def test_norm_of_special_rows_among_others(m, k, act, eps):
+    """Zeros, infinities, NaN, values whose squares leave float32's range and values below its
+    normal range, in rows by themselves and beside ordinary ones, in small and large batches.
+    Without eps the factor of a row of zeros or of the smallest values is infinite."""
+    x, r = rand((m, k), 1, dtype=act), rand((m, k), 2, dtype=act)
+    big, small, least = (3e38, 1e-30, 1e-39) if act == torch.bfloat16 else (65504.0, 1e-5, 6e-8)
+    fills = [0.0, -0.0, big, -small, least, float("inf"), float("nan")]
+    for i, v in enumerate(fills):
+        x[i::17], r[i::17] = v, 0.0  # whole rows
+        x[i + 7::17, i * 31 % k] = v  # one value
+    x[14::17, ::3], r[14::17] = 0.0, 0.0
+    x[15::17], r[15::17] = small, -small  # a sum of zero
+    w = rand((k,), 3, 0.1, act) + 1.0
+    for res in (None, r):
+        q, s, rout = mxfp4.add_rmsnorm_quant_mxfp4(x, res, w, eps)
+        y, r0 = om.norm_rows(np_(x), None if res is None else np_(r), np_(w), eps, DT[act], DT[act])
+        check(q, s, y)
+        if res is not None:
+            assert np.array_equal(np_(rout), r0, equal_nan=True)
+
+
 @pytest.mark.parametrize("m,k", [(1, 32), (1, 6144), (33, 1056), (8, 14336), (300, 6144)])
 @pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
 def test_silu_mul_quant(m, k, act):
