@@ -11,11 +11,13 @@
 // are rotated with one another: values 8c.. and rot/2 + 8c.. (or, interleaved, two chunks in
 // a row), so that a lane needs eight angles and nothing from another lane but the sum of
 // squares, a butterfly over the group.  (With neighbouring values in a lane and the pairs'
-// other halves shuffled, the kernel took 42 us where this takes 36, 8192 tokens x 40 heads
-// of 128.)  A group takes up to P neighbouring heads of one token: their loads are all in
-// flight together, and the token's angles are read once for them.  The kernel reads and
-// writes each value once: 36 us is 72 % of the measured copy rate, with the latency of a
-// group's loads (position, then angles) at 31 % occupancy as what is left.
+// other halves shuffled, the kernel took 42 us where it then took 36, 8192 tokens x 40 heads of
+// 128.)  In a large batch a group of lanes takes two neighbouring heads of one token, which
+// share its angles, and has the next two on their way meanwhile: with the latency of position,
+// then angles, and 31 % occupancy the kernel waited for loads a third of its time without.
+// It reads and writes each value once: 32 us is 80 % of the measured copy rate.  Heads a group
+// and CTAs an SM otherwise (4096 tokens; 15.6 us so): 2 and 6 16.3, 2 and 7 18.9, 3 and 5 17.6,
+// 4 and 4 16.6, 1 and 8 26.9; a CTA per four heads without the loop 17.5.
 #include <algorithm>
 
 #include "common.cuh"
@@ -26,7 +28,8 @@
 namespace i8l {
 
 constexpr int kQkThreads = 128;
-constexpr int kQkHeads = 4;  // heads per group in a large batch
+constexpr int kQkHeads = 2;  // heads per group in a large batch
+constexpr int kQkCtas = 5;   // CTAs per SM then
 
 struct QkArgs {
   const void *qkv;
@@ -51,120 +54,141 @@ struct QkArgs {
   int w_vec, cs_vec;
 };
 
-// G lanes per head (a power of two, G * 16 >= dim), P heads per group.  In place is fine: a
-// lane stores the elements that it alone loaded.
-template <int DT, int G, int P>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a) {
+// G lanes per head (a power of two, G * 16 >= dim), P heads per group.  With kLoop the grid
+// covers the GPU once and a CTA goes on to further groups.  In place is fine: a lane stores the
+// elements that it alone loaded.
+template <int DT, int G, int P, bool kLoop>
+__global__ void __launch_bounds__(kQkThreads, kLoop ? kQkCtas : 1) qk_norm_rope_kernel(const QkArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   using T = typename ActType<DT>::T;
-  const uint32_t group = blockIdx.x * (kQkThreads / G) + threadIdx.x / G;
+  constexpr uint32_t kGroups = kQkThreads / G;
   const int lane = threadIdx.x % G;
-  const bool live = group < a.groups;
-  const long long token = live ? a.per_token.div(group) : 0;
-  const int part = live ? static_cast<int>(group - static_cast<uint32_t>(token) * a.parts) : 0;
   const int half = a.rot / 2;
   // The lane's chunks begin at c0 and c1; what lies behind the rotated values follows in order.
   const bool split = !a.interleaved && lane < a.rot / 16;
   const int c0 = split ? 8 * lane : 16 * lane, c1 = split ? half + 8 * lane : 16 * lane + 8;
-  const bool has0 = live && c0 < a.dim, has1 = live && c1 < a.dim;
-  const int all = a.heads + a.kv_heads, head0 = part * P;
-  const T *src = static_cast<const T *>(a.qkv) + token * a.ld + static_cast<long long>(head0) * a.dim;
-  uint4 raw[P][2];
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const bool in = head0 + i < all;
-    raw[i][0] = in && has0 ? *reinterpret_cast<const uint4 *>(src + i * a.dim + c0) : make_uint4(0u, 0u, 0u, 0u);
-    raw[i][1] = in && has1 ? *reinterpret_cast<const uint4 *>(src + i * a.dim + c1) : make_uint4(0u, 0u, 0u, 0u);
-  }
+  const bool has0 = c0 < a.dim, has1 = c1 < a.dim;
+  const int all = a.heads + a.kv_heads;
 
-  long long pos = 0;
-  if (live)
-    pos = a.pos64 ? static_cast<const long long *>(a.positions)[token] : static_cast<const int *>(a.positions)[token];
-  // A position outside the table has no angles: the token's heads come out as NaN.
-  const bool known = a.rot == 0 || (pos >= 0 && pos < a.max_pos);
-  // Angles 8 lane .. 8 lane + 7; those past the last are none.
-  float cs[8], sn[8];
+  // A group's values and its token's position.
+  struct Group {
+    uint4 raw[P][2];
+    long long token, pos;
+    int head0;  // `all` behind the last group
+  } next;
+  auto fetch = [&](uint32_t id) {
+    const bool in = id < a.groups;
+    next.token = in ? a.per_token.div(id) : 0;
+    next.head0 = in ? static_cast<int>(id - static_cast<uint32_t>(next.token) * a.parts) * P : all;
+    const T *src = static_cast<const T *>(a.qkv) + next.token * a.ld + static_cast<long long>(next.head0) * a.dim;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-  }
-  if (has0 && known && 8 * lane < half) {
-    const uint8_t *table = static_cast<const uint8_t *>(a.cos_sin) + pos * a.rot * (a.cs_dtype == I8L_F32 ? 4 : 2);
-    if (8 * lane + 8 <= half) {
-      load_weight_vec<8>(table, a.cs_dtype, 8 * lane, a.cs_vec != 0, cs);
-      load_weight_vec<8>(table, a.cs_dtype, half + 8 * lane, a.cs_vec != 0, sn);
-    } else {  // interleaved, and four angles left
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cs[i] = load_weight(table, a.cs_dtype, 8 * lane + i);
-        sn[i] = load_weight(table, a.cs_dtype, half + 8 * lane + i);
-      }
+    for (int i = 0; i < P; ++i) {
+      const bool here = next.head0 + i < all;
+      next.raw[i][0] = here && has0 ? *reinterpret_cast<const uint4 *>(src + i * a.dim + c0) : make_uint4(0u, 0u, 0u, 0u);
+      next.raw[i][1] = here && has1 ? *reinterpret_cast<const uint4 *>(src + i * a.dim + c1) : make_uint4(0u, 0u, 0u, 0u);
     }
-  }
+    next.pos = 0;
+    if (in)
+      next.pos = a.pos64 ? static_cast<const long long *>(a.positions)[next.token]
+                         : static_cast<const int *>(a.positions)[next.token];
+  };
 
+  uint32_t id = blockIdx.x * kGroups + threadIdx.x / G;
+  fetch(id);
   float w[16] = {};
   int loaded = -1;  // which weight `w` holds: 0 queries, 1 keys
+  // Whole warps take part in every turn, for their shuffles.
+  for (uint32_t first = blockIdx.x * kGroups; first < a.groups; first += gridDim.x * kGroups) {
+    const Group now = next;
+    // A position outside the table has no angles: the token's heads come out as NaN.
+    const bool known = a.rot == 0 || (now.pos >= 0 && now.pos < a.max_pos);
+    // Angles 8 lane .. 8 lane + 7; those past the last are none.
+    float cs[8], sn[8];
 #pragma unroll
-  for (int turn = 0; turn < P; ++turn) {
-    const int head = head0 + turn;
-    const bool here = live && head < all;
-    const int key = head >= a.heads ? 1 : 0;
-    if (here && key != loaded) {
-      const void *weight = key ? a.wk : a.wq;
-      if (has0) load_weight_vec<8>(weight, a.w_dtype, c0, a.w_vec != 0, *reinterpret_cast<float(*)[8]>(w));
-      if (has1) load_weight_vec<8>(weight, a.w_dtype, c1, a.w_vec != 0, *reinterpret_cast<float(*)[8]>(w + 8));
+    for (int i = 0; i < 8; ++i) {
+      cs[i] = 1.f;
+      sn[i] = 0.f;
     }
-    loaded = key;
-    float x[16];
+    if (has0 && now.head0 < all && known && 8 * lane < half) {
+      const uint8_t *table = static_cast<const uint8_t *>(a.cos_sin) + now.pos * a.rot * (a.cs_dtype == I8L_F32 ? 4 : 2);
+      if (8 * lane + 8 <= half) {
+        load_weight_vec<8>(table, a.cs_dtype, 8 * lane, a.cs_vec != 0, cs);
+        load_weight_vec<8>(table, a.cs_dtype, half + 8 * lane, a.cs_vec != 0, sn);
+      } else {  // interleaved, and four angles left
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      unpack2<DT>(raw[turn][h].x, x[8 * h], x[8 * h + 1]);
-      unpack2<DT>(raw[turn][h].y, x[8 * h + 2], x[8 * h + 3]);
-      unpack2<DT>(raw[turn][h].z, x[8 * h + 4], x[8 * h + 5]);
-      unpack2<DT>(raw[turn][h].w, x[8 * h + 6], x[8 * h + 7]);
-    }
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) fma2_rn(s0, s1, x[i], x[i + 1], x[i], x[i + 1], s0, s1);
-    float ss = s0 + s1;
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
-    float rs = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
-    if (!known) rs = __int_as_float(0x7fc00000);
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      mul2_rn(x[i], x[i + 1], x[i], x[i + 1], rs, rs);
-      mul2_rn(x[i], x[i + 1], x[i], x[i + 1], w[i], w[i + 1]);
-    }
-    if (a.interleaved) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float u = x[2 * i], v = x[2 * i + 1];
-        x[2 * i] = fmaf(u, cs[i], -(v * sn[i]));
-        x[2 * i + 1] = fmaf(v, cs[i], u * sn[i]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        float t0, t1, r0, r1;
-        mul2_rn(t0, t1, x[8 + i], x[9 + i], -sn[i], -sn[i + 1]);
-        mul2_rn(r0, r1, x[i], x[i + 1], sn[i], sn[i + 1]);
-        fma2_rn(x[i], x[i + 1], x[i], x[i + 1], cs[i], cs[i + 1], t0, t1);
-        fma2_rn(x[8 + i], x[9 + i], x[8 + i], x[9 + i], cs[i], cs[i + 1], r0, r1);
+        for (int i = 0; i < 4; ++i) {
+          cs[i] = load_weight(table, a.cs_dtype, 8 * lane + i);
+          sn[i] = load_weight(table, a.cs_dtype, half + 8 * lane + i);
+        }
       }
     }
-    if (here) {
-      T *dst = key ? static_cast<T *>(a.k) + token * a.ldk + static_cast<long long>(head - a.heads) * a.dim
-                   : static_cast<T *>(a.q) + token * a.ldq + static_cast<long long>(head) * a.dim;
-      if (has0)
-        *reinterpret_cast<uint4 *>(dst + c0) = make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]),
-                                                          pack2<DT>(x[4], x[5]), pack2<DT>(x[6], x[7]));
-      if (has1)
-        *reinterpret_cast<uint4 *>(dst + c1) = make_uint4(pack2<DT>(x[8], x[9]), pack2<DT>(x[10], x[11]),
-                                                          pack2<DT>(x[12], x[13]), pack2<DT>(x[14], x[15]));
+
+    if (kLoop) {  // the next group is on its way while this one is computed
+      id += gridDim.x * kGroups;
+      if (first + gridDim.x * kGroups < a.groups) fetch(id);
     }
+#pragma unroll
+    for (int turn = 0; turn < P; ++turn) {
+      const int head = now.head0 + turn;
+      const bool here = head < all;
+      const int key = head >= a.heads ? 1 : 0;
+      if (here && key != loaded) {
+        const void *weight = key ? a.wk : a.wq;
+        if (has0) load_weight_vec<8>(weight, a.w_dtype, c0, a.w_vec != 0, *reinterpret_cast<float(*)[8]>(w));
+        if (has1) load_weight_vec<8>(weight, a.w_dtype, c1, a.w_vec != 0, *reinterpret_cast<float(*)[8]>(w + 8));
+      }
+      if (here) loaded = key;
+      float x[16];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        unpack2<DT>(now.raw[turn][h].x, x[8 * h], x[8 * h + 1]);
+        unpack2<DT>(now.raw[turn][h].y, x[8 * h + 2], x[8 * h + 3]);
+        unpack2<DT>(now.raw[turn][h].z, x[8 * h + 4], x[8 * h + 5]);
+        unpack2<DT>(now.raw[turn][h].w, x[8 * h + 6], x[8 * h + 7]);
+      }
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) fma2_rn(s0, s1, x[i], x[i + 1], x[i], x[i + 1], s0, s1);
+      float ss = s0 + s1;
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o, G);
+      float rs = rsqrtf(fmaf(ss, a.inv_dim, a.eps));
+      if (!known) rs = __int_as_float(0x7fc00000);
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        mul2_rn(x[i], x[i + 1], x[i], x[i + 1], rs, rs);
+        mul2_rn(x[i], x[i + 1], x[i], x[i + 1], w[i], w[i + 1]);
+      }
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = x[2 * i], v = x[2 * i + 1];
+          x[2 * i] = fmaf(u, cs[i], -(v * sn[i]));
+          x[2 * i + 1] = fmaf(v, cs[i], u * sn[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          float t0, t1, r0, r1;
+          mul2_rn(t0, t1, x[8 + i], x[9 + i], -sn[i], -sn[i + 1]);
+          mul2_rn(r0, r1, x[i], x[i + 1], sn[i], sn[i + 1]);
+          fma2_rn(x[i], x[i + 1], x[i], x[i + 1], cs[i], cs[i + 1], t0, t1);
+          fma2_rn(x[8 + i], x[9 + i], x[8 + i], x[9 + i], cs[i], cs[i + 1], r0, r1);
+        }
+      }
+      if (here) {
+        T *dst = key ? static_cast<T *>(a.k) + now.token * a.ldk + static_cast<long long>(head - a.heads) * a.dim
+                     : static_cast<T *>(a.q) + now.token * a.ldq + static_cast<long long>(head) * a.dim;
+        if (has0)
+          *reinterpret_cast<uint4 *>(dst + c0) = make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]),
+                                                            pack2<DT>(x[4], x[5]), pack2<DT>(x[6], x[7]));
+        if (has1)
+          *reinterpret_cast<uint4 *>(dst + c1) = make_uint4(pack2<DT>(x[8], x[9]), pack2<DT>(x[10], x[11]),
+                                                            pack2<DT>(x[12], x[13]), pack2<DT>(x[14], x[15]));
+      }
+    }
+    if (!kLoop) break;
   }
 }
 
@@ -174,16 +198,18 @@ using namespace i8l;
 
 namespace {
 
-template <int DT, int P>
-cudaError_t launch_qk(const QkArgs &a, int lanes, cudaStream_t s) {
+template <int DT, int P, bool kLoop>
+cudaError_t launch_qk(const QkArgs &a, int lanes, int sms, cudaStream_t s) {
   const unsigned per_block = kQkThreads / lanes;
-  const dim3 grid((a.groups + per_block - 1) / per_block);
+  unsigned ctas = (a.groups + per_block - 1) / per_block;
+  if (kLoop) ctas = std::min<unsigned>(ctas, kQkCtas * sms);
+  const dim3 grid(ctas);
   switch (lanes) {
-    case 1: return launch(qk_norm_rope_kernel<DT, 1, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 2: return launch(qk_norm_rope_kernel<DT, 2, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 4: return launch(qk_norm_rope_kernel<DT, 4, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    case 8: return launch(qk_norm_rope_kernel<DT, 8, P>, grid, dim3(kQkThreads), 0, s, 1, a);
-    default: return launch(qk_norm_rope_kernel<DT, 16, P>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 1: return launch(qk_norm_rope_kernel<DT, 1, P, kLoop>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 2: return launch(qk_norm_rope_kernel<DT, 2, P, kLoop>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 4: return launch(qk_norm_rope_kernel<DT, 4, P, kLoop>, grid, dim3(kQkThreads), 0, s, 1, a);
+    case 8: return launch(qk_norm_rope_kernel<DT, 8, P, kLoop>, grid, dim3(kQkThreads), 0, s, 1, a);
+    default: return launch(qk_norm_rope_kernel<DT, 16, P, kLoop>, grid, dim3(kQkThreads), 0, s, 1, a);
   }
 }
 
@@ -247,10 +273,12 @@ extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, 
   a.cs_vec = aligned16(cos_sin) && (rot_dim / 2 * (cs_dtype == I8L_F32 ? 4 : 2)) % 16 == 0 ? 1 : 0;
   int lanes = 1;
   while (lanes * 16 < head_dim) lanes *= 2;
-  // One head per group until the groups fill the SMs twice over, then kQkHeads.
+  // One head per group and no loop until the lanes fill half of the SMs' threads (us by one head
+  // and by the loop, 40 heads of 128: 256 tokens 3.0 and 3.1, 512 4.2 and 3.5; 24 heads of 64:
+  // 1536 tokens 3.4 and 3.5, 3000 5.2 and 5.1; 24 heads of 256: 256 3.2 and 3.3, 1024 6.8 and 6.1).
   DeviceInfo di;
   if (int e = device_info(&di)) return e;
-  const bool many = static_cast<int64_t>(tokens) * all > 2LL * di.sms * (2048 / lanes);
+  const bool many = static_cast<int64_t>(tokens) * all * lanes > 1024LL * di.sms;
   a.parts = static_cast<int>(many ? (all + kQkHeads - 1) / kQkHeads : all);
   const int64_t groups = static_cast<int64_t>(tokens) * a.parts;
   if (groups > INT32_MAX - kQkThreads)
@@ -260,9 +288,9 @@ extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t err;
   if (act_dtype == I8L_BF16)
-    err = many ? launch_qk<I8L_BF16, kQkHeads>(a, lanes, s) : launch_qk<I8L_BF16, 1>(a, lanes, s);
+    err = many ? launch_qk<I8L_BF16, kQkHeads, true>(a, lanes, di.sms, s) : launch_qk<I8L_BF16, 1, false>(a, lanes, di.sms, s);
   else
-    err = many ? launch_qk<I8L_F16, kQkHeads>(a, lanes, s) : launch_qk<I8L_F16, 1>(a, lanes, s);
+    err = many ? launch_qk<I8L_F16, kQkHeads, true>(a, lanes, di.sms, s) : launch_qk<I8L_F16, 1, false>(a, lanes, di.sms, s);
   if (err != cudaSuccess) return cuda_error(err, "qk_norm_rope launch");
   err = cudaGetLastError();
   return err == cudaSuccess ? I8L_OK : cuda_error(err, "qk_norm_rope launch");

@@ -75,6 +75,47 @@ def test_against_float64(m, heads, kv, d, rot, interleaved, dtype):
     assert torch.equal(qkv, keep)
 
 
+@pytest.mark.parametrize("m,heads,kv,d,rot,interleaved", [
+    (3000, 5, 2, 128, 128, False), (2003, 3, 4, 256, 64, True), (10007, 7, 1, 32, 16, False), (26001, 3, 0, 24, 24, True),
+    (160001, 1, 0, 8, 8, True), (40000, 0, 1, 64, 32, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_batches(m, heads, kv, d, rot, interleaved, dtype):
+    """CTAs that take several groups of heads: odd numbers of heads, a group with a query and a
+    key head, results in place, tokens without angles and heads that are zero, infinite or NaN
+    among others."""
+    qkv = rand((m, (heads + 2 * kv) * d), d, 3.0, dtype)
+    wq, wk = rand((d,), 1, 0.2, dtype) + 1, rand((d,), 2, 0.2, dtype) + 1
+    pos = torch.randint(0, 999, (m,), generator=torch.Generator().manual_seed(m)).cuda()
+    cs = table(999, rot)
+    want = qk_norm_rope(qkv, wq, wk, EPS, pos, cs, heads, kv, interleaved=interleaved)
+    check(qkv, wq, wk, pos, cs, heads, kv, interleaved, want)
+    # Rows do not depend on the batch: a slice by itself takes the small batches' kernel.
+    for lo in (0, m // 2, m - 5):
+        part = qk_norm_rope(qkv[lo:lo + 5].contiguous(), wq, wk, EPS, pos[lo:lo + 5], cs, heads, kv,
+                            interleaved=interleaved)
+        assert all(torch.equal(a[lo:lo + 5], b) for a, b in zip(want, part))
+    work = qkv.clone()
+    got = qk_norm_rope(work, wq, wk, EPS, pos, cs, heads, kv, interleaved=interleaved,
+                       q_out=work[:, :heads * d].view(m, heads, d),
+                       k_out=work[:, heads * d:(heads + kv) * d].view(m, kv, d))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(work[:, (heads + kv) * d:], qkv[:, (heads + kv) * d:])
+
+    pos[3::7] = torch.tensor([-1, 999, 2 ** 40], device="cuda").repeat(m)[:pos[3::7].numel()]
+    qkv[1::5, :d], qkv[2::5, d // 2], qkv[4::5, d - 1] = 0.0, float("inf"), float("nan")
+    got = qk_norm_rope(qkv, wq, wk, EPS, pos, cs, heads, kv, interleaved=interleaved)
+    spoilt = torch.zeros(m, heads + kv, dtype=torch.bool, device="cuda")
+    spoilt[2::5, 0] = spoilt[4::5, 0] = True
+    spoilt[3::7] = True
+    zero = torch.zeros_like(spoilt)
+    zero[1::5, 0] = True
+    out, was = torch.cat(got, 1), torch.cat(want, 1)
+    assert torch.equal(out.isfinite().all(-1), ~spoilt)
+    assert out[zero & ~spoilt].eq(0).all()
+    fine = ~spoilt & ~zero
+    assert torch.equal(out[fine], was[fine])
+
+
 @pytest.mark.parametrize("wdt", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("tdt", [torch.bfloat16, torch.float16, torch.float32])
 def test_weight_and_angle_types_and_odd_pointers(wdt, tdt):
