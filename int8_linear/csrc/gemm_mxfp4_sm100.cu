@@ -18,7 +18,7 @@
 // of its 128 rows, the whole weight tile's.  TMEM's 512 columns do not hold two accumulators
 // of 256 and the scales, so every other tile has 192 weight rows: 256 + 192 columns of
 // accumulators leave 64 for the scales, and one tile's epilogue runs beside the next tile's
-// MMAs.  4096 x 12288 x 2048 takes 49 us (4.2 PFLOP/s; 5.8 at K = 8192).  What bounds it is
+// MMAs.  4096 x 12288 x 2048 takes 48 us (4.3 PFLOP/s; 5.8 at K = 8192).  What bounds it is
 // the operands' way from L2: with the loads left out the same MMAs ran at 8.3 PFLOP/s, and
 // 36 KB a stage and SM is 97 bytes a ns and SM.  Other tilings measured: 256 x 256 with two
 // accumulators sharing 32 columns 53 us (each tile waits for the last one's shared columns),
