@@ -9,7 +9,7 @@
 // neighbouring lanes share a block (two shuffles), and the matrix is walked as one flat
 // list of eight-value vectors or of blocks.  All four kernels move each byte once and are
 // bound by HBM: at 8192 rows (inputs larger than L2) quant_mxfp4 and dequant_mxfp4 take 26 us
-// of 8192 values, the measured copy rate; SiLU takes 38 us of 6144 (92 %; its arithmetic is
+// of 8192 values, the measured copy rate; SiLU takes 40 us of 6144 (86 %; its arithmetic is
 // what is left) and the norm 39 of 4096 with a residual (86 %).
 //
 // A 4-bit value next to the border between two steps flips on the last bit of y, so y is
@@ -157,8 +157,8 @@ __device__ __noinline__ uint32_t silu_mul2_exact(uint32_t gw, uint32_t uw) {
 // rcp.approx 1: 3 + (2 + 0.61 |g|) s.  For g > 0, s < 1/2 and |g| s < 0.28, so that is below
 // 4.2; for g = -1, -2, -3, -4 it is 4.9, 5.8, 6.7 and 7.4 and grows by 0.61 from there on.  So
 // v is within 4.25 + 0.83 max(-g, 0) of those units, and y is right wherever both ends of that
-// interval round alike; about one bf16 value in 4000 is unsure.  Where v is below float32's
-// normal range it has no such bound: see mx_tiny.
+// interval round alike; about one bf16 value in 4000 is unsure.  Where 1 / (1 + e) or v is below
+// float32's normal range there is no such bound: see silu_deep and mx_tiny.
 template <int DT>
 __device__ __forceinline__ uint32_t silu_mul2(uint32_t gw, uint32_t uw, bool &unsure) {
   constexpr float kUnit = 1.0f / 8388608.0f;
@@ -177,6 +177,16 @@ __device__ __forceinline__ uint32_t silu_mul2(uint32_t gw, uint32_t uw, bool &un
   const uint32_t low = pack2<DT>(l0, l1), high = pack2<DT>(h0, h1);
   unsure = low != high;
   return low;
+}
+
+// Whether the larger half of `gates`, two bf16 gates, is below -87: 1 + e is above 2^126 then,
+// its reciprocal may be taken for zero, and a large up brings the product back.  The negative
+// gates furthest from zero (and NaN) have the largest bits as unsigned numbers.  (In fp16, ups
+// end at 65504 and the product rounds to zero.)  The check takes 1.2 of 22 us of 4096 x 6144,
+// taken here or within the loop over the pairs.
+template <int DT>
+__device__ __forceinline__ bool silu_deep(uint32_t gates) {
+  return DT == I8L_BF16 && max(gates & 0xffffu, gates >> 16) > 0xc2aeu;
 }
 
 // Whether a block's largest y is so small that values below float32's normal range may decide
@@ -303,7 +313,8 @@ __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a
         return unsure ? silu_mul2_exact<DT>(g, u) : y;
       };
       x = make_uint4(settle(gate.x, up.x), settle(gate.y, up.y), settle(gate.z, up.z), settle(gate.w, up.w));
-      if (mx_tiny<DT>(mx_amax8<DT>(x)))
+      const bool deep = silu_deep<DT>(__vmaxu2(__vmaxu2(gate.x, gate.y), __vmaxu2(gate.z, gate.w)));
+      if (mx_tiny<DT>(mx_amax8<DT>(x)) || deep)
         x = make_uint4(silu_mul2_exact<DT>(gate.x, up.x), silu_mul2_exact<DT>(gate.y, up.y),
                        silu_mul2_exact<DT>(gate.z, up.z), silu_mul2_exact<DT>(gate.w, up.w));
     }
@@ -323,7 +334,7 @@ __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a
 // issue (77 % of the slots, 111 instructions per 8 values, 50 % of HBM at 8192 x 8192), but
 // spreads a small matrix over four times as many threads.
 // Threads: 128 (4096 x 4096 7.6 us, with 64 9.7); with SiLU 64, as a CTA stays as long as the
-// last of its warps that has unsure values (4096 x 6144 22.0 us, with 128 22.8, with 32 26.4).
+// last of its warps that has unsure values (4096 x 6144 22 us, with 128 23, with 32 26).
 template <bool kSilu>
 constexpr int kBlockThreads = kSilu ? 64 : 128;
 
@@ -348,13 +359,17 @@ __global__ void __launch_bounds__(kBlockThreads<kSilu>) mx_block_kernel(const Fl
     load_block(a.x, at + static_cast<long long>(a.blocks) * kMxBlock, a.vec, up);
     // The unsure pairs are few: they are read again and done after all others, which keeps
     // the slow code out of the unrolled loop.
-    uint32_t todo = 0u;
+    uint32_t todo = 0u, most = 0u;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) most = __vimax3_u16x2(most, x[i], x[i + 1]);
+    const bool deep = silu_deep<DT>(most);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       bool unsure;
       x[i] = silu_mul2<DT>(x[i], up[i], unsure);
       if (unsure) todo |= 1u << i;
     }
+    if (deep) todo = 0xffffu;
     for (bool all = false;; all = true) {
       while (todo) {
         const int i = __ffs(todo) - 1;
@@ -722,7 +737,7 @@ int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uin
     cudaError_t err;
     // A thread per block from 256 blocks an SM on (SiLU: 512); with fewer, four lanes a block
     // finish sooner (us by threads and by lanes: 18944 blocks 1.85 and 1.77, 75776 2.27 and
-    // 3.18, 151552 2.8 and 5.7; SiLU 37888 3.6 and 3.3, 56832 4.1 and 4.1, 75776 4.5 and 4.7).
+    // 3.18, 151552 2.8 and 5.7; SiLU 37888 3.6 and 3.3, 56832 4.1 and 4.1, 75776 4.6 and 4.8).
     const int64_t total = a.vectors / 4;
     if (dtype != I8L_F32 && total >= (kSilu ? 512 : 256) * di.sms) {
       if (a.vec && reinterpret_cast<uintptr_t>(x) % 32 == 0 && (ldx * 2) % 32 == 0) a.vec = 2;

@@ -271,6 +271,25 @@ def test_silu_of_all_gates_in_a_large_batch(act):
 
 
 @pytest.mark.parametrize("rows", [20, 410])
+def test_silu_of_deep_gates_beside_ordinary_ones(rows):
+    """bf16 gates so negative that 1 / (1 + exp(-gate)) leaves float32's normal range, with ups
+    so large that the product does not, beside ordinary values of the product's size."""
+    g = torch.Generator().manual_seed(rows)
+    gate = -80.0 - 30.0 * torch.rand((rows, 6144), generator=g, dtype=torch.float64)
+    up = 10.0 ** (36.0 + 2.5 * torch.rand((rows, 6144), generator=g, dtype=torch.float64))
+    up *= torch.randint(0, 2, up.shape, generator=g) * 2 - 1
+    size = (gate * torch.exp(gate) * up).abs()
+    plain = torch.rand((rows, 6144), generator=g) < 0.5
+    near = size.view(rows, -1, 32).amax(2, keepdim=True).expand(-1, -1, 32).reshape(rows, -1)
+    near = near * torch.exp2(-8.0 * torch.rand((rows, 1), generator=g, dtype=torch.float64))
+    up = torch.where(plain, near * torch.randn(up.shape, generator=g), up)
+    gate = torch.where(plain, torch.randn(up.shape, generator=g).double(), gate)
+    gate[:, 5::640] = -1e30
+    gu = torch.cat([gate, up], 1).to(torch.bfloat16).cuda()
+    check(*mxfp4.silu_mul_quant_mxfp4(gu), om.silu_rows(np_(gu), "bf16"))
+
+
+@pytest.mark.parametrize("rows", [20, 410])
 @pytest.mark.parametrize("act", [torch.bfloat16, torch.float16])
 def test_silu_of_padded_batches(act, rows):
     """Rows of zeros, of zero gates and of zero ups, by turns with others."""
