@@ -24,6 +24,7 @@
 // accumulators sharing 32 columns 53 us (each tile waits for the last one's shared columns),
 // 256 x 192 throughout 53 us (a 256-row MMA takes the same time for 192 and 256 columns).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "epilogue.cuh"
@@ -400,9 +401,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 }
 
 // 64 columns from n0 on of a warp's 32 token rows (the first is m0): bias, rounding and the
-// stores, through the warp's staging buffer (rows of 128 bytes in the 128-byte swizzle, then
-// one TMA store; two for float32) or straight to memory.  bias: lane i holds those of columns
-// i and 32 + i.
+// stores, through the warp's staging buffer (rows of 128 bytes in the 128-byte swizzle), by a
+// TMA store (two for float32) or, where TMA cannot address the output, by the lanes.  bias:
+// lane i holds those of columns i and 32 + i.
 template <int DT>
 __device__ __forceinline__ void pair_emit(const MxGemmArgs &a, const CUtensorMap *map_out, int m0, int n0, int lane,
                                           const float (&bias)[2], const uint32_t (&r)[2][32], uint8_t *staging) {
@@ -413,36 +414,46 @@ __device__ __forceinline__ void pair_emit(const MxGemmArgs &a, const CUtensorMap
 #pragma unroll
     for (int j = 0; j < 64; ++j) v[j] += __shfl_sync(0xffffffffu, bias[j / 32], j % 32);
   }
-  if (a.tma_out) {
-    constexpr int kBoxes = DT == I8L_F32 ? 2 : 1, kCols = 64 / kBoxes;
+  constexpr int kBoxes = DT == I8L_F32 ? 2 : 1, kCols = 64 / kBoxes;
 #pragma unroll
-    for (int h = 0; h < kBoxes; ++h) {
-      if (lane == 0) bulk_wait_read<0>();  // the last store has read the buffer
-      __syncwarp();
-      uint8_t *rowp = staging + lane * 128;
+  for (int h = 0; h < kBoxes; ++h) {
+    if (a.tma_out && lane == 0) bulk_wait_read<0>();  // the last store has read the buffer
+    __syncwarp();
+    uint8_t *rowp = staging + lane * 128;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4 w;
-        if constexpr (DT == I8L_F32)
-          w = make_uint4(__float_as_uint(v[32 * h + 4 * c]), __float_as_uint(v[32 * h + 4 * c + 1]),
-                         __float_as_uint(v[32 * h + 4 * c + 2]), __float_as_uint(v[32 * h + 4 * c + 3]));
-        else
-          w = make_uint4(pack16x2(DT, v[8 * c], v[8 * c + 1]), pack16x2(DT, v[8 * c + 2], v[8 * c + 3]),
-                         pack16x2(DT, v[8 * c + 4], v[8 * c + 5]), pack16x2(DT, v[8 * c + 6], v[8 * c + 7]));
-        *reinterpret_cast<uint4 *>(rowp + ((c ^ (lane & 7)) << 4)) = w;
-      }
+    for (int c = 0; c < 8; ++c) {
+      uint4 w;
+      if constexpr (DT == I8L_F32)
+        w = make_uint4(__float_as_uint(v[32 * h + 4 * c]), __float_as_uint(v[32 * h + 4 * c + 1]),
+                       __float_as_uint(v[32 * h + 4 * c + 2]), __float_as_uint(v[32 * h + 4 * c + 3]));
+      else
+        w = make_uint4(pack16x2(DT, v[8 * c], v[8 * c + 1]), pack16x2(DT, v[8 * c + 2], v[8 * c + 3]),
+                       pack16x2(DT, v[8 * c + 4], v[8 * c + 5]), pack16x2(DT, v[8 * c + 6], v[8 * c + 7]));
+      *reinterpret_cast<uint4 *>(rowp + ((c ^ (lane & 7)) << 4)) = w;
+    }
+    if (a.tma_out) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         if (n0 + kCols * h < a.N && m0 < a.M) tma_store_2d(map_out, staging, n0 + kCols * h, m0);
         bulk_commit();
       }
-    }
-  } else if (m0 + lane < a.M) {
+    } else {
+      // Row after row, neighbouring columns by neighbouring lanes: the rows of such an output
+      // begin anywhere (4096 x 4099 x 2048 31.8 us; a row by each lane, from registers, 166).
+      __syncwarp();
+      using E = std::conditional_t<DT == I8L_F32, uint32_t, uint16_t>;
+      const int rows = min(32, a.M - m0);
+#pragma unroll 4
+      for (int row = 0; row < rows; ++row) {
+        E *o = static_cast<E *>(a.out) + static_cast<long long>(m0 + row) * a.ldc + n0 + kCols * h;
 #pragma unroll
-    for (int j = 0; j < 64; j += 4) {
-      const float q[4] = {v[j], v[j + 1], v[j + 2], v[j + 3]};
-      if (n0 + j < a.N) store_out4(a, m0 + lane, n0 + j, q);
+        for (int j = 0; j < kCols; j += 32) {
+          const int at = (j + lane) * static_cast<int>(sizeof(E));
+          const E e = *reinterpret_cast<const E *>(staging + row * 128 + ((((at >> 4) ^ row) & 7) << 4) + (at & 15));
+          if (n0 + kCols * h + j + lane < a.N) o[j + lane] = e;
+        }
+      }
     }
   }
 }
