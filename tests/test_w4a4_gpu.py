@@ -136,6 +136,25 @@ def test_strides_pointers_and_out(m, n, k):
             assert buf.eq(7.0).all()
 
 
+@pytest.mark.parametrize("n", [1, 255, 449, 1002, 4099])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_pair_tiles_of_any_width(n, dtype):
+    """Widths that TMA cannot store, with a bias, into rows of an odd distance: the columns of a
+    product with more weight rows, and nothing beside them."""
+    m, k, rows = 700, 320, -(-n // 128) * 128
+    a, sa = mxfp4.quant_mxfp4(rand((m, k), 1))
+    w, sw = mxfp4.quant_mxfp4(rand((rows, k), 2))
+    bias = rand((rows,), 3, 1.0, dtype)
+    pair = Config(128, 256, split=4)
+    want = mxfp4.w4a4_mm(a, w.t(), sa, sw, dtype, bias, config=pair)[:, :n]
+    assert torch.equal(mxfp4.w4a4_mm(a, w[:n].t(), sa, sw, dtype, bias[:n], config=pair), want)
+    buf = torch.full((m, n + 4 + n % 2), 7.0, dtype=dtype, device="cuda")
+    out = mxfp4.w4a4_mm(a, w[:n].t(), sa, sw, dtype, bias[:n], config=pair, out=buf[:, 3:3 + n])
+    assert torch.equal(out, want)
+    out.fill_(7.0)
+    assert buf.eq(7.0).all()
+
+
 def test_nan_blocks_reach_their_rows_and_columns_only():
     a, sa = mxfp4.quant_mxfp4(rand((40, 512), 1))
     x = rand((40, 512), 1)
