@@ -1397,9 +1397,9 @@ static int make_operand_map(CUtensorMap *map, const int8_t *ptr, int64_t rows, i
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(kBK), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(ptr), dims, strides,
-                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(fn, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2u, const_cast<int8_t *>(ptr), dims, strides,
+                            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(I8L_ECUDA, "cuTensorMapEncodeTiled failed (CUresult %d) for [%lld x %lld], ld %lld",
                      static_cast<int>(r), static_cast<long long>(rows), static_cast<long long>(k),

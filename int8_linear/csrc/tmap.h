@@ -29,6 +29,17 @@ inline EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// Encodes a map.  The driver wants the thread to have a current context, which a thread that
+// has launched nothing yet lacks: it gets that of its current device then.
+template <typename... Args>
+CUresult encode_tiled(EncodeTiledFn fn, Args... args) {
+  CUresult r = fn(args...);
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = fn(args...);
+  return r;
+}
+
 // Tensor map over a row-major 2-D matrix of `rows` x `cols` elements (row stride
 // `ld_bytes`), boxes of box_cols x box_rows.
 inline int make_map(CUtensorMap *map, CUtensorMapDataType type, const void *ptr, int64_t rows,
@@ -41,9 +52,9 @@ inline int make_map(CUtensorMap *map, CUtensorMapDataType type, const void *ptr,
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld_bytes)};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, type, 2, const_cast<void *>(ptr), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(fn, map, type, 2u, const_cast<void *>(ptr), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promotion,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(I8L_ECUDA, "cuTensorMapEncodeTiled failed (CUresult %d) for the %s map [%lld x %lld]",
                      static_cast<int>(r), what, static_cast<long long>(rows),
