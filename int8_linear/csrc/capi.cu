@@ -33,7 +33,6 @@ int cuda_error(cudaError_t e, const char *what) {
 }
 
 namespace {
-constexpr int kMaxDevices = 64;
 std::mutex g_mu;
 DeviceInfo g_info[kMaxDevices];
 bool g_have[kMaxDevices];

@@ -690,25 +690,12 @@ struct MxPlan {
   int stages;
 };
 
-template <typename Kernel>
-static int allow_smem(Kernel kernel, size_t smem, size_t *configured) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_error(e, "cudaGetDevice");
-  if (dev < 0 || dev >= 64 || smem > configured[dev]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(mxfp4 gemm smem)");
-    if (dev >= 0 && dev < 64) configured[dev] = smem;
-  }
-  return I8L_OK;
-}
-
 template <int TN>
 static int launch_split(const CUtensorMap &mx, const CUtensorMap &my, const CUtensorMap &msx, const CUtensorMap &msy,
                         const MxGemmArgs &a, cudaStream_t stream) {
-  static size_t configured[64] = {};
+  static std::atomic<bool> allowed[kMaxDevices];
   const size_t smem = SplitLayout<TN>::bytes(a.stages);
-  if (int e = allow_smem(mx_split_kernel<TN>, smem, configured)) return e;
+  if (int e = allow_smem(mx_split_kernel<TN>, allowed, "shared memory of the mxfp4 gemm")) return e;
   cudaError_t e = launch(mx_split_kernel<TN>, dim3(static_cast<unsigned>(a.tiles_n) * a.tiles_m * a.cluster),
                          dim3(kSplitThreads), smem, stream, a.cluster, mx, my, msx, msy, a);
   if (e != cudaSuccess) return cuda_error(e, "mxfp4 gemm launch");
@@ -720,9 +707,9 @@ template <int DT>
 static int launch_pair(const CUtensorMap &mx, const CUtensorMap &my, const CUtensorMap &mn, const CUtensorMap &msx,
                        const CUtensorMap &msy, const CUtensorMap &mo, const MxGemmArgs &a, int pairs,
                        cudaStream_t stream) {
-  static size_t configured[64] = {};
+  static std::atomic<bool> allowed[kMaxDevices];
   const size_t smem = pair_smem(a.stages);
-  if (int e = allow_smem(mx_pair_kernel<DT>, smem, configured)) return e;
+  if (int e = allow_smem(mx_pair_kernel<DT>, allowed, "shared memory of the mxfp4 gemm")) return e;
   cudaError_t e = launch(mx_pair_kernel<DT>, dim3(2 * pairs), dim3(kPairThreads), smem, stream, 2, mx, my, mn, msx,
                          msy, mo, a);
   if (e != cudaSuccess) return cuda_error(e, "mxfp4 gemm launch");

@@ -1672,19 +1672,9 @@ static int launch_tn(const CUtensorMap &mx, const CUtensorMap &my, const CUtenso
                      const CUtensorMap &mw, const GemmArgs &a, int ctas, int stages,
                      cudaStream_t stream) {
   const size_t smem = SmemLayout<TN, kVar>::bytes(stages);
-  // Largest dynamic shared memory already allowed, per device (the attribute is
-  // set on the function as loaded in each device's context).
-  static size_t configured[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_error(e, "cudaGetDevice");
-  if (dev < 0 || dev >= 64 || smem > configured[dev]) {
-    e = cudaFuncSetAttribute(w8a8_gemm_sm100<TN, kVar>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
-    if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(gemm smem)");
-    if (dev >= 0 && dev < 64) configured[dev] = smem;
-  }
-  e = launch(w8a8_gemm_sm100<TN, kVar>, dim3(ctas), dim3(kThreads), smem, stream,
+  static std::atomic<bool> allowed[kMaxDevices];
+  if (int e = allow_smem(w8a8_gemm_sm100<TN, kVar>, allowed, "shared memory of the gemm")) return e;
+  cudaError_t e = launch(w8a8_gemm_sm100<TN, kVar>, dim3(ctas), dim3(kThreads), smem, stream,
              kVar == kVarPair ? 2 : a.cluster, mx, my, mo,
              mw, a);
   if (e != cudaSuccess) return cuda_error(e, "gemm launch");

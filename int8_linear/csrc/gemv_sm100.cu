@@ -481,17 +481,9 @@ __global__ void __launch_bounds__(kGemvThreads, MT <= 8 ? 2 : 1) w8a8_gemv_sm100
 
 template <int MT, int RG, int NVP>
 static int launch_gemv(const GemvArgs &a, int ctas, size_t smem, cudaStream_t stream) {
-  static size_t configured[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_error(e, "cudaGetDevice");
-  if (dev < 0 || dev >= 64 || smem > configured[dev]) {
-    e = cudaFuncSetAttribute(w8a8_gemv_sm100<MT, RG, NVP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
-    if (e != cudaSuccess) return cuda_error(e, "cudaFuncSetAttribute(gemv smem)");
-    if (dev >= 0 && dev < 64) configured[dev] = smem;
-  }
-  e = launch(w8a8_gemv_sm100<MT, RG, NVP>, dim3(ctas), dim3(kGemvThreads), smem, stream, 1, a);
+  static std::atomic<bool> allowed[kMaxDevices];
+  if (int e = allow_smem(w8a8_gemv_sm100<MT, RG, NVP>, allowed, "shared memory of the gemv")) return e;
+  cudaError_t e = launch(w8a8_gemv_sm100<MT, RG, NVP>, dim3(ctas), dim3(kGemvThreads), smem, stream, 1, a);
   if (e != cudaSuccess) return cuda_error(e, "gemv launch");
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_error(e, "gemv launch");

@@ -1,6 +1,7 @@
 // Host-side helpers shared by the translation units of the library.
 #pragma once
 
+#include <atomic>
 #include <cstdarg>
 #include <cstddef>
 #include <cstdint>
@@ -25,6 +26,26 @@ struct DeviceInfo {
   int cc_major, cc_minor;
 };
 int device_info(DeviceInfo *out);
+constexpr int kMaxDevices = 64;  // device_info refuses indices from here on
+
+// Lets `kernel` take all the dynamic shared memory of the current device, once per device (an
+// attribute of the function as loaded in each device's context); `done` are the kernel's own
+// flags.  Always the most, so that threads that come here together set the same value and none
+// lowers what another relies on.
+template <typename Kernel>
+int allow_smem(Kernel kernel, std::atomic<bool> (&done)[kMaxDevices], const char *what) {
+  DeviceInfo di;
+  if (int e = device_info(&di)) return e;
+  if (done[di.device].load(std::memory_order_acquire)) return I8L_OK;
+  cudaFuncAttributes fa;
+  cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             di.max_smem_optin - static_cast<int>(fa.sharedSizeBytes));
+  if (e != cudaSuccess) return cuda_error(e, what);
+  done[di.device].store(true, std::memory_order_release);
+  return I8L_OK;
+}
 
 // Device pointer of the status word kernels set when a bounded wait gives up.
 int *status_ptr();
