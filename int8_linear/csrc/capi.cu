@@ -29,6 +29,7 @@ int set_error(int code, const char *fmt, ...) {
 }
 
 int cuda_error(cudaError_t e, const char *what) {
+  cudaGetLastError();  // reported here: not by the thread's next launch once more
   return set_error(I8L_ECUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
 
