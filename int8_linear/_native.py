@@ -190,8 +190,10 @@ def clear_status() -> None:
 
 def set_pdl(enable: bool) -> None:
     """Launch every kernel with programmatic dependent launch (see i8l_set_pdl): a kernel
-    may start while the previous one in the stream runs, and GEMMs prefetch weight tiles
-    before waiting for it.  Only for weights that the preceding kernel never writes."""
+    may start while those before it in the stream run, and GEMMs prefetch weight tiles
+    before waiting for them.  Weights must be complete when a GEMM is called (synchronise the
+    stream after writing them, and after turning this on); quant_mxfp4 alone may make one for
+    the very next product."""
     check(load().i8l_set_pdl(1 if enable else 0))
 
 

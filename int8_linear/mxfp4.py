@@ -196,8 +196,9 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
     (swap_ab token tiles of 16 to 128 with split 1 or 3, cluster and stages; CTA pairs: bm
     128, bn 256, split 4; or CUDA cores for at most four tokens: bm 1, 2 or 4, bn 0, split 5)
     in place of the library's choice.  Raises NotSupported for what the kernel does not take and ValueError
-    for inconsistent arguments.  With programmatic dependent launch (set_pdl) the weight must
-    not have been written by the kernel just before, as for w8a8_mm."""
+    for inconsistent arguments.  With programmatic dependent launch (set_pdl) a weight
+    that quant_mxfp4 did not make, with it on, must be complete before the call: the stream
+    synchronised, or a kernel of another library launched, after whatever wrote it."""
     if a_q.dtype != _U8 or b_q.dtype != _U8:
         raise NotSupported(f"uint8 4-bit codes only, got {a_q.dtype} and {b_q.dtype}")
     shape_a, shape_b = a_q.shape, b_q.shape
