@@ -82,19 +82,34 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Waits until the previous kernel finished and its writes are visible.  A no-op for a launch
+// without the programmatic attribute.
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Wait for the phase with the given parity to complete.  Returns false (after
 // setting *abort and the status bit) when the wait ran past kWaitLimitNs or when
-// another role of the CTA already gave up.
+// another role of the CTA already gave up.  A kernel launched programmatically may wait for
+// data that follow the previous kernel, however long that runs, so the limit counts once more
+// from when that kernel is done.
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity,
                                                   volatile int *abort,
                                                   int *status, int bit) {
   if (mbar_try_wait(bar, parity)) return true;
   unsigned long long t0 = globaltimer_ns();
+  bool again = true;
   for (uint32_t it = 1;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63u) == 0) {
       if (*abort) return false;
       if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        if (again) {
+          again = false;
+          pdl_wait();
+          t0 = globaltimer_ns();
+          continue;
+        }
         *abort = 1;
         if (status) atomicOr(status, bit);
         return false;
@@ -410,14 +425,9 @@ __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
 
 // ---------------------------------------------------------------- PDL
 // Programmatic dependent launch: let the next kernel in the stream start its
-// prologue now / wait until the previous kernel finished and its writes are
-// visible.  Both are no-ops for a launch without the programmatic attribute.
+// prologue now.  A no-op where that is not launched with the programmatic attribute.
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
-__device__ __forceinline__ void pdl_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- barriers
