@@ -351,7 +351,8 @@ int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, const uint8_t 
 /*
  * RMSNorm of every query and key head of a qkv product and its rotation by the token's
  * position, in one pass:
- *     n = x / sqrt(mean(x^2) + eps) * weight          (per head, in float32)
+ *     n = x / sqrt(mean(x^2) + eps) * weight          (per head, in float32; a power of two
+ *         is taken out of bf16 heads whose squares float32 cannot hold)
  *     pairs (a, b) of n's first rot_dim values -> (a cos - b sin, b cos + a sin)
  * then one rounding to act_dtype (I8L_BF16/F16).
  *   qkv       token t's row at qkv + t*ld elements: `heads` query heads, then `kv_heads`

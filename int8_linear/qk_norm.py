@@ -5,7 +5,8 @@ B200 (sm_100a).
 
 is the step between the qkv linear of a Qwen3-shaped layer and its attention: each head is
 normalised over its own values, scaled by its weight and rotated by its token's position.
-The kernel is csrc/qk_norm.cu behind the C ABI; float32 inside, one rounding at the end; also
+The kernel is csrc/qk_norm.cu behind the C ABI; float32 inside, with a power of two taken out
+of bf16 heads whose squares float32 cannot hold, and one rounding at the end; also
 torch.ops.int8_linear.qk_norm_rope.
 The reference package (AshrithaG/int8-linear) leaves this step to vLLM.
 """
