@@ -263,7 +263,11 @@ extern "C" int i8l_qk_norm_rope(const void *qkv, int64_t ld, int32_t act_dtype, 
   if (!qkv || !positions || (rot_dim && !cos_sin) || (heads && (!q_weight || !q_out)) ||
       (kv_heads && (!k_weight || !k_out)))
     return set_error(I8L_EINVAL, "NULL pointer argument");
-  if (tokens == 1) ld = std::max<int64_t>(ld, (all * head_dim + 7) / 8 * 8);  // never used
+  if (tokens == 1) {  // distances between tokens are never used
+    ld = all * head_dim;
+    ldq = static_cast<int64_t>(heads) * head_dim;
+    ldk = static_cast<int64_t>(kv_heads) * head_dim;
+  }
   if (ld < all * head_dim || (heads && ldq < static_cast<int64_t>(heads) * head_dim) ||
       (kv_heads && ldk < static_cast<int64_t>(kv_heads) * head_dim))
     return set_error(I8L_EINVAL, "row stride smaller than the heads of a token");

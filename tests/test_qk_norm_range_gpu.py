@@ -66,3 +66,17 @@ def test_plain_heads_beside_others_keep_their_bits(m):
     nan = torch.zeros(d, dtype=torch.bool, device="cuda")
     nan[7], nan[7 + d // 2] = True, True
     assert got[:, 4][:, nan].isnan().all() and got[:, 4][:, ~nan].eq(0).all()
+
+
+def test_one_token_may_have_any_distance():
+    heads, kv, d = 3, 1, 24
+    x, w = rand((1, (heads + kv) * d), 5), rand((d,), 1, 0.2) + 1
+    pos, cs = torch.tensor([7]).cuda(), table(99, 16)
+    want = qk_norm_rope(x, w, w, 1e-6, pos, cs, heads, kv)
+    buf = torch.zeros(300, dtype=torch.bfloat16, device="cuda")
+    for stride in (0, 5, 101):
+        q, k = (torch.as_strided(buf, (1, n, d), (stride, d, 1), 96 * i) for i, n in ((1, heads), (2, kv)))
+        row = torch.as_strided(buf, (1, (heads + kv) * d), (stride, 1))
+        row.copy_(x)
+        got = qk_norm_rope(row, w, w, 1e-6, pos, cs, heads, kv, q_out=q, k_out=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
