@@ -164,6 +164,9 @@ def on_device(index: int, fn, *args) -> None:
         check(code)
 
 
+MOST_ROWS = 2 ** 31 - 1  # sizes are int32 in the C ABI; ctypes would cut larger ones
+
+
 # Called when the status word shows a kernel gave up a wait, and by clear_status():
 # the GEMM module registers the re-zeroing of its split-K workspaces here.
 STATUS_HOOKS: list = []

@@ -33,7 +33,7 @@ import ctypes
 import torch
 
 from int8_linear import _native
-from int8_linear._native import NotSupported
+from int8_linear._native import MOST_ROWS, NotSupported
 from int8_linear.fused_quant import _ACT, _WEIGHT
 from int8_linear.kernel import Config, current_stream
 
@@ -51,6 +51,8 @@ def _rows(x: torch.Tensor, name: str, kinds: dict) -> tuple[int, int, int, int]:
     shape, stride = x.shape, x.stride()
     if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise NotSupported(f"{name} must be a 2-D tensor with contiguous rows")
+    if shape[0] > MOST_ROWS:
+        raise NotSupported(f"{name} has {shape[0]} rows, more than {MOST_ROWS}")
     dev = x.get_device()
     if dev < 0:
         raise ValueError(f"the 4-bit quantisers run on a CUDA device, got {x.device}")
@@ -152,8 +154,8 @@ def dequant_mxfp4(q: torch.Tensor, s: torch.Tensor, out_dtype: torch.dtype = tor
         raise NotSupported("q must be a 2-D tensor with contiguous rows")
     m, half = shape
     k, dev, ldq = 2 * half, q.get_device(), stride[0]
-    if k % BLOCK:
-        raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks)")
+    if k % BLOCK or m > MOST_ROWS:
+        raise NotSupported(f"K={k} must be a multiple of {BLOCK} (whole blocks) and M={m} at most {MOST_ROWS}")
     if dev < 0:
         raise ValueError(f"dequant_mxfp4 runs on a CUDA device, got {q.device}")
     s = _scales(s, m, k, dev, "s")
@@ -206,8 +208,9 @@ def w4a4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_b
         raise ValueError(f"cannot multiply {tuple(shape_a)} by {tuple(shape_b)}")
     m, half = shape_a
     n, k, dev = shape_b[1], 2 * half, a_q.get_device()
-    if k == 0 or k % BLOCK:
-        raise NotSupported(f"K={k} must be a positive multiple of {BLOCK} (whole blocks)")
+    if k == 0 or k % BLOCK or m > MOST_ROWS or n > MOST_ROWS:
+        raise NotSupported(f"K={k} must be a positive multiple of {BLOCK} (whole blocks), M={m} and N={n} at most "
+                           f"{MOST_ROWS}")
     lda, unit_a = a_q.stride()
     unit_b, ldw = b_q.stride()
     if unit_b != 1 and n > 1:

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from int8_linear import _native
-from int8_linear._native import NotSupported
+from int8_linear._native import MOST_ROWS, NotSupported
 from int8_linear.fused_quant import _ACT, _WEIGHT
 from int8_linear.kernel import current_stream
 
@@ -60,6 +60,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise NotSupported("qkv must be a 2-D activation with contiguous rows")
     m, width = shape
+    if m > MOST_ROWS:
+        raise NotSupported(f"{m} tokens are more than {MOST_ROWS}")
     d, dev = q_weight.numel(), qkv.get_device()
     wdt = q_weight.dtype
     if wdt not in _WEIGHT or k_weight.dtype != wdt or k_weight.numel() != d or d == 0:

@@ -1,0 +1,32 @@
+"""Sizes beyond the C ABI's int32: refused, not cut (no GPU and no memory needed: the rows of
+these tensors are one row)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from int8_linear import NotSupported, mxfp4
+from int8_linear.qk_norm import qk_norm_rope
+
+MANY = 2 ** 32 + 128
+
+
+def rows(n, cols, dtype):
+    return torch.zeros((1, cols), dtype=dtype).expand(n, cols)
+
+
+@pytest.mark.parametrize("n", [2 ** 31, MANY])
+def test_more_rows_than_int32_holds(n):
+    x, q = rows(n, 64, torch.bfloat16), rows(n, 32, torch.uint8)
+    s = torch.zeros((1, 1, 512), dtype=torch.uint8)
+    many_s = s.expand(-(-n // 128), 1, 512)
+    one = torch.ones(64)
+    small = torch.zeros((1, 32), dtype=torch.uint8)
+    for call in (lambda: mxfp4.quant_mxfp4(x), lambda: mxfp4.silu_mul_quant_mxfp4(x),
+                 lambda: mxfp4.add_rmsnorm_quant_mxfp4(x, None, one, 1e-6), lambda: mxfp4.dequant_mxfp4(q, many_s),
+                 lambda: mxfp4.w4a4_mm(small, q.t(), s, many_s), lambda: mxfp4.w4a4_mm(q, small.t(), many_s, s),
+                 lambda: qk_norm_rope(x, one[:32], one[:32], 1e-6, torch.zeros(1, dtype=torch.int64).expand(n),
+                                      torch.zeros((1, 32)), 1, 1)):
+        with pytest.raises(NotSupported):
+            call()
