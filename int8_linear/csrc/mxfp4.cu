@@ -846,6 +846,8 @@ extern "C" int i8l_add_rmsnorm_quant_mxfp4(const void *x, int64_t ldx, const voi
   RowShape rs;
   if (!row_shape(K, 8, &rs)) return set_error(I8L_ENOTSUP, "row of %d values is too long", K);
   const int ktiles = (K + 127) / 128;
+  // a CTA per row and, behind them, a few per 128-value tile of K for the zero scales
+  if (M > INT32_MAX - 128 * ktiles) return set_error(I8L_ENOTSUP, "M=%d rows are too many", M);
   MxNormArgs a;
   a.x = x;
   a.ldx = ldx;

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from int8_linear import NotSupported, mxfp4
+from int8_linear import NotSupported, _native, mxfp4
 from int8_linear.qk_norm import qk_norm_rope
 
 MANY = 2 ** 32 + 128
@@ -30,3 +30,9 @@ def test_more_rows_than_int32_holds(n):
                                       torch.zeros((1, 32)), 1, 1)):
         with pytest.raises(NotSupported):
             call()
+
+def test_norm_whose_grid_would_be_too_large():
+    p = 1 << 20   # never dereferenced: refused before any CUDA call
+    lib = _native.load()
+    assert lib.i8l_add_rmsnorm_quant_mxfp4(p, 32, None, 0, p, 0, 0, p, 16, p, None, 0, 2 ** 31 - 1, 32, 1e-6,
+                                           None) == _native.ENOTSUP
