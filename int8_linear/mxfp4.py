@@ -22,7 +22,8 @@ A block's scale is 2^(floor(log2 max|y|) - 2), the rule of the OCP microscaling 
 block's largest value lands between 4 and 8 steps and saturates at 6.  Values are rounded to
 the nearest, ties to even.  A block that holds an infinity or a NaN becomes NaN.  The
 kernels are csrc/mxfp4.cu, csrc/gemm_mxfp4_sm100.cu and csrc/gemv_mxfp4.cu behind the C ABI;
-the quantisers and the product are torch custom ops too, under torch.ops.int8_linear.  The reference package
+the quantisers and the product are torch custom ops too, under torch.ops.int8_linear.  The
+reference package
 (AshrithaG/int8-linear) has no 4-bit form.
 """
 
@@ -287,7 +288,7 @@ def add_rmsnorm_quant_mxfp4_op(x: torch.Tensor, residual: torch.Tensor, weight: 
 
 @add_rmsnorm_quant_mxfp4_op.register_fake
 def _(x, residual, weight, eps):
-    return (*_fake(x, x.shape[0], x.shape[1]), torch.empty_like(x))
+    return (*_fake(x, x.shape[0], x.shape[1]), x.new_empty(x.shape))
 
 
 @torch.library.custom_op("int8_linear::silu_mul_quant_mxfp4", mutates_args=())

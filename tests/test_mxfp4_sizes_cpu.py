@@ -36,3 +36,8 @@ def test_norm_whose_grid_would_be_too_large():
     lib = _native.load()
     assert lib.i8l_add_rmsnorm_quant_mxfp4(p, 32, None, 0, p, 0, 0, p, 16, p, None, 0, 2 ** 31 - 1, 32, 1e-6,
                                            None) == _native.ENOTSUP
+
+def test_meta_function_of_the_norm_has_the_strides_of_the_op():
+    x = torch.empty((64, 48), dtype=torch.bfloat16, device="meta").t()
+    q, s, res = torch.ops.int8_linear.add_rmsnorm_quant_mxfp4(x, x, torch.empty(64, device="meta"), 1e-6)
+    assert res.shape == (48, 64) and res.is_contiguous()
