@@ -23,8 +23,7 @@ block's largest value lands between 4 and 8 steps and saturates at 6.  Values ar
 the nearest, ties to even.  A block that holds an infinity or a NaN becomes NaN.  The
 kernels are csrc/mxfp4.cu, csrc/gemm_mxfp4_sm100.cu and csrc/gemv_mxfp4.cu behind the C ABI;
 the quantisers and the product are torch custom ops too, under torch.ops.int8_linear.  The
-reference package
-(AshrithaG/int8-linear) has no 4-bit form.
+reference package (AshrithaG/int8-linear) has no 4-bit form.
 """
 
 from __future__ import annotations
