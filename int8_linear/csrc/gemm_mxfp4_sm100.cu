@@ -6,7 +6,9 @@
 // Split tiles (mx_split_kernel), for batches of up to a few hundred tokens: the weight is
 // the MMA's 128-row side and TN tokens its other side; the CTAs of a thread-block cluster
 // share one tile's K, one tile per cluster.  Streaming the weight from HBM bounds these
-// shapes, so the split exists to keep every SM loading.  Each CTA leaves its float32
+// shapes, so the split exists to have more SMs loading; clusters double in size, so that tiles
+// between half and all of the SMs leave the rest of them idle (96 of 148 load at N = 12288).
+// Each CTA leaves its float32
 // partial tile in its own shared memory; after a cluster barrier each CTA adds, for its
 // share of the outputs, every CTA's partial in rank order through distributed shared
 // memory.  So a shape's result does not vary from run to run.
@@ -18,9 +20,12 @@
 // of its 128 rows, the whole weight tile's.  TMEM's 512 columns do not hold two accumulators
 // of 256 and the scales, so every other tile has 192 weight rows: 256 + 192 columns of
 // accumulators leave 64 for the scales, and one tile's epilogue runs beside the next tile's
-// MMAs.  4096 x 12288 x 2048 takes 48 us (4.3 PFLOP/s; 5.8 at K = 8192).  What bounds it is
-// the operands' way from L2: with the loads left out the same MMAs ran at 8.3 PFLOP/s, and
-// 36 KB a stage and SM is 97 bytes a ns and SM.  Other tilings measured: 256 x 256 with two
+// MMAs.  4096 x 12288 x 2048 takes 48 to 50 us (4.2 PFLOP/s; 5.8 at K = 8192).  Two things bound
+// it.  The outputs: with K = 256 the product still takes 29 us, for 100 MB that the copy rate
+// would write in 15.  And the operands' way from L2: every further 1024 of K takes 11 to 13 us
+// up to K = 2048 and 15 from 4096 on, 7 PFLOP/s, where the same MMAs with the loads left out ran at
+// 8.3.  The outputs' part is hidden behind the operands' only in part until that is the longer
+// one.  Other tilings measured: 256 x 256 with two
 // accumulators sharing 32 columns 53 us (each tile waits for the last one's shared columns),
 // 256 x 192 throughout 53 us (a 256-row MMA takes the same time for 192 and 256 columns).
 #include <algorithm>

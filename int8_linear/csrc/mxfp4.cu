@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a
 // The flat quantisers for matrices that fill the GPU: one thread takes a whole block, so
 // there is nothing to exchange, and addresses, the scale and the index arithmetic are shared
 // by 32 values instead of 8.  The four-lanes-a-block kernel above was bound by instruction
-// issue (77 % of the slots, 111 instructions per 8 values, 50 % of HBM at 8192 x 8192), but
+// issue (77 % of the slots, 111 instructions per 8 values; 8192 x 8192 42.6 us), but
 // spreads a small matrix over four times as many threads.
 // Threads: 128 (4096 x 4096 7.6 us, with 64 9.7); with SiLU 64, as a CTA stays as long as the
 // last of its warps that has unsure values (4096 x 6144 22 us, with 128 23, with 32 26).
@@ -761,8 +761,8 @@ int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uin
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err;
     // A thread per block from 256 blocks an SM on (SiLU: 512); with fewer, four lanes a block
-    // finish sooner (us by threads and by lanes: 18944 blocks 1.85 and 1.77, 75776 2.27 and
-    // 3.18, 151552 2.8 and 5.7; SiLU 37888 3.6 and 3.3, 56832 4.1 and 4.1, 75776 4.6 and 4.8).
+    // finish sooner (us by threads and by lanes: 18944 blocks 1.69 and 1.63, 37888 1.79 and 1.91,
+    // 151552 2.8 and 4.4; fp32 stays with four lanes, 8192 x 8192 46.7 us, the copy rate; SiLU 37888 3.6 and 3.3, 56832 4.1 and 4.1, 75776 4.6 and 4.8).
     const int64_t total = a.vectors / 4;
     if (dtype != I8L_F32 && total >= (kSilu ? 512 : 256) * di.sms) {
       if (a.vec && reinterpret_cast<uintptr_t>(x) % 32 == 0 && (ldx * 2) % 32 == 0) a.vec = 2;

@@ -92,8 +92,8 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     length, rot = angles
     _native.on_device(dev, _native.load().i8l_qk_norm_rope, qkv.data_ptr(), stride[0], _ACT[qkv.dtype],
                       wq.data_ptr(), wk.data_ptr(), _WEIGHT[wdt], eps, pos.data_ptr(), wide, table.data_ptr(),
-                      _WEIGHT[table.dtype], length, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), m, heads,
-                      kv_heads, d, rot, interleaved, current_stream(dev))
+                      _WEIGHT[table.dtype], length, q.data_ptr(), q.stride(0) if m > 1 else 0, k.data_ptr(),
+                      k.stride(0) if m > 1 else 0, m, heads, kv_heads, d, rot, interleaved, current_stream(dev))
     return q, k
 
 
