@@ -391,14 +391,14 @@ int i8l_clear_status(void);
  * Programmatic dependent launch (process-wide, off by default).  When on, every kernel
  * of the library is launched so that it may start while the kernels before it in the
  * stream are still running: it sets up, and a GEMM loads the weight tiles of its first
- * pipeline stages, then waits for those kernels before reading activations or
- * anything else that they wrote, or writing anything.  Most kernels let the next one start at entry,
- * so several launches may be under way at once.  A GEMM's weight (W, and the scales of a
+ * pipeline stages, then waits for those kernels before reading activations or anything
+ * else that they wrote, or writing anything.  Most kernels let the next one start at
+ * entry, so several launches may be under way at once.  A GEMM's weight (W, and the scales of a
  * 4-bit one) must therefore be complete when the GEMM is launched: between its last write
  * and that launch the stream was synchronised, or a kernel launched without the attribute
  * (any other library's) came after the writing one.  Only i8l_quant_mxfp4, called with it
- * on, needs neither: it lets nothing start before it has written, so its result may be the
- * weight of the very next product.
+ * on, needs neither: its result may be the weight of the very next product (if it wrote
+ * the weight in pieces of rows, each had 128 or more).
  * No reference counterpart (Triton launches are stream-ordered).
  */
 int i8l_set_pdl(int32_t enable);

@@ -57,6 +57,7 @@ struct MxGemmArgs {
   int out_dtype;
   long long ldc;
   int vec_store;        // four consecutive outputs of a row may be stored at once
+  int early;            // see mx_weight_early
   int tma_out;          // pair tiles: outputs leave through shared memory by TMA stores
   FastDiv per_col;      // pair tiles: token tiles (a division per tile and role took 500 cycles)
   int *status;
@@ -171,7 +172,7 @@ __global__ void __launch_bounds__(kSplitThreads)
   const int kb0 = a.kblocks * rank / a.cluster, kb1 = a.kblocks * (rank + 1) / a.cluster;
 
   const uint64_t pol_w = policy_evict_first(), pol_a = policy_evict_last();
-  const int pre = min(S, kb1 - kb0);
+  const int pre = a.early ? min(S, kb1 - kb0) : 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
       mbar_init(&full[i], 1);
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     bool more = walk.next(a, kind, tm, n0);
     // The first tile's weight stages do not wait for the previous kernel.
     int pre = 0;
-    if (more)
+    if (more && a.early)
       for (; pre < min(S, a.kblocks); ++pre) load_w(pre, pre);
     pdl_wait();
     bool ok = true;
@@ -838,6 +839,7 @@ extern "C" int i8l_w4a4_mm(const uint8_t *A, int64_t lda, const uint8_t *sa, con
   a.tiles_n = (N + w_rows - 1) / w_rows;
   a.tiles_m = (M + p.tn - 1) / p.tn;
   a.cluster = p.cluster;
+  a.early = mx_weight_early(N) ? 1 : 0;
   a.stages = p.stages;
   a.bias = bias;
   a.bias_dtype = bias_dtype;

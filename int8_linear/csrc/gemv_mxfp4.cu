@@ -30,6 +30,7 @@ struct MxGemvArgs {
   long long lda, ldw;
   int M, N;
   int blocks, ktiles;
+  int early;  // see mx_weight_early
   const void *bias;
   int bias_dtype;
   void *out;
@@ -78,8 +79,9 @@ __global__ void __launch_bounds__(2 * kSpan) mx_gemv_kernel(const MxGemvArgs a) 
       s1 = *reinterpret_cast<const uint2 *>(p + 16);
     }
   };
-  load_w(t);
+  if (a.early) load_w(t);
   pdl_wait();
+  if (!a.early) load_w(t);
 
   float acc[kRows][MT] = {};
   for (int b = t; b < a.blocks; b += kSpan) {
@@ -186,6 +188,7 @@ int mx_gemv_run(const uint8_t *A, int64_t lda, const uint8_t *sa, const uint8_t 
   a.N = N;
   a.blocks = K / kMxBlock;
   a.ktiles = (K + 127) / 128;
+  a.early = mx_weight_early(N) ? 1 : 0;
   a.bias = bias;
   a.bias_dtype = bias_dtype;
   a.out = out;

@@ -211,19 +211,24 @@ struct FlatArgs {
   FastDiv per_row;         // vectors per row
   int vec;                 // 1: 16-byte loads allowed, 2: 32-byte loads
   int q16;                 // 16-byte stores of codes allowed
+  int rows_all;            // rows of the call
   int pdl;                 // launched with programmatic stream serialisation
 };
 
-// The end of the plain quantiser, whose result may be a weight; all threads of a CTA come here
-// together.  A product reads its weight before it waits for earlier kernels, and those let it
-// start as soon as they have started themselves, so that it may run beside a kernel some
-// launches before it.  This one therefore lets nothing start at entry, and its stores have been
-// performed when its CTAs are done.  One thread's fence covers what its CTA wrote (8192 x 8192
-// 26.3 us, with a fence in every thread 28.0, with no order at all 25.4; stand-in decoder, us a
-// layer with and without the order: 1 token 24.1 and 24.2, 8 25.8 and 24.6, 32 29.1 and 27.7,
-// 128 40.3 and 40.8).
-__device__ __forceinline__ void weight_written(const FlatArgs &a) {
-  if (a.pdl) {
+// The plain quantiser's result may be a weight.  A product reads its weight before it waits for
+// earlier kernels, and those let it start as soon as they have started themselves, so that it
+// may run beside a kernel some launches before it.  From kWeightRows rows on, this one therefore
+// lets nothing start at entry, and its stores have been performed when its CTAs are done; one
+// thread's fence covers what its CTA wrote (8192 x 8192 26.3 us, with a fence in every thread
+// 28.0, with no order at all 25.4).  Products wait before they read a weight of fewer rows,
+// so that small batches of tokens keep the overlap (stand-in decoder, us a layer with and
+// without the order for all: 8 tokens 25.8 and 24.7, 32 29.1 and 27.7, 128 40.3 and 40.8).
+__device__ __forceinline__ void plain_begin(const FlatArgs &a) {
+  if (a.rows_all < kWeightRows) pdl_launch_dependents();
+}
+// All threads of a CTA come here together.
+__device__ __forceinline__ void plain_end(const FlatArgs &a) {
+  if (a.pdl && a.rows_all >= kWeightRows) {
     __syncthreads();
     if (threadIdx.x == 0) __threadfence();
   }
@@ -307,7 +312,10 @@ __device__ __forceinline__ void store_block(const MxOut &o, int q16, long long r
 template <int DT, bool kSilu>
 __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a) {
   static_assert(!kSilu || DT != I8L_F32, "SiLU takes 16-bit activations");
-  if (kSilu) pdl_launch_dependents();
+  if constexpr (kSilu)
+    pdl_launch_dependents();
+  else
+    plain_begin(a);
   pdl_wait();
   const uint32_t id = blockIdx.x * kFlatThreads + threadIdx.x;
   const uint32_t row = a.per_row.div(id), vec = id - row * a.per_row.d;
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(kFlatThreads) mx_quant_kernel(const FlatArgs a
   } else if (id - a.vectors < a.pad_words) {
     zero_pad_word(a.o, a.rows, id - a.vectors);
   }
-  if (!kSilu) weight_written(a);
+  if constexpr (!kSilu) plain_end(a);
 }
 
 // The flat quantisers for matrices that fill the GPU: one thread takes a whole block, so
@@ -419,10 +427,13 @@ __device__ __forceinline__ void mx_block(const FlatArgs &a) {
 
 template <int DT, bool kSilu>
 __global__ void __launch_bounds__(kBlockThreads<kSilu>) mx_block_kernel(const FlatArgs a) {
-  if (kSilu) pdl_launch_dependents();
+  if constexpr (kSilu)
+    pdl_launch_dependents();
+  else
+    plain_begin(a);
   pdl_wait();
   mx_block<DT, kSilu>(a);
-  if (!kSilu) weight_written(a);
+  if constexpr (!kSilu) plain_end(a);
 }
 
 // ------------------------------------------------------------------ add + RMSNorm
@@ -757,12 +768,14 @@ int run_flat(const void *x, int64_t ldx, int dtype, uint8_t *q, int64_t ldq, uin
     a.pad_words = static_cast<uint32_t>(pad) * ktiles;
     a.vec = vec_rows(x, ldx, dtype) && (!kSilu || (static_cast<int64_t>(K) * act_size(dtype)) % 16 == 0) ? 1 : 0;
     a.q16 = aligned16(q) && ldq % 16 == 0 ? 1 : 0;
+    a.rows_all = M;
     a.pdl = pdl_enabled() ? 1 : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t err;
     // A thread per block from 256 blocks an SM on (SiLU: 512); with fewer, four lanes a block
     // finish sooner (us by threads and by lanes: 18944 blocks 1.69 and 1.63, 37888 1.79 and 1.91,
-    // 151552 2.8 and 4.4; fp32 stays with four lanes, 8192 x 8192 46.7 us, the copy rate; SiLU 37888 3.6 and 3.3, 56832 4.1 and 4.1, 75776 4.6 and 4.8).
+    // 151552 2.8 and 4.4; fp32 stays with four lanes, 8192 x 8192 46.7 us, the copy rate; SiLU
+    // 37888 3.6 and 3.3, 56832 4.1 and 4.1, 75776 4.6 and 4.8).
     const int64_t total = a.vectors / 4;
     if (dtype != I8L_F32 && total >= (kSilu ? 512 : 256) * di.sms) {
       if (a.vec && reinterpret_cast<uintptr_t>(x) % 32 == 0 && (ldx * 2) % 32 == 0) a.vec = 2;

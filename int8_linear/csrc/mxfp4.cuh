@@ -13,12 +13,18 @@
 #pragma once
 
 #include "common.cuh"
+#include "internal.h"
 
 namespace i8l {
 
 constexpr int kMxBlock = 32;       // values per scale
 constexpr int kSfTileBytes = 512;  // 128 rows x 4 blocks
 constexpr int kMxMaxK = 1 << 26;   // 128 rows of eight-value vectors fit a 31-bit index
+
+// Whether a product reads its weight before the kernels before it are done: under programmatic
+// launch not where quant_mxfp4, for as few rows, may still be writing it.
+constexpr int kWeightRows = 128;
+inline bool mx_weight_early(int rows) { return rows >= kWeightRows || !pdl_enabled(); }
 
 // Byte offset of the word that holds the scales of blocks 4*kt .. 4*kt+3 of a row.
 __host__ __device__ __forceinline__ long long sf_word_offset(long long row, int kt, int ktiles) {

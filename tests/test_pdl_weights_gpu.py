@@ -25,7 +25,9 @@ def pdl():
 @pytest.mark.parametrize("between", ["nothing", "one", "several"])
 @pytest.mark.parametrize("m,n,k,cfg", [(2, 4096, 2048, Config(4, 0, split=5)), (16, 8192, 8192, None),
                                        (100, 8192, 4096, Config(128, 128, swap_ab=True, split=1)),
-                                       (600, 4096, 8192, Config(128, 256, split=4)), (2, 128, 256, Config(4, 0, split=5))])
+                                       (600, 4096, 8192, Config(128, 256, split=4)), (2, 128, 256, Config(4, 0, split=5)),
+                                       (2, 127, 4096, Config(4, 0, split=5)), (16, 100, 16384, None),
+                                       (300, 127, 8192, Config(128, 256, split=4))])
 def test_weight_quantised_just_before_its_product(m, n, k, cfg, between, pdl):
     """The weight's buffers hold another weight's codes from the turn before (the allocator
     hands them out again), so that a product that reads them too early differs."""
