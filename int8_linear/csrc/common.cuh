@@ -27,7 +27,7 @@ enum StatusBits : int {
 
 // A wait that should take microseconds gives up after this many nanoseconds
 // (a broken pipeline then ends the kernel with a status bit set instead of
-// hanging the GPU).
+// hanging the GPU), or after twice as many where the first ran out (mbar_wait_bounded).
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
 
 __device__ __forceinline__ unsigned long long globaltimer_ns() {
